@@ -355,6 +355,127 @@ int rbt_model_decode_batch(RbtModel *m, const int32_t *tokens, const int32_t *po
 int rbt_model_set_router_bias(RbtModel *m, int layer, const float *bias);
 RbtMoe *rbt_model_moe(RbtModel *m);
 
+/* ---- A paged KV cache (serving requests of different lengths; no counterpart in the
+ * reference, whose State holds one sequence, rabbit2.c:101-106) ----
+ * The positions of a sequence live in pages of page_size positions, taken from one
+ * pool; row i of a block table lists sequence i's pages in order.  A step of a
+ * server is: rbt_paged_release_device (pages of finished requests back to the free
+ * list), rbt_paged_plan_device (pages and slots for the step's new tokens), then per
+ * layer rbt_paged_append_device (QK-norm, RoPE, k and v into their slots) and
+ * rbt_paged_attention_device (every new token over its sequence's positions).
+ *
+ * Layouts, all row-major: k and v of a layer are [n_pages][n_kv_heads][page_size]
+ * [head_dim]; a slot is page * page_size + offset; the new tokens of a step are rows
+ * one after the other, those of sequence i at d_cu[i] .. d_cu[i+1]; the heads of a
+ * token's q, k, v or output row are contiguous, rows are *_stride elements apart.
+ *
+ * Every call is enqueued on `stream` (NULL = the default stream) of the context's
+ * device without synchronising, allocates nothing and can be captured into a CUDA
+ * graph; the calling thread's current device is left as it was.  Pointers are device
+ * pointers on the context's device.  The attention keeps partial results in the
+ * context: two attention calls of one context whose kernels overlap on the GPU
+ * (unordered streams, two graphs in flight) race on them; create a second context
+ * over the same caches for that.  The other calls keep nothing.
+ *
+ * What only the kernels can see (lengths, pages, slots) is checked there, never
+ * followed out of bounds, and leaves a code in the context's status word, which
+ * rbt_paged_status returns: 0x801 too few free pages, 0x802 a table row too narrow,
+ * 0x803 more new tokens than rows, 0x804 a negative length or count, 0x805 the free
+ * list is full, 0x806 a table or free-list entry that is no page, 0x811 a slot
+ * outside the cache, 0x812 a position outside the angle tables, 0x821 row offsets
+ * outside the rows, 0x822 a length that its table row does not hold, 0x823 a table
+ * entry that is no page, 0x824 a bounded wait that ran out. */
+#define RBT_PAGED_MAX_SEQ 2048  /* sequences per call */
+
+typedef struct RbtPagedConfig {
+    int32_t n_layers;    /* caches to bind (rbt_paged_bind_layer); 0: block tables only, the heads unused */
+    int32_t n_heads, n_kv_heads, head_dim; /* head_dim 64 or 128; n_heads a multiple of n_kv_heads */
+    int32_t page_size;   /* a power of two, 8 .. 256 */
+    int32_t n_pages;     /* pages of the pool, the same for every layer */
+    int32_t dtype;       /* of the caches, and of q and the output of the attention */
+} RbtPagedConfig;
+
+typedef struct RbtPaged RbtPaged; /* opaque: the attention's workspace, the status word, bound caches */
+
+int rbt_paged_create(RbtPaged **out, const RbtPagedConfig *cfg, int device);
+void rbt_paged_destroy(RbtPaged *p);
+
+/* Bind layer `layer`'s caches: device memory the caller owns and keeps alive, 16-byte
+ * aligned. */
+int rbt_paged_bind_layer(RbtPaged *p, int layer, void *d_k, void *d_v);
+
+/* The status word (0: nothing went wrong), cleared after reading; synchronises the
+ * device. */
+int rbt_paged_status(RbtPaged *p, unsigned *status_out);
+
+/* The pages of the sequences with d_done[i] != 0 go behind the first d_n_free[0]
+ * entries of the free list d_free [free_cap], sequence by sequence, block by block;
+ * d_n_free_out[0] is the new count, d_len_out[i] is 0 for those sequences and
+ * d_len[i] for the others.  On an error (0x804, 0x805) no page moves and the outputs
+ * repeat the inputs.  The outputs must not overlap the inputs. */
+int rbt_paged_release_device(RbtPaged *p, int n_seq, const int32_t *d_len, const int32_t *d_done,
+                             const int32_t *d_table, int table_stride, int32_t *d_free, int free_cap,
+                             const int32_t *d_n_free, int32_t *d_len_out, int32_t *d_n_free_out, void *stream);
+
+/* d_new[i] >= 0 new tokens for each sequence of d_len[i] positions: the pages they
+ * need beyond those the sequence holds are taken from the end of the free list
+ * (d_free[d_n_free[0] - 1] first), sequence by sequence, and written into d_table.
+ * d_len_out[i] = d_len[i] + d_new[i]; d_n_free_out[0] the pages left; d_cu [n_seq+1]
+ * the rows of each sequence; for every row of the new tokens its slot and position.
+ * Rows n_tokens .. n_rows (the padding of a step of fixed size) get slot -1 and
+ * position 0.  On an error (0x801 .. 0x804) nothing is taken: the table stays, the
+ * lengths and the count repeat the inputs, d_cu is all 0 and every slot -1.  The
+ * outputs must not overlap the inputs. */
+int rbt_paged_plan_device(RbtPaged *p, int n_seq, const int32_t *d_len, const int32_t *d_new, int32_t *d_table,
+                          int table_stride, const int32_t *d_free, const int32_t *d_n_free, int n_rows,
+                          int32_t *d_len_out, int32_t *d_n_free_out, int32_t *d_cu, int64_t *d_slot, int32_t *d_pos,
+                          void *stream);
+
+/* k and v of n_rows tokens into the slots of layer `layer`, and q for the attention:
+ * whole-projection QK-norm when d_q_norm/d_k_norm are given (rabbit2.c:477-480), RoPE
+ * at d_pos when d_cos/d_sin [rope_len][head_dim/2] are given (:481-482, pairs (i, i +
+ * head_dim/2)), each result rounded once to the cache's type.  q, k, v are of
+ * src_dtype; q_out, of the cache's type, may be the q rows themselves when the types
+ * and strides are equal.  A row with a negative slot is padding: nothing is read or
+ * written for it.  The slots of a call must be distinct.  All rows 16-byte aligned. */
+typedef struct RbtPagedAppend {
+    const void *d_q, *d_k, *d_v;
+    int64_t q_stride, k_stride, v_stride; /* elements between rows */
+    int32_t src_dtype, n_rows;
+    const int64_t *d_slot;                /* [n_rows] */
+    const int32_t *d_pos;                 /* [n_rows]; may be NULL without RoPE */
+    const float *d_q_norm, *d_k_norm;     /* [n_heads*head_dim], [n_kv_heads*head_dim], or both NULL */
+    float eps;
+    int32_t rope_len;
+    const float *d_cos, *d_sin;           /* or both NULL */
+    void *d_q_out;
+    int64_t q_out_stride;
+} RbtPagedAppend;
+int rbt_paged_append_device(RbtPaged *p, int layer, const RbtPagedAppend *a, void *stream);
+
+/* Attention of every new token: row r of sequence i stands at position
+ * d_len[i] - (d_cu[i+1] - d_cu[i]) + (r - d_cu[i]) and sees the cached positions up
+ * to its own (causal), of those the last `window` (window > 0); causal == 0 shows it
+ * all d_len[i] positions (window must be 0 then).  d_len counts the new tokens.
+ *   out = softmax(scale q . k) v,   lse = ln sum exp(scale q . k)
+ * A row that sees nothing gets zeros and lse -inf.  Rows before d_cu[0] and from
+ * d_cu[n_seq] on are left as they were.  max_new is the caller's upper bound of the
+ * sequences' new tokens; it only chooses among the kernels (a larger count is
+ * computed all the same).  d_lse [n_rows][n_heads] f32 may be NULL.  f32: products and
+ * sums in f32.  bf16: exact products with f32 sums, the softmax in f32, its weights
+ * rounded to bf16 for the product with v.  q and out must not overlap the caches. */
+typedef struct RbtPagedAttention {
+    const void *d_q;
+    void *d_out;
+    float *d_lse;
+    int64_t q_stride, out_stride;  /* elements between rows */
+    int32_t n_rows, n_seq, max_new;
+    const int32_t *d_cu, *d_len, *d_table;
+    int32_t table_stride, causal, window;
+    float scale;
+} RbtPagedAttention;
+int rbt_paged_attention_device(RbtPaged *p, int layer, const RbtPagedAttention *a, void *stream);
+
 /* Last error message of the calling thread ("" if none). */
 const char *rbt_moe_last_error(void);
 

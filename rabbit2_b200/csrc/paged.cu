@@ -1,0 +1,373 @@
+// paged.cu -- the C ABI of the paged KV cache (rbt_paged_*): the context, the checks of
+// arguments and the launches.  The kernels are in paged_tables.cu and paged_attn*.cu.
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdarg.h>
+#include <stdio.h>
+
+#include <new>
+#include <vector>
+
+#include "../../include/rbt_moe.h"
+#include "kernels.h"
+#include "paged.h"
+
+namespace rbt {
+void set_last_error(const char* msg);
+}
+
+struct RbtPaged {
+    RbtPagedConfig cfg{};
+    int device = 0, sm_count = 0, page_shift = 0;
+    struct Layer {
+        void *k = nullptr, *v = nullptr;
+    };
+    std::vector<Layer> layers;
+    unsigned* status = nullptr;
+    float* part = nullptr;          // partial tiles of the attention
+    rbt::PagedJoin* join = nullptr;
+};
+
+namespace {
+
+using namespace rbt;
+
+int fail(const char* fmt, ...) __attribute__((format(printf, 1, 2)));
+int fail(const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    fprintf(stderr, "rbt_paged: %s\n", buf);
+    set_last_error(buf);
+    return 0;
+}
+
+#define CU(call)                                                                                  \
+    do {                                                                                          \
+        cudaError_t e_ = (call);                                                                  \
+        if (e_ != cudaSuccess) return fail("%s failed: %s (%s:%d)", #call, cudaGetErrorString(e_), \
+                                           __FILE__, __LINE__);                                   \
+    } while (0)
+
+// The context's device for the calls of one entry point; the caller's afterwards.
+struct OnDevice {
+    int before = -1;
+    cudaError_t err;
+    explicit OnDevice(int device) {
+        err = cudaGetDevice(&before);
+        if (err == cudaSuccess && before == device) before = -1;
+        else if (err == cudaSuccess) err = cudaSetDevice(device);
+    }
+    ~OnDevice() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+#define ON_DEVICE(p)              \
+    OnDevice on_device_(p->device); \
+    CU(on_device_.err)
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return na && nb && x < y + nb && y < x + na;
+}
+
+int check_seqs(const RbtPaged* p, int n_seq, int table_stride) {
+    if (!p) return fail("null context");
+    if (n_seq < 0 || n_seq > RBT_PAGED_MAX_SEQ) return fail("n_seq %d outside [0, %d]", n_seq, RBT_PAGED_MAX_SEQ);
+    if (table_stride < 0) return fail("table_stride must be >= 0 (got %d)", table_stride);
+    return 1;
+}
+
+int check_layer(const RbtPaged* p, int layer) {
+    if (!p) return fail("null context");
+    if (layer < 0 || layer >= p->cfg.n_layers) return fail("layer %d out of range [0, %d)", layer, p->cfg.n_layers);
+    if (!p->layers[layer].k) return fail("layer %d has no caches (rbt_paged_bind_layer)", layer);
+    return 1;
+}
+
+size_t esize(int dtype) { return dtype == RBT_MOE_DT_BF16 ? 2 : 4; }
+
+// rows of `width` elements, stride elements apart, 16-byte aligned
+int check_rows(const char* name, const void* ptr, int64_t stride, int width, int dtype) {
+    if (!ptr) return fail("null %s", name);
+    if (stride < width) return fail("%s rows of %d elements with a stride of %lld", name, width, (long long)stride);
+    if (!aligned16(ptr) || stride * esize(dtype) % 16) return fail("%s rows must be 16-byte aligned", name);
+    return 1;
+}
+
+int attn_ctas(const RbtPaged* p) { return p->sm_count * 2; }
+
+}  // namespace
+
+extern "C" {
+
+int rbt_paged_create(RbtPaged** out, const RbtPagedConfig* cfg, int device) {
+    if (!out || !cfg) return fail("null argument");
+    *out = nullptr;
+    const RbtPagedConfig& c = *cfg;
+    if (c.n_layers < 0) return fail("n_layers must be >= 0 (got %d)", c.n_layers);
+    if (c.page_size < 8 || c.page_size > 256 || (c.page_size & (c.page_size - 1)))
+        return fail("page_size %d must be a power of two in [8, 256]", c.page_size);
+    if (c.n_pages <= 0) return fail("n_pages must be positive (got %d)", c.n_pages);
+    if (c.n_layers > 0) {
+        if (c.dtype != RBT_MOE_DT_F32 && c.dtype != RBT_MOE_DT_BF16) return fail("dtype must be 0 (f32) or 1 (bf16)");
+        if (c.head_dim != 64 && c.head_dim != 128) return fail("head_dim %d must be 64 or 128", c.head_dim);
+        if (c.n_heads <= 0 || c.n_kv_heads <= 0 || c.n_heads % c.n_kv_heads)
+            return fail("n_heads %d is not a multiple of n_kv_heads %d", c.n_heads, c.n_kv_heads);
+        if (c.n_heads > 1024) return fail("n_heads %d above the supported 1024", c.n_heads);
+        if ((int64_t)c.n_pages * c.n_kv_heads * c.page_size > INT32_MAX)
+            return fail("n_pages %d * n_kv_heads %d * page_size %d exceeds 2^31 - 1 rows", c.n_pages, c.n_kv_heads,
+                        c.page_size);
+    }
+    int ndev = 0;
+    CU(cudaGetDeviceCount(&ndev));
+    if (device < 0 || device >= ndev) return fail("device %d out of range (%d visible)", device, ndev);
+    OnDevice on(device);
+    CU(on.err);
+    RbtPaged* p = new (std::nothrow) RbtPaged();
+    if (!p) return fail("out of host memory");
+    p->cfg = c;
+    p->device = device;
+    while ((1 << p->page_shift) < c.page_size) p->page_shift++;
+    try {
+        p->layers.resize(c.n_layers);
+    } catch (...) {
+        delete p;
+        return fail("out of host memory");
+    }
+    cudaError_t e = cudaDeviceGetAttribute(&p->sm_count, cudaDevAttrMultiProcessorCount, device);
+    if (e == cudaSuccess) e = cudaMalloc((void**)&p->status, sizeof(unsigned));
+    if (e == cudaSuccess) e = cudaMemset(p->status, 0, sizeof(unsigned));
+    if (e == cudaSuccess && c.n_layers > 0) {
+        const size_t tile = (size_t)64 * (2 + c.head_dim) * sizeof(float);
+        e = cudaMalloc((void**)&p->part, (size_t)attn_ctas(p) * 2 * tile);
+        if (e == cudaSuccess) e = cudaMalloc((void**)&p->join, (size_t)attn_ctas(p) * sizeof(PagedJoin));
+    }
+    if (e != cudaSuccess) {
+        rbt_paged_destroy(p);
+        return fail("cannot set up the paged context: %s", cudaGetErrorString(e));
+    }
+    *out = p;
+    return 1;
+}
+
+void rbt_paged_destroy(RbtPaged* p) {
+    if (!p) return;
+    OnDevice on(p->device);
+    cudaFree(p->status);
+    cudaFree(p->part);
+    cudaFree(p->join);
+    delete p;
+}
+
+int rbt_paged_bind_layer(RbtPaged* p, int layer, void* d_k, void* d_v) {
+    if (!p) return fail("null context");
+    if (layer < 0 || layer >= p->cfg.n_layers) return fail("layer %d out of range [0, %d)", layer, p->cfg.n_layers);
+    if (!d_k || !d_v) return fail("null cache pointer");
+    if (!aligned16(d_k) || !aligned16(d_v)) return fail("the caches must be 16-byte aligned");
+    p->layers[layer].k = d_k;
+    p->layers[layer].v = d_v;
+    return 1;
+}
+
+int rbt_paged_status(RbtPaged* p, unsigned* status_out) {
+    if (!p || !status_out) return fail("null argument");
+    ON_DEVICE(p);
+    CU(cudaDeviceSynchronize());
+    CU(cudaMemcpy(status_out, p->status, sizeof(unsigned), cudaMemcpyDeviceToHost));
+    if (*status_out) CU(cudaMemset(p->status, 0, sizeof(unsigned)));
+    return 1;
+}
+
+int rbt_paged_release_device(RbtPaged* p, int n_seq, const int32_t* d_len, const int32_t* d_done,
+                             const int32_t* d_table, int table_stride, int32_t* d_free, int free_cap,
+                             const int32_t* d_n_free, int32_t* d_len_out, int32_t* d_n_free_out, void* stream) {
+    if (!check_seqs(p, n_seq, table_stride)) return 0;
+    if (free_cap < 0) return fail("free_cap must be >= 0 (got %d)", free_cap);
+    if (!d_n_free || !d_n_free_out || (n_seq && (!d_len || !d_done || !d_len_out)) ||
+        (n_seq && table_stride && !d_table) || (free_cap && !d_free))
+        return fail("null pointer");
+    const size_t n4 = (size_t)n_seq * 4;
+    if (overlap(d_len_out, n4, d_len, n4) || overlap(d_len_out, n4, d_done, n4) || overlap(d_n_free_out, 4, d_n_free, 4))
+        return fail("the outputs must not overlap the inputs");
+    ON_DEVICE(p);
+    PagedTablesArgs a{};
+    a.page_shift = p->page_shift;
+    a.n_pages = p->cfg.n_pages;
+    a.n_seq = n_seq;
+    a.table_stride = table_stride;
+    a.len = d_len;
+    a.count = d_done;
+    a.table = const_cast<int32_t*>(d_table);
+    a.free_list = d_free;
+    a.free_cap = free_cap;
+    a.n_free = d_n_free;
+    a.len_out = d_len_out;
+    a.n_free_out = d_n_free_out;
+    a.status = p->status;
+    CU(launch_paged_release(a, p->sm_count, (cudaStream_t)stream));
+    return 1;
+}
+
+int rbt_paged_plan_device(RbtPaged* p, int n_seq, const int32_t* d_len, const int32_t* d_new, int32_t* d_table,
+                          int table_stride, const int32_t* d_free, const int32_t* d_n_free, int n_rows,
+                          int32_t* d_len_out, int32_t* d_n_free_out, int32_t* d_cu, int64_t* d_slot, int32_t* d_pos,
+                          void* stream) {
+    if (!check_seqs(p, n_seq, table_stride)) return 0;
+    if (n_rows < 0) return fail("n_rows must be >= 0 (got %d)", n_rows);
+    if (!d_n_free || !d_n_free_out || !d_free || !d_cu || (n_seq && (!d_len || !d_new || !d_len_out)) ||
+        (n_seq && table_stride && !d_table) || (n_rows && (!d_slot || !d_pos)))
+        return fail("null pointer");
+    const size_t n4 = (size_t)n_seq * 4;
+    if (overlap(d_len_out, n4, d_len, n4) || overlap(d_len_out, n4, d_new, n4) ||
+        overlap(d_n_free_out, 4, d_n_free, 4) || overlap(d_cu, n4 + 4, d_len, n4) || overlap(d_cu, n4 + 4, d_new, n4))
+        return fail("the outputs must not overlap the inputs");
+    ON_DEVICE(p);
+    PagedTablesArgs a{};
+    a.page_shift = p->page_shift;
+    a.n_pages = p->cfg.n_pages;
+    a.n_seq = n_seq;
+    a.table_stride = table_stride;
+    a.len = d_len;
+    a.count = d_new;
+    a.table = d_table;
+    a.free_list = const_cast<int32_t*>(d_free);
+    a.n_free = d_n_free;
+    a.n_rows = n_rows;
+    a.len_out = d_len_out;
+    a.n_free_out = d_n_free_out;
+    a.cu = d_cu;
+    a.slot = d_slot;
+    a.pos = d_pos;
+    a.status = p->status;
+    CU(launch_paged_plan(a, p->sm_count, (cudaStream_t)stream));
+    return 1;
+}
+
+int rbt_paged_append_device(RbtPaged* p, int layer, const RbtPagedAppend* args, void* stream) {
+    if (!check_layer(p, layer)) return 0;
+    if (!args) return fail("null argument");
+    const RbtPagedAppend& x = *args;
+    const RbtPagedConfig& c = p->cfg;
+    if (x.n_rows < 0) return fail("n_rows must be >= 0 (got %d)", x.n_rows);
+    if (x.src_dtype != RBT_MOE_DT_F32 && x.src_dtype != RBT_MOE_DT_BF16)
+        return fail("src_dtype must be 0 (f32) or 1 (bf16)");
+    if (x.n_rows == 0) return 1;
+    const int nq = c.n_heads * c.head_dim, nkv = c.n_kv_heads * c.head_dim;
+    if (!check_rows("q", x.d_q, x.q_stride, nq, x.src_dtype) || !check_rows("k", x.d_k, x.k_stride, nkv, x.src_dtype) ||
+        !check_rows("v", x.d_v, x.v_stride, nkv, x.src_dtype) ||
+        !check_rows("q_out", x.d_q_out, x.q_out_stride, nq, c.dtype))
+        return 0;
+    if (!x.d_slot) return fail("null slots");
+    if (!x.d_q_norm != !x.d_k_norm) return fail("q_norm and k_norm must both be given or both be NULL");
+    if (!x.d_cos != !x.d_sin) return fail("cos and sin must both be given or both be NULL");
+    if (x.d_cos && (!x.d_pos || x.rope_len <= 0)) return fail("RoPE needs positions and rope_len > 0");
+    // in place only row by row, element by element; any other overlap would race
+    const size_t es = esize(x.src_dtype), eo = esize(c.dtype);
+    const auto span = [&](int64_t stride, int width, size_t e) { return ((size_t)(x.n_rows - 1) * stride + width) * e; };
+    const size_t n_out = span(x.q_out_stride, nq, eo);
+    const bool in_place = x.d_q_out == x.d_q && x.q_out_stride == x.q_stride && x.src_dtype == c.dtype;
+    if (!in_place && overlap(x.d_q_out, n_out, x.d_q, span(x.q_stride, nq, es)))
+        return fail("q_out overlaps q (in place needs the same type, address and stride)");
+    const auto rows_apart = [&](const void* b, int64_t stride) {  // both inside one row of the same stride, side by side
+        if (stride != x.q_out_stride || es != eo) return false;
+        const intptr_t d = reinterpret_cast<intptr_t>(b) - reinterpret_cast<intptr_t>(x.d_q_out);
+        const intptr_t row = (intptr_t)stride * (intptr_t)es, off = ((d % row) + row) % row;
+        return off >= nq * (intptr_t)es && off + nkv * (intptr_t)es <= row;
+    };
+    if ((overlap(x.d_q_out, n_out, x.d_k, span(x.k_stride, nkv, es)) && !rows_apart(x.d_k, x.k_stride)) ||
+        (overlap(x.d_q_out, n_out, x.d_v, span(x.v_stride, nkv, es)) && !rows_apart(x.d_v, x.v_stride)))
+        return fail("q_out overlaps k or v");
+    ON_DEVICE(p);
+    PagedAppendArgs a{};
+    a.q = x.d_q;
+    a.k = x.d_k;
+    a.v = x.d_v;
+    a.q_stride = x.q_stride;
+    a.k_stride = x.k_stride;
+    a.v_stride = x.v_stride;
+    a.n_rows = x.n_rows;
+    a.n_heads = c.n_heads;
+    a.n_kv = c.n_kv_heads;
+    a.hd = c.head_dim;
+    a.page_shift = p->page_shift;
+    a.n_slots = (int64_t)c.n_pages << p->page_shift;
+    a.slot = x.d_slot;
+    a.pos = x.d_pos;
+    a.q_norm = x.d_q_norm;
+    a.k_norm = x.d_k_norm;
+    a.eps = x.eps;
+    a.rope_len = x.rope_len;
+    a.cos = x.d_cos;
+    a.sin = x.d_sin;
+    a.q_out = x.d_q_out;
+    a.q_out_stride = x.q_out_stride;
+    a.kc = p->layers[layer].k;
+    a.vc = p->layers[layer].v;
+    a.status = p->status;
+    CU(launch_paged_append(x.src_dtype, c.dtype, a, (cudaStream_t)stream));
+    return 1;
+}
+
+int rbt_paged_attention_device(RbtPaged* p, int layer, const RbtPagedAttention* args, void* stream) {
+    if (!check_layer(p, layer)) return 0;
+    if (!args) return fail("null argument");
+    const RbtPagedAttention& x = *args;
+    const RbtPagedConfig& c = p->cfg;
+    if (!check_seqs(p, x.n_seq, x.table_stride)) return 0;
+    if (x.n_rows < 0 || x.max_new < 0) return fail("n_rows and max_new must be >= 0");
+    if (x.window < 0) return fail("window must be >= 0 (got %d)", x.window);
+    if (x.window && !x.causal) return fail("a window needs causal");
+    if (!isfinite(x.scale)) return fail("scale must be finite");
+    if (x.n_rows == 0 || x.n_seq == 0) return 1;
+    const int nq = c.n_heads * c.head_dim;
+    if (!check_rows("q", x.d_q, x.q_stride, nq, c.dtype) || !check_rows("out", x.d_out, x.out_stride, nq, c.dtype))
+        return 0;
+    if (!x.d_cu || !x.d_len || (x.table_stride && !x.d_table)) return fail("null pointer");
+    if ((int64_t)x.n_rows * (c.n_heads / c.n_kv_heads) > INT32_MAX - 256)
+        return fail("n_rows %d * the heads of a kv head exceeds 31 bits", x.n_rows);
+    const size_t e = esize(c.dtype);
+    if (overlap(x.d_q, ((size_t)(x.n_rows - 1) * x.q_stride + nq) * e, x.d_out,
+                ((size_t)(x.n_rows - 1) * x.out_stride + nq) * e))
+        return fail("out overlaps q");
+    ON_DEVICE(p);
+    PagedAttnArgs a{};
+    a.q = x.d_q;
+    a.k = p->layers[layer].k;
+    a.v = p->layers[layer].v;
+    a.out = x.d_out;
+    a.lse = x.d_lse;
+    a.q_stride = x.q_stride;
+    a.out_stride = x.out_stride;
+    a.cu = x.d_cu;
+    a.len = x.d_len;
+    a.table = x.d_table;
+    a.table_stride = x.table_stride;
+    a.n_rows = x.n_rows;
+    a.n_seq = x.n_seq;
+    a.n_heads = c.n_heads;
+    a.n_kv = c.n_kv_heads;
+    a.group = c.n_heads / c.n_kv_heads;
+    a.page_shift = p->page_shift;
+    a.n_pages = c.n_pages;
+    a.causal = x.causal;
+    a.window = x.window;
+    a.scale = x.scale;
+    a.part = p->part;
+    a.join = p->join;
+    a.status = p->status;
+    a.rows_lo = 0;
+    a.rows_hi = INT32_MAX;
+    cudaStream_t s = (cudaStream_t)stream;
+    const int ctas = attn_ctas(p);
+    CU(launch_paged_attn_rows(c.dtype, c.head_dim, a, ctas, s));
+    CU(launch_paged_join(c.dtype, c.head_dim, 64, a, ctas, s));
+    return 1;
+}
+
+}  // extern "C"

@@ -1,0 +1,95 @@
+// paged.h -- internal interface of the paged KV cache's kernels (not part of the C ABI).
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace rbt {
+
+// codes of the status word (include/rbt_moe.h lists them)
+enum PagedStatus : unsigned {
+    kPagedNoPages = 0x801,
+    kPagedNarrow = 0x802,
+    kPagedRows = 0x803,
+    kPagedNegative = 0x804,
+    kPagedFreeFull = 0x805,
+    kPagedPage = 0x806,
+    kPagedSlot = 0x811,
+    kPagedPos = 0x812,
+    kPagedCu = 0x821,
+    kPagedLen = 0x822,
+    kPagedTable = 0x823,
+    kPagedWait = 0x824,
+};
+
+constexpr int kPagedMaxSeq = 2048;
+constexpr int kPagedMaxCtas = 1024;  // CTAs of one attention launch (an entry of PagedJoin each)
+
+// The tile that CTA c begins and others finish: its partial results are in slot 1 of CTA c
+// and slot 0 of CTAs c+1 .. last.  last == c: none.
+struct PagedJoin {
+    int last;
+    int row0, n_rows;   // first packed row of the tile, and how many
+    int tok0, kvh;      // row of the sequence's first token, kv head
+};
+
+struct PagedAttnArgs {
+    const void *q, *k, *v;
+    void* out;
+    float* lse;
+    long q_stride, out_stride;
+    const int32_t *cu, *len, *table;
+    int table_stride, n_rows, n_seq, n_heads, n_kv, group;
+    int page_shift, n_pages;
+    int causal, window;
+    int rows_lo, rows_hi;  // sequences with rows_lo < new tokens * group <= rows_hi are this launch's
+    float scale;
+    float* part;           // [ctas][2] partial tiles: max[rows], sum[rows], o[rows][head_dim]
+    PagedJoin* join;       // [ctas]
+    unsigned* status;
+};
+
+// One attention launch of up to `ctas` CTAs, its partial tiles and its joins.
+struct PagedAttnPlan {
+    int ctas;
+    int tile_rows;
+};
+
+cudaError_t launch_paged_attn_rows(int dtype, int hd, const PagedAttnArgs& a, int ctas, cudaStream_t s);
+cudaError_t launch_paged_join(int dtype, int hd, int tile_rows, const PagedAttnArgs& a, int ctas, cudaStream_t s);
+
+struct PagedTablesArgs {
+    int page_shift, n_pages, n_seq, table_stride;
+    const int32_t *len, *count;  // count: new tokens (plan) or done flags (release)
+    int32_t *table, *free_list;
+    int free_cap;
+    const int32_t* n_free;
+    int n_rows;
+    int32_t *len_out, *n_free_out, *cu;
+    int64_t* slot;
+    int32_t* pos;
+    unsigned* status;
+};
+cudaError_t launch_paged_plan(const PagedTablesArgs& a, int sm_count, cudaStream_t s);
+cudaError_t launch_paged_release(const PagedTablesArgs& a, int sm_count, cudaStream_t s);
+
+struct PagedAppendArgs {
+    const void *q, *k, *v;
+    long q_stride, k_stride, v_stride;
+    int n_rows, n_heads, n_kv, hd, page_shift;
+    int64_t n_slots;
+    const int64_t* slot;
+    const int32_t* pos;
+    const float *q_norm, *k_norm;
+    float eps;
+    int rope_len;
+    const float *cos, *sin;
+    void* q_out;
+    long q_out_stride;
+    void *kc, *vc;
+    unsigned* status;
+};
+cudaError_t launch_paged_append(int src_dtype, int dtype, const PagedAppendArgs& a, cudaStream_t s);
+
+}  // namespace rbt

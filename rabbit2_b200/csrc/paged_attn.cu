@@ -1,0 +1,322 @@
+// paged_attn.cu -- attention over a paged KV cache: the CUDA-core kernel and the
+// kernel that joins the parts of tiles shared by several CTAs.
+//
+//   o_r = sum_p exp(x_rp - m_r) v_p / l_r,  x_rp = scale q_r . k_p,
+//   m_r = max_p x_rp, l_r = sum_p exp(x_rp - m_r), lse_r = m_r + ln l_r
+// over the positions p that row r sees, in one pass over them: m, l and o are
+// running values, rescaled when a block of positions raises m.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "../../include/rbt_moe.h"
+#include "common.cuh"
+#include "paged.h"
+#include "paged_sched.cuh"
+
+namespace rbt {
+namespace {
+
+using namespace paged;
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void store4(float* p, const float (&f)[4]) {
+    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+}
+__device__ __forceinline__ void store4(uint16_t* p, const float (&f)[4]) {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(f[0], f[1]), y = __floats2bfloat162_rn(f[2], f[3]);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+}
+
+// ---------------------------------------------------------------- rows kernel
+// 16 x 16 threads: thread (ty, tx) owns rows ty kRM .. + kRM, score columns tx + 16 j and
+// output dims 4 tx + 64 k.
+constexpr int kRowsThreads = 256;
+
+template <int HD>
+struct RowsCfg {
+    static constexpr int kRM = 4, kRows = 16 * kRM;
+    static constexpr int kKN = HD == 64 ? 4 : 2, kBlock = 16 * kKN;
+    static constexpr int kLd = HD + 4, kLdP = kBlock + 4;
+    static constexpr int kFloats = kRows * kLd + 2 * kBlock * kLd + kRows * kLdP;
+    static constexpr int kPart = kRows * (2 + HD);  // floats of one partial tile
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedAttnArgs a) {
+    using C = RowsCfg<HD>;
+    constexpr int RM = C::kRM, KN = C::kKN, KB = C::kBlock, LD = C::kLd, LDP = C::kLdP, DV = HD / 64;
+    constexpr int V = WeightTraits<T>::kVec, CH = HD / V;
+    extern __shared__ __align__(16) float sm[];
+    float* Qs = sm;
+    float* Ks = Qs + C::kRows * LD;
+    float* Vs = Ks + KB * LD;
+    float* Ps = Vs + KB * LD;
+    int* starts = reinterpret_cast<int*>(sm + C::kFloats);
+    __shared__ Share share;
+    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    find_share<kRowsThreads, C::kRows, KB, 4>(a, starts, &share);
+    Walk<C::kRows, KB> w(share, starts);
+    if (tid == 0) a.join[blockIdx.x].last = blockIdx.x;
+    const float k2 = a.scale * kLog2e;
+    const int page = 1 << a.page_shift;
+    while (w.next(a)) {
+        const Tile& t = w.t;
+        for (int e = tid; e < C::kRows * CH; e += kRowsThreads) {
+            const int r = e / CH, c = (e - r * CH) * V;
+            float f[V];
+            if (r < t.rows) {
+                const int tok = (t.r0 + r) / a.group, g = (t.r0 + r) - tok * a.group;
+                const T* src = static_cast<const T*>(a.q) + (t.s.row0 + tok) * a.q_stride +
+                               (size_t)(t.kvh * a.group + g) * HD + c;
+                WeightTraits<T>::unpack(*reinterpret_cast<const uint4*>(src), f);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; i++) f[i] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < V; i++) Qs[r * LD + c + i] = f[i];
+        }
+        int from[RM], to[RM];  // positions [from, to) that the thread's rows see
+        float m[RM], l[RM];
+        float4 o[RM][DV];
+#pragma unroll
+        for (int i = 0; i < RM; i++) {
+            const int r = ty * RM + i, pos = t.off + (t.r0 + r) / a.group;
+            to[i] = r >= t.rows ? 0 : a.causal ? min(t.s.len, pos + 1) : t.s.len;
+            from[i] = a.window ? max(0, pos - a.window + 1) : 0;
+            m[i] = -INFINITY;
+            l[i] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < DV; k++) o[i][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        const int32_t* table = a.table + (size_t)t.seq * a.table_stride;
+        for (int b = w.first; b < w.first + w.n; b++) {
+            const int p0 = b * KB;
+            __syncthreads();  // the block before is consumed (and Qs written, on the first pass)
+            for (int e = tid; e < KB * CH; e += kRowsThreads) {
+                const int r = e / CH, c = (e - r * CH) * V, p = p0 + r;
+                float fk[V], fv[V];
+#pragma unroll
+                for (int i = 0; i < V; i++) fk[i] = fv[i] = 0.0f;
+                if (p < t.hi) {
+                    const int id = table[p >> a.page_shift];
+                    if ((unsigned)id < (unsigned)a.n_pages) {
+                        const size_t at = ((((size_t)id * a.n_kv + t.kvh) << a.page_shift) + (p & (page - 1))) * HD + c;
+                        WeightTraits<T>::unpack(ld_stream16(static_cast<const T*>(a.k) + at), fk);
+                        WeightTraits<T>::unpack(ld_stream16(static_cast<const T*>(a.v) + at), fv);
+                    } else {
+                        atomicCAS(a.status, 0u, (unsigned)kPagedTable);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    Ks[r * LD + c + i] = fk[i];
+                    Vs[r * LD + c + i] = fv[i];
+                }
+            }
+            __syncthreads();
+            float s[RM][KN];
+#pragma unroll
+            for (int i = 0; i < RM; i++)
+#pragma unroll
+                for (int j = 0; j < KN; j++) s[i][j] = 0.0f;
+#pragma unroll 4
+            for (int c = 0; c < HD; c += 4) {
+                float4 q4[RM], k4[KN];
+#pragma unroll
+                for (int i = 0; i < RM; i++) q4[i] = *reinterpret_cast<const float4*>(Qs + (ty * RM + i) * LD + c);
+#pragma unroll
+                for (int j = 0; j < KN; j++) k4[j] = *reinterpret_cast<const float4*>(Ks + (tx + 16 * j) * LD + c);
+#pragma unroll
+                for (int i = 0; i < RM; i++)
+#pragma unroll
+                    for (int j = 0; j < KN; j++) {
+                        s[i][j] = fmaf(q4[i].x, k4[j].x, s[i][j]);
+                        s[i][j] = fmaf(q4[i].y, k4[j].y, s[i][j]);
+                        s[i][j] = fmaf(q4[i].z, k4[j].z, s[i][j]);
+                        s[i][j] = fmaf(q4[i].w, k4[j].w, s[i][j]);
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < RM; i++) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < KN; j++) {
+                    const int p = p0 + tx + 16 * j;
+                    s[i][j] = p >= from[i] && p < to[i] ? s[i][j] * k2 : -INFINITY;
+                    top = fmaxf(top, s[i][j]);
+                }
+#pragma unroll
+                for (int d = 1; d < 16; d <<= 1) top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, d));
+                const float mn = fmaxf(m[i], top), base = mn == -INFINITY ? 0.0f : mn;  // (nothing seen yet)
+                const float alpha = ex2(m[i] - base);
+                float sum = 0.0f;
+#pragma unroll
+                for (int j = 0; j < KN; j++) {
+                    const float p = ex2(s[i][j] - base);
+                    Ps[(ty * RM + i) * LDP + tx + 16 * j] = p;
+                    sum += p;
+                }
+#pragma unroll
+                for (int d = 1; d < 16; d <<= 1) sum += __shfl_xor_sync(FULL_MASK, sum, d);
+                l[i] = l[i] * alpha + sum;
+                m[i] = mn;
+#pragma unroll
+                for (int k = 0; k < DV; k++) {
+                    o[i][k].x *= alpha;
+                    o[i][k].y *= alpha;
+                    o[i][k].z *= alpha;
+                    o[i][k].w *= alpha;
+                }
+            }
+            __syncwarp();  // the 16 threads of a row are lanes of one warp
+#pragma unroll 2
+            for (int c = 0; c < KB; c += 4) {
+                float4 p4[RM];
+#pragma unroll
+                for (int i = 0; i < RM; i++) p4[i] = *reinterpret_cast<const float4*>(Ps + (ty * RM + i) * LDP + c);
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+#pragma unroll
+                    for (int k = 0; k < DV; k++) {
+                        const float4 v4 = *reinterpret_cast<const float4*>(Vs + (c + e) * LD + 4 * tx + 64 * k);
+#pragma unroll
+                        for (int i = 0; i < RM; i++) {
+                            const float p = e == 0 ? p4[i].x : e == 1 ? p4[i].y : e == 2 ? p4[i].z : p4[i].w;
+                            o[i][k].x = fmaf(p, v4.x, o[i][k].x);
+                            o[i][k].y = fmaf(p, v4.y, o[i][k].y);
+                            o[i][k].z = fmaf(p, v4.z, o[i][k].z);
+                            o[i][k].w = fmaf(p, v4.w, o[i][k].w);
+                        }
+                    }
+            }
+            __syncwarp();
+        }
+        if (w.whole) {
+#pragma unroll
+            for (int i = 0; i < RM; i++) {
+                const int r = ty * RM + i;
+                if (r >= t.rows) continue;
+                const int tok = (t.r0 + r) / a.group, h = t.kvh * a.group + (t.r0 + r) - tok * a.group;
+                const float inv = l[i] > 0.0f || l[i] != l[i] ? 1.0f / l[i] : 0.0f;
+                T* dst = static_cast<T*>(a.out) + (t.s.row0 + tok) * a.out_stride + (size_t)h * HD;
+#pragma unroll
+                for (int k = 0; k < DV; k++) {
+                    const float f[4] = {o[i][k].x * inv, o[i][k].y * inv, o[i][k].z * inv, o[i][k].w * inv};
+                    store4(dst + 4 * tx + 64 * k, f);
+                }
+                if (a.lse && tx == 0)
+                    a.lse[(size_t)(t.s.row0 + tok) * a.n_heads + h] = l[i] == 0.0f ? -INFINITY : m[i] * kLn2 + logf(l[i]);
+            }
+        } else {
+            float* part = a.part + ((size_t)blockIdx.x * 2 + (w.head ? 1 : 0)) * C::kPart;
+#pragma unroll
+            for (int i = 0; i < RM; i++) {
+                const int r = ty * RM + i;
+                if (r >= t.rows) continue;
+                if (tx == 0) {
+                    part[r] = m[i];
+                    part[C::kRows + r] = l[i];
+                }
+#pragma unroll
+                for (int k = 0; k < DV; k++)
+                    *reinterpret_cast<float4*>(part + 2 * C::kRows + (size_t)r * HD + 4 * tx + 64 * k) = o[i][k];
+            }
+            if (w.head && tid == 0)
+                a.join[blockIdx.x] = PagedJoin{w.finisher(), t.r0, t.rows, t.s.row0, t.kvh};
+        }
+        __syncthreads();  // Qs is free
+    }
+}
+
+// ---------------------------------------------------------------- join
+// CTA c adds up the parts of the tile that attention CTA c began and others finished: a
+// warp per row, M = max m_i, o = sum o_i 2^(m_i - M) / sum l_i 2^(m_i - M), in CTA order.
+constexpr int kJoinThreads = 128, kJoinSplit = 8;
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAttnArgs a, int tile_rows) {
+    const PagedJoin j = a.join[blockIdx.x];
+    const int c0 = blockIdx.x;
+    if (j.last <= c0) return;
+    constexpr int DL = HD / 32;
+    const int lane = threadIdx.x & 31, part_floats = tile_rows * (2 + HD);
+    for (int r = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5); r < j.n_rows;
+         r += kJoinSplit * (kJoinThreads / 32)) {
+        float M = -INFINITY, L = 0.0f, o[DL];
+#pragma unroll
+        for (int d = 0; d < DL; d++) o[d] = 0.0f;
+        for (int c = c0; c <= j.last; c++) {
+            const float* p = a.part + ((size_t)c * 2 + (c == c0)) * part_floats;
+            const float m = p[r], l = p[tile_rows + r];
+            const float* po = p + 2 * tile_rows + (size_t)r * HD + lane * DL;
+            const float mn = fmaxf(M, m), base = mn == -INFINITY ? 0.0f : mn;
+            const float x = ex2(M - base), y = ex2(m - base);
+            L = L * x + l * y;
+            float f[DL];
+            if constexpr (DL == 4) *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(po);
+            else *reinterpret_cast<float2*>(f) = *reinterpret_cast<const float2*>(po);
+#pragma unroll
+            for (int d = 0; d < DL; d++) o[d] = o[d] * x + f[d] * y;
+            M = mn;
+        }
+        const int pr = j.row0 + r, tok = pr / a.group, h = j.kvh * a.group + pr - tok * a.group;
+        const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;
+        T* dst = static_cast<T*>(a.out) + (j.tok0 + tok) * a.out_stride + (size_t)h * HD + lane * DL;
+#pragma unroll
+        for (int d = 0; d < DL; d++) o[d] *= inv;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int d = 0; d < DL; d++) dst[d] = o[d];
+        } else {
+#pragma unroll
+            for (int d = 0; d < DL; d += 2) {
+                const __nv_bfloat162 b = __floats2bfloat162_rn(o[d], o[d + 1]);
+                *reinterpret_cast<uint32_t*>(dst + d) = *reinterpret_cast<const uint32_t*>(&b);
+            }
+        }
+        if (a.lse && lane == 0)
+            a.lse[(size_t)(j.tok0 + tok) * a.n_heads + h] = L == 0.0f ? -INFINITY : M * kLn2 + logf(L);
+    }
+}
+
+template <typename T, int HD>
+cudaError_t rows_case(const PagedAttnArgs& a, int ctas, cudaStream_t s) {
+    using C = RowsCfg<HD>;
+    const int smem = C::kFloats * 4 + (a.n_seq + 1) * 4;
+    cudaError_t e = cudaFuncSetAttribute(paged_rows_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         C::kFloats * 4 + (kPagedMaxSeq + 1) * 4);
+    if (e != cudaSuccess) return e;
+    paged_rows_kernel<T, HD><<<ctas, kRowsThreads, smem, s>>>(a);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_paged_attn_rows(int dtype, int hd, const PagedAttnArgs& a, int ctas, cudaStream_t s) {
+    if (dtype == RBT_MOE_DT_BF16) return hd == 64 ? rows_case<uint16_t, 64>(a, ctas, s) : rows_case<uint16_t, 128>(a, ctas, s);
+    return hd == 64 ? rows_case<float, 64>(a, ctas, s) : rows_case<float, 128>(a, ctas, s);
+}
+
+cudaError_t launch_paged_join(int dtype, int hd, int tile_rows, const PagedAttnArgs& a, int ctas, cudaStream_t s) {
+    const dim3 grid(ctas, kJoinSplit);
+    if (dtype == RBT_MOE_DT_BF16) {
+        if (hd == 64) paged_join_kernel<uint16_t, 64><<<grid, kJoinThreads, 0, s>>>(a, tile_rows);
+        else paged_join_kernel<uint16_t, 128><<<grid, kJoinThreads, 0, s>>>(a, tile_rows);
+    } else {
+        if (hd == 64) paged_join_kernel<float, 64><<<grid, kJoinThreads, 0, s>>>(a, tile_rows);
+        else paged_join_kernel<float, 128><<<grid, kJoinThreads, 0, s>>>(a, tile_rows);
+    }
+    return cudaGetLastError();
+}
+
+}  // namespace rbt

@@ -1,0 +1,394 @@
+// paged_tables.cu -- block tables and slot maps of the paged KV cache, built on the GPU
+// from request lengths, and the write of a step's new tokens into their slots.
+//
+// release / plan: every CTA scans all sequences' counts itself (at most kPagedMaxSeq, a
+// few per thread: two 64-bit sums by warp shuffles), so one launch needs no exchange
+// between CTAs, and then writes its share of the pages, slots and positions.  Both are
+// bound by latency (a launch, one round of loads, the scan, one or two dependent
+// loads), not by bytes.  The outputs must not overlap the inputs because CTAs read and
+// write at different times; the table (plan) and the free list (release) are only
+// written where no CTA of the call reads them.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/rbt_moe.h"
+#include "common.cuh"
+#include "paged.h"
+
+namespace rbt {
+namespace {
+
+constexpr int kTabThreads = 512;
+constexpr int kTabPer = kPagedMaxSeq / kTabThreads;  // sequences per thread, at most
+
+__device__ __forceinline__ void record(unsigned* status, unsigned code) { atomicCAS(status, 0u, code); }
+
+// Exclusive sums of (a, b) over the threads of the CTA in thread order, and the totals.
+struct Pair {
+    long long a, b;
+};
+__device__ Pair block_scan(Pair v, Pair* total) {
+    __shared__ Pair warp_sum_s[kTabThreads / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    Pair inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long a = __shfl_up_sync(FULL_MASK, inc.a, o), b = __shfl_up_sync(FULL_MASK, inc.b, o);
+        if (lane >= o) {
+            inc.a += a;
+            inc.b += b;
+        }
+    }
+    if (lane == 31) warp_sum_s[warp] = inc;
+    __syncthreads();
+    Pair before{0, 0}, all{0, 0};
+#pragma unroll
+    for (int w = 0; w < kTabThreads / 32; w++) {
+        const Pair s = warp_sum_s[w];
+        if (w < warp) {
+            before.a += s.a;
+            before.b += s.b;
+        }
+        all.a += s.a;
+        all.b += s.b;
+    }
+    *total = all;
+    return Pair{before.a + inc.a - v.a, before.b + inc.b - v.b};
+}
+
+// largest i in [0, n) with start[i] <= x (start ascending, start[0] <= x); of equal
+// starts the last, so sequences without any entry are passed over
+__device__ __forceinline__ int find_seq(const int* start, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (start[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+__global__ void __launch_bounds__(kTabThreads) plan_kernel(const PagedTablesArgs a) {
+    __shared__ int row_s[kPagedMaxSeq], fresh_s[kPagedMaxSeq], len_s[kPagedMaxSeq];
+    const int tid = threadIdx.x, n = a.n_seq, page = 1 << a.page_shift;
+    const int per = (n + kTabThreads - 1) / kTabThreads, i0 = tid * per;
+    const int n_free = *a.n_free;
+    int len[kTabPer], cnt[kTabPer], need[kTabPer];
+    unsigned bad = n_free < 0 ? kPagedNegative : 0u;
+    Pair mine{0, 0};
+#pragma unroll
+    for (int j = 0; j < kTabPer; j++) {
+        const int i = i0 + j;
+        const bool in = j < per && i < n;
+        len[j] = in ? a.len[i] : 0;
+        cnt[j] = in ? a.count[i] : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < kTabPer; j++) {
+        const long long end = (long long)len[j] + cnt[j];
+        if (len[j] < 0 || cnt[j] < 0) bad = kPagedNegative;
+        else if (end > (long long)a.table_stride * page || end > INT32_MAX) bad = bad ? bad : kPagedNarrow;
+        need[j] = bad ? 0 : (int)((end + page - 1) >> a.page_shift) - (int)(((long long)len[j] + page - 1) >> a.page_shift);
+        mine.a += cnt[j];
+        mine.b += need[j];
+    }
+    Pair total;
+    Pair at = block_scan(mine, &total);
+    // one reason for the whole call, the same in every CTA: the lowest code found
+    const unsigned code = __reduce_min_sync(FULL_MASK, bad ? bad : 0xffffffffu);
+    __shared__ unsigned code_s;
+    if (tid == 0) code_s = 0xffffffffu;
+    __syncthreads();
+    if ((tid & 31) == 0 && code != 0xffffffffu) atomicMin(&code_s, code);
+    __syncthreads();
+    unsigned err = code_s == 0xffffffffu ? 0u : code_s;
+    if (!err && total.b > n_free) err = kPagedNoPages;
+    if (!err && total.a > a.n_rows) err = kPagedRows;
+    if (err) {
+        if (blockIdx.x == 0) {
+            if (tid == 0) {
+                record(a.status, err);
+                *a.n_free_out = n_free;
+                a.cu[n] = 0;
+            }
+            for (int i = tid; i < n; i += kTabThreads) {
+                a.len_out[i] = a.len[i];
+                a.cu[i] = 0;
+            }
+        }
+        for (int r = blockIdx.x * kTabThreads + tid; r < a.n_rows; r += gridDim.x * kTabThreads) {
+            a.slot[r] = -1;
+            a.pos[r] = 0;
+        }
+        return;
+    }
+    // first row and first fresh page of every sequence
+#pragma unroll
+    for (int j = 0; j < kTabPer; j++) {
+        const int i = i0 + j;
+        if (j < per && i < n) {
+            row_s[i] = (int)at.a;
+            fresh_s[i] = (int)at.b;
+            len_s[i] = len[j];
+            if (blockIdx.x == 0) {
+                a.cu[i] = (int)at.a;
+                a.len_out[i] = len[j] + cnt[j];
+            }
+            at.a += cnt[j];
+            at.b += need[j];
+        }
+    }
+    if (blockIdx.x == 0 && tid == 0) {
+        a.cu[n] = (int)total.a;
+        *a.n_free_out = n_free - (int)total.b;
+    }
+    __syncthreads();
+    // fresh page f of the step is entry n_free - 1 - f of the free list
+    for (int f = blockIdx.x * kTabThreads + tid; f < (int)total.b; f += gridDim.x * kTabThreads) {
+        const int i = find_seq(fresh_s, n, f);
+        const int block = ((len_s[i] + page - 1) >> a.page_shift) + f - fresh_s[i];
+        const int id = a.free_list[n_free - 1 - f];
+        if ((unsigned)id >= (unsigned)a.n_pages) record(a.status, kPagedPage);
+        a.table[(size_t)i * a.table_stride + block] = id;
+    }
+    for (int r = blockIdx.x * kTabThreads + tid; r < a.n_rows; r += gridDim.x * kTabThreads) {
+        int64_t slot = -1;
+        int pos = 0;
+        if (r < (int)total.a) {
+            const int i = find_seq(row_s, n, r);
+            pos = len_s[i] + r - row_s[i];
+            const int block = pos >> a.page_shift, old = (len_s[i] + page - 1) >> a.page_shift;
+            // a block that the sequence already holds is in the table, a fresh one in the free list
+            const int id = block < old ? a.table[(size_t)i * a.table_stride + block]
+                                       : a.free_list[n_free - 1 - (fresh_s[i] + block - old)];
+            if ((unsigned)id < (unsigned)a.n_pages) slot = (int64_t)id * page + (pos & (page - 1));
+            else record(a.status, kPagedPage);
+        }
+        a.slot[r] = slot;
+        a.pos[r] = pos;
+    }
+}
+
+__global__ void __launch_bounds__(kTabThreads) release_kernel(const PagedTablesArgs a) {
+    __shared__ int first_s[kPagedMaxSeq];
+    const int tid = threadIdx.x, n = a.n_seq, page = 1 << a.page_shift;
+    const int per = (n + kTabThreads - 1) / kTabThreads, i0 = tid * per;
+    const int n_free = *a.n_free;
+    int len[kTabPer], held[kTabPer];
+    bool done[kTabPer];
+    int bad = n_free < 0;
+    Pair mine{0, 0};
+#pragma unroll
+    for (int j = 0; j < kTabPer; j++) {
+        const int i = i0 + j;
+        const bool in = j < per && i < n;
+        len[j] = in ? a.len[i] : 0;
+        done[j] = in && a.count[i] != 0;
+    }
+#pragma unroll
+    for (int j = 0; j < kTabPer; j++) {
+        if (len[j] < 0) bad = 1;
+        held[j] = done[j] && len[j] > 0 ? (int)(((long long)len[j] + page - 1) >> a.page_shift) : 0;
+        if (held[j] > a.table_stride) bad = 1;
+        mine.a += held[j];
+    }
+    Pair total;
+    Pair at = block_scan(mine, &total);
+    unsigned err = __syncthreads_or(bad) ? kPagedNegative : 0u;
+    if (!err && total.a > (long long)a.free_cap - n_free) err = kPagedFreeFull;
+    if (blockIdx.x == 0) {
+#pragma unroll
+        for (int j = 0; j < kTabPer; j++)
+            if (j < per && i0 + j < n) a.len_out[i0 + j] = done[j] && !err ? 0 : len[j];
+        if (tid == 0) {
+            if (err) record(a.status, err);
+            *a.n_free_out = err ? n_free : n_free + (int)total.a;
+        }
+    }
+    if (err) return;
+#pragma unroll
+    for (int j = 0; j < kTabPer; j++)
+        if (j < per && i0 + j < n) {
+            first_s[i0 + j] = (int)at.a;
+            at.a += held[j];
+        }
+    __syncthreads();
+    for (int f = blockIdx.x * kTabThreads + tid; f < (int)total.a; f += gridDim.x * kTabThreads) {
+        const int i = find_seq(first_s, n, f);
+        const int id = a.table[(size_t)i * a.table_stride + f - first_s[i]];
+        if ((unsigned)id >= (unsigned)a.n_pages) record(a.status, kPagedPage);
+        a.free_list[n_free + f] = id;
+    }
+}
+
+// ---------------------------------------------------------------- append
+// One CTA per token.  With the QK-norm the CTA first sums the squares of the whole q and
+// k rows (f32, a fixed order), then a thread takes kVec adjacent dims i and their partners
+// i + hd/2 (16-byte loads of the source): norm, rotation, one rounding to the cache's
+// type.  v is copied (and rounded).  Bound by bytes: each row is read once from HBM (the
+// second read of q and k with the norm hits L1) and written once.
+constexpr int kAppThreads = 256;
+
+template <typename S>
+struct Source;
+template <>
+struct Source<float> {
+    static constexpr int kVec = 4;
+};
+template <>
+struct Source<uint16_t> {
+    static constexpr int kVec = 8;
+};
+
+template <typename S>
+__device__ __forceinline__ void load_vec(const S* p, float (&f)[Source<S>::kVec]) {
+    WeightTraits<S>::unpack(*reinterpret_cast<const uint4*>(p), f);
+}
+
+template <int N>
+__device__ __forceinline__ void store_vec(float* p, const float (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+}
+template <int N>
+__device__ __forceinline__ void store_vec(uint16_t* p, const float (&f)[N]) {
+    uint32_t w[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; i++) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    if constexpr (N == 8) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+}
+
+template <typename S, typename T>
+__global__ void __launch_bounds__(kAppThreads) append_kernel(const PagedAppendArgs a) {
+    constexpr int V = Source<S>::kVec;
+    __shared__ float red[2][kAppThreads / 32];
+    const int r = blockIdx.x, tid = threadIdx.x, hd = a.hd, half = hd / 2;
+    const int64_t slot = a.slot[r];
+    if (slot < 0) return;
+    if (slot >= a.n_slots) {
+        if (tid == 0) record(a.status, kPagedSlot);
+        return;
+    }
+    const float *cs = nullptr, *sn = nullptr;
+    if (a.cos) {
+        const int pos = a.pos[r];
+        if (pos < 0 || pos >= a.rope_len) {
+            if (tid == 0) record(a.status, kPagedPos);
+            return;
+        }
+        cs = a.cos + (size_t)pos * half;
+        sn = a.sin + (size_t)pos * half;
+    }
+    const S* q = static_cast<const S*>(a.q) + r * a.q_stride;
+    const S* k = static_cast<const S*>(a.k) + r * a.k_stride;
+    const S* v = static_cast<const S*>(a.v) + r * a.v_stride;
+    const int nq = a.n_heads * hd, nkv = a.n_kv * hd;
+    float inv_q = 1.0f, inv_k = 1.0f;
+    if (a.q_norm) {
+        float sq = 0.0f, sk = 0.0f;
+        for (int i = tid; i < (nq + nkv) / V; i += kAppThreads) {
+            const bool is_q = i < nq / V;
+            float f[V], t = 0.0f;
+            load_vec<S>(is_q ? q + (size_t)i * V : k + (size_t)(i - nq / V) * V, f);
+#pragma unroll
+            for (int e = 0; e < V; e++) t = fmaf(f[e], f[e], t);
+            if (is_q) sq += t;
+            else sk += t;
+        }
+        sq = warp_sum(sq);
+        sk = warp_sum(sk);
+        if ((tid & 31) == 0) {
+            red[0][tid >> 5] = sq;
+            red[1][tid >> 5] = sk;
+        }
+        __syncthreads();
+        sq = sk = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kAppThreads / 32; w++) {
+            sq += red[0][w];
+            sk += red[1][w];
+        }
+        inv_q = 1.0f / sqrtf(sq / (float)nq + a.eps);
+        inv_k = 1.0f / sqrtf(sk / (float)nkv + a.eps);
+    }
+    const int64_t page = slot >> a.page_shift;
+    const int off = (int)(slot & ((1 << a.page_shift) - 1));
+    // element 0 of kv head 0 at this slot; kv heads are page_size * hd apart
+    const size_t base = (((size_t)page * a.n_kv << a.page_shift) + off) * hd;
+    const size_t head_step = (size_t)hd << a.page_shift;
+    const int hv = half / V, n_pairs = (a.n_heads + a.n_kv) * hv, n_v = nkv / V;
+    for (int it = tid; it < n_pairs + n_v; it += kAppThreads) {
+        if (it >= n_pairs) {  // v
+            const int e = (it - n_pairs) * V, h = e / hd;
+            float f[V];
+            load_vec<S>(v + e, f);
+            store_vec<V>(static_cast<T*>(a.vc) + base + h * head_step + (e - h * hd), f);
+            continue;
+        }
+        const int hh = it / hv, i = (it - hh * hv) * V;
+        const bool is_q = hh < a.n_heads;
+        const int h = is_q ? hh : hh - a.n_heads;
+        const S* src = (is_q ? q : k) + (size_t)h * hd + i;
+        float x[V], y[V];
+        load_vec<S>(src, x);
+        load_vec<S>(src + half, y);
+        if (a.q_norm) {
+            const float* w = (is_q ? a.q_norm : a.k_norm) + (size_t)h * hd + i;
+            const float inv = is_q ? inv_q : inv_k;
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                x[e] = x[e] * inv * w[e];
+                y[e] = y[e] * inv * w[e + half];
+            }
+        }
+        if (cs) {
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                const float c = cs[i + e], s = sn[i + e], u = x[e], t = y[e];
+                x[e] = u * c - t * s;
+                y[e] = t * c + u * s;
+            }
+        }
+        T* dst = is_q ? static_cast<T*>(a.q_out) + r * a.q_out_stride + (size_t)h * hd + i
+                      : static_cast<T*>(a.kc) + base + h * head_step + i;
+        store_vec<V>(dst, x);
+        store_vec<V>(dst + half, y);
+    }
+}
+
+}  // namespace
+
+cudaError_t launch_paged_plan(const PagedTablesArgs& a, int sm_count, cudaStream_t s) {
+    int ctas = (a.n_rows + kTabThreads - 1) / kTabThreads;
+    ctas = ctas < 1 ? 1 : ctas > sm_count ? sm_count : ctas;
+    plan_kernel<<<ctas, kTabThreads, 0, s>>>(a);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_paged_release(const PagedTablesArgs& a, int sm_count, cudaStream_t s) {
+    // the host knows no lengths: CTAs for a quarter of the table
+    const long long most = (long long)a.n_seq * a.table_stride / 4 / kTabThreads + 1;
+    const int ctas = most > sm_count ? sm_count : (int)most;
+    release_kernel<<<ctas, kTabThreads, 0, s>>>(a);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_paged_append(int src_dtype, int dtype, const PagedAppendArgs& a, cudaStream_t s) {
+    if (a.n_rows == 0) return cudaSuccess;
+    if (src_dtype == RBT_MOE_DT_BF16 && dtype == RBT_MOE_DT_BF16)
+        append_kernel<uint16_t, uint16_t><<<a.n_rows, kAppThreads, 0, s>>>(a);
+    else if (src_dtype == RBT_MOE_DT_BF16)
+        append_kernel<uint16_t, float><<<a.n_rows, kAppThreads, 0, s>>>(a);
+    else if (dtype == RBT_MOE_DT_BF16)
+        append_kernel<float, uint16_t><<<a.n_rows, kAppThreads, 0, s>>>(a);
+    else
+        append_kernel<float, float><<<a.n_rows, kAppThreads, 0, s>>>(a);
+    return cudaGetLastError();
+}
+
+}  // namespace rbt

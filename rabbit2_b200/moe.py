@@ -84,6 +84,13 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
         "rbt_model_decode_batch": [vp, vp, vp, i32, vp, vp, vp],
         "rbt_model_set_router_bias": [vp, i32, vp],
         "rbt_moe_router_logits": [vp, vp, i32],
+        "rbt_paged_create": [C.POINTER(vp), vp, i32],
+        "rbt_paged_bind_layer": [vp, i32, vp, vp],
+        "rbt_paged_status": [vp, C.POINTER(C.c_uint)],
+        "rbt_paged_release_device": [vp, i32, vp, vp, vp, i32, vp, i32, vp, vp, vp, vp],
+        "rbt_paged_plan_device": [vp, i32, vp, vp, vp, i32, vp, vp, i32, vp, vp, vp, vp, vp, vp],
+        "rbt_paged_append_device": [vp, i32, vp, vp],
+        "rbt_paged_attention_device": [vp, i32, vp, vp],
         "rbt_expf_device": [C.c_uint32, C.c_int64, vp, vp],
         "rbt_seq_sumsq_device": [vp, i32, i32, vp, vp],
     }
@@ -93,6 +100,8 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
         fn.restype = C.c_int
     lib.rbt_moe_destroy.argtypes = [vp]
     lib.rbt_moe_destroy.restype = None
+    lib.rbt_paged_destroy.argtypes = [vp]
+    lib.rbt_paged_destroy.restype = None
     lib.rbt_model_destroy.argtypes = [vp]
     lib.rbt_model_destroy.restype = None
     lib.rbt_model_moe.argtypes = [vp]

@@ -1,0 +1,53 @@
+"""The paged KV cache's C ABI and binding without a GPU: what they refuse, and how."""
+import ctypes as C
+
+import pytest
+
+from rabbit2_b200 import moe, paged
+
+
+def _lib():
+    return moe.load_library()
+
+
+def _error():
+    return _lib().rbt_moe_last_error().decode()
+
+
+@pytest.mark.parametrize("change, word", [
+    (dict(page_size=24), "page_size"), (dict(page_size=4), "page_size"), (dict(page_size=512), "page_size"),
+    (dict(n_pages=0), "n_pages"), (dict(head_dim=96), "head_dim"), (dict(n_kv_heads=3), "n_kv_heads"),
+    (dict(n_kv_heads=0), "n_kv_heads"), (dict(dtype=2), "dtype"), (dict(n_layers=-1), "n_layers"),
+    (dict(n_pages=1 << 26), "rows"), (dict(n_heads=2048, n_kv_heads=2048), "n_heads"),
+])
+def test_create_refuses(change, word):
+    cfg = dict(n_layers=1, n_heads=8, n_kv_heads=4, head_dim=64, page_size=16, n_pages=10, dtype=1)
+    cfg.update(change)
+    h = C.c_void_p()
+    assert _lib().rbt_paged_create(C.byref(h), C.byref(paged.RbtPagedConfig(**cfg)), 0) == 0
+    assert word in _error() and not h.value
+
+
+def test_null_contexts_are_refused():
+    lib = _lib()
+    assert lib.rbt_paged_bind_layer(None, 0, None, None) == 0
+    assert lib.rbt_paged_status(None, None) == 0
+    assert lib.rbt_paged_release_device(None, 1, *[None] * 2, None, 1, None, 1, None, None, None, None) == 0
+    assert lib.rbt_paged_plan_device(None, 1, None, None, None, 1, None, None, 1, *[None] * 6) == 0
+    assert lib.rbt_paged_append_device(None, 0, None, None) == 0
+    assert lib.rbt_paged_attention_device(None, 0, None, None) == 0
+    assert "null context" in _error()
+    lib.rbt_paged_destroy(None)
+
+
+def test_structs_match_the_header():
+    """Field order of the argument structs as the header declares them."""
+    import re
+    text = open(moe.HEADER).read()
+    for cls in (paged.RbtPagedConfig, paged.RbtPagedAppend, paged.RbtPagedAttention):
+        name = cls.__name__
+        body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), text, re.S).group(1)
+        body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
+        names = re.findall(r"(\w+)\s*(?=[,;])", body)
+        assert names == [f[0] for f in cls._fields_], name
+    assert int(re.search(r"RBT_PAGED_MAX_SEQ (\d+)", text).group(1)) == paged.MAX_SEQ

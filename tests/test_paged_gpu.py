@@ -1,0 +1,636 @@
+"""The paged KV cache on the GPU (rbt_paged_*): block tables and slot maps against plain Python,
+the write of new tokens and the attention against the formulas in 64 bits, each at the sizes and
+masks where it can go wrong, and a run of them together as a server makes it."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from rabbit2_b200 import moe
+
+pytestmark = pytest.mark.gpu
+U32 = 2.0 ** -24                                   # half a step of f32, relative
+DT = {"f32": torch.float32, "bf16": torch.bfloat16}
+STEP = {"f32": U32, "bf16": 2.0 ** -8}
+
+
+def dev(v, dtype=torch.int32):
+    return torch.tensor(v, dtype=dtype, device="cuda")
+
+
+# ---------------------------------------------------------------- tables
+def py_release(page, length, done, table, free, n_free):
+    free, held = list(free), list(length)
+    at = n_free
+    for i, d in enumerate(done):
+        if d:
+            for b in range(-(-length[i] // page)):
+                free[at] = table[i][b]
+                at += 1
+            held[i] = 0
+    return held, free, at
+
+
+def py_plan(page, length, new, table, free, n_free, rows):
+    table = [list(r) for r in table]
+    cu, slot, pos, out = [0], [], [], []
+    for i, (n, m) in enumerate(zip(length, new)):
+        for b in range(-(-n // page), -(-(n + m) // page)):
+            n_free -= 1
+            table[i][b] = free[n_free]
+        for p in range(n, n + m):
+            slot.append(table[i][p // page] * page + p % page)
+            pos.append(p)
+        cu.append(cu[-1] + m)
+        out.append(n + m)
+    slot += [-1] * (rows - len(slot))
+    pos += [0] * (rows - len(pos))
+    return out, n_free, table, cu, slot, pos
+
+
+class Pool:
+    """A pool with sequences of the given lengths, pages in shuffled order."""
+
+    def __init__(self, page, length, width, spare, seed=0):
+        rng = np.random.default_rng(seed)
+        held = [-(-n // page) for n in length]
+        self.page, self.n_pages = page, sum(held) + spare
+        ids = rng.permutation(self.n_pages).tolist()
+        self.table, at = [], 0
+        for h in held:
+            self.table.append(ids[at:at + h] + [0] * (width - h))
+            at += h
+        self.free, self.n_free = ids[at:] + [0] * at, self.n_pages - at
+        self.length = list(length)
+
+
+def run_tables(pool, new, rows, kv, done=None):
+    n = len(pool.length)
+    done = done or [0] * n
+    d = dict(length=dev(pool.length), done=dev(done), new=dev(new), table=dev(pool.table).view(n, -1),
+             free=dev(pool.free), n_free=dev([pool.n_free]))
+    held, n_mid = torch.full_like(d["length"], -7), dev([-7])
+    after, n_left, cu = torch.full_like(held, -7), dev([-7]), dev([-7] * (n + 1))
+    slot, pos = dev([-7] * rows, torch.int64), dev([-7] * rows)
+    kv.release(d["length"], d["done"], d["table"], d["free"], d["n_free"], held, n_mid)
+    kv.plan(held, d["new"], d["table"], d["free"], n_mid, after, n_left, cu, slot, pos)
+    status = kv.status()
+    got = dict(held=held, n_mid=n_mid, free=d["free"], after=after, n_left=n_left, table=d["table"], cu=cu, slot=slot,
+               pos=pos)
+    return {k: v.cpu().numpy() for k, v in got.items()}, status
+
+
+@pytest.mark.parametrize("page", [8, 16, 64, 256])
+@pytest.mark.parametrize("n", [1, 2, 33, 512, 513, 2048])
+def test_tables_match_plain_python(page, n):
+    from rabbit2_b200.paged import PagedTables
+    rng = np.random.default_rng(n * 1000 + page)
+    length = [int(x) for x in rng.choice([0, 1, page - 1, page, page + 1, 5 * page, 7 * page + 3], n)]
+    new = [int(x) for x in rng.choice([0, 0, 1, 1, 2, page - 1, page, 2 * page + 1], n)]
+    done = [int(rng.random() < 0.3) for _ in range(n)]
+    new = [0 if d and i % 2 else m for i, (d, m) in enumerate(zip(done, new))]  # some rows are taken up again
+    width = max(-(-(a + b) // page) for a, b in zip(length, new)) + 2
+    rows = sum(new) + 5
+    pool = Pool(page, length, width, spare=sum(-(-m // page) + 1 for m in new), seed=page + n)
+    kv = PagedTables(page, pool.n_pages)
+    got, status = run_tables(pool, new, rows, kv, done)
+    held, free, n_mid = py_release(page, length, done, pool.table, pool.free, pool.n_free)
+    after, n_left, table, cu, slot, pos = py_plan(page, held, new, pool.table, free, n_mid, rows)
+    assert status == 0
+    for k, want in dict(held=held, n_mid=[n_mid], free=free, after=after, n_left=[n_left], table=table, cu=cu, slot=slot,
+                        pos=pos).items():
+        np.testing.assert_array_equal(got[k].reshape(-1), np.array(want).reshape(-1), err_msg=k)
+
+
+def test_tables_of_one_long_sequence_and_of_none():
+    from rabbit2_b200.paged import PagedTables
+    pool = Pool(16, [100], 5000, spare=4500)
+    kv = PagedTables(16, pool.n_pages)
+    got, status = run_tables(pool, [70001], 70001, kv)
+    after, n_left, table, cu, slot, pos = py_plan(16, [100], [70001], pool.table, pool.free, pool.n_free, 70001)
+    assert status == 0
+    np.testing.assert_array_equal(got["slot"], slot)
+    np.testing.assert_array_equal(got["pos"], pos)
+    np.testing.assert_array_equal(got["table"][0], table[0])
+    assert got["n_left"][0] == n_left
+    empty = torch.zeros(0, dtype=torch.int32, device="cuda")
+    n_out, cu, slot, pos = dev([-7]), dev([-7]), dev([-7] * 3, torch.int64), dev([-7] * 3)
+    kv.plan(empty, empty, empty.view(0, 4), dev([1, 2]), dev([2]), empty.clone(), n_out, cu, slot, pos)
+    assert kv.status() == 0 and n_out.item() == 2 and cu.item() == 0
+    assert slot.tolist() == [-1] * 3 and pos.tolist() == [0] * 3
+
+
+@pytest.mark.parametrize("what, code", [("pages", 0x801), ("narrow", 0x802), ("rows", 0x803), ("negative", 0x804)])
+def test_plan_that_does_not_fit_takes_nothing(what, code):
+    from rabbit2_b200.paged import PagedTables
+    length, new = [20, 0, 31], [30, 17, 1]  # 2 + 2 + 0 fresh pages of 16
+    pool = Pool(16, length, 3 if what == "narrow" else 8, spare=3 if what == "pages" else 9)
+    if what == "negative":
+        new[1] = -1
+    rows = 40 if what == "rows" else 60
+    kv = PagedTables(16, pool.n_pages)
+    got, status = run_tables(pool, new, rows, kv)
+    assert status == code
+    assert got["after"].tolist() == length and got["n_left"][0] == pool.n_free and not got["cu"].any()
+    assert (got["slot"] == -1).all() and not got["pos"].any()
+    np.testing.assert_array_equal(got["table"], np.array(pool.table))
+    assert kv.status() == 0  # cleared
+    got, status = run_tables(Pool(16, [20], 8, spare=9), [3], 4, kv)  # and the next call works
+    assert status == 0 and got["after"].tolist() == [23]
+
+
+def test_release_into_a_full_list_moves_nothing():
+    from rabbit2_b200.paged import PagedTables
+    kv = PagedTables(16, 10)
+    free, n_out, held = dev([5, 6, 7]), dev([-7]), dev([-7, -7])
+    kv.release(dev([17, 3]), dev([1, 1]), dev([[1, 2], [3, 0]]), free, dev([1]), held, n_out)
+    assert kv.status() == 0x805 and free.tolist() == [5, 6, 7] and held.tolist() == [17, 3] and n_out.item() == 1
+    kv.release(dev([17, 3]), dev([1, 0]), dev([[1, 2], [3, 0]]), free, dev([1]), held, n_out)
+    assert kv.status() == 0 and free.tolist() == [5, 1, 2] and held.tolist() == [0, 3] and n_out.item() == 3
+
+
+def test_a_page_outside_the_pool_is_reported():
+    from rabbit2_b200.paged import PagedTables
+    kv = PagedTables(16, 10)
+    table, slot, pos, after, n_out, cu = dev([[3, 0]]), dev([0] * 4, torch.int64), dev([0] * 4), dev([0]), dev([0]), dev([0, 0])
+    kv.plan(dev([14]), dev([4]), table, dev([2, 99]), dev([2]), after, n_out, cu, slot, pos)
+    assert kv.status() == 0x806 and slot.tolist() == [3 * 16 + 14, 3 * 16 + 15, -1, -1]
+
+
+def test_tables_refuse_what_they_cannot_take():
+    from rabbit2_b200.paged import PagedTables
+    kv = PagedTables(16, 10)
+    n, t, f = dev([3, 4]), dev([[1], [2]]), dev([5, 6])
+    with pytest.raises(moe.RbtMoeError, match="overlap"):
+        kv.release(n, dev([0, 1]), t, f, dev([0]), n, dev([0]))
+    with pytest.raises(moe.RbtMoeError, match="overlap"):
+        one = dev([1])
+        kv.plan(n, dev([0, 1]), t, f, one, dev([0, 0]), one, dev([0, 0, 0]), dev([0], torch.int64), dev([0]))
+    with pytest.raises(ValueError, match="length"):
+        kv.release(n.long(), dev([0, 1]), t, f, dev([0]), dev([0, 0]), dev([0]))
+    with pytest.raises(ValueError, match="done"):
+        kv.release(n, dev([0]), t, f, dev([0]), dev([0, 0]), dev([0]))
+    with pytest.raises(ValueError, match="cpu"):
+        kv.release(n.cpu(), dev([0, 1]), t, f, dev([0]), dev([0, 0]), dev([0]))
+    with pytest.raises(moe.RbtMoeError, match="n_seq"):
+        big = torch.zeros(2049, dtype=torch.int32, device="cuda")
+        kv.release(big, big, big.view(-1, 1), f, dev([0]), big.clone(), dev([0]))
+    with pytest.raises(moe.RbtMoeError, match="layer"):
+        moe._check(kv.lib.rbt_paged_attention_device(kv.handle, 0, None, None), kv.lib)
+
+
+# ---------------------------------------------------------------- append
+def angles(positions, hd, base=10000.0):
+    a = torch.arange(positions, dtype=torch.float64)[:, None] * base ** (torch.arange(hd // 2, dtype=torch.float64) * (-2.0 / hd))
+    return a.cos().float().cuda(), a.sin().float().cuda()
+
+
+def exact_append(q, norm, cos, sin, pos, eps):
+    """(value, sum of the terms' magnitudes) of norm and rotation in 64 bits."""
+    x = q.double()
+    if norm is not None:
+        flat = x.flatten(1)
+        x = (flat / (flat.square().mean(1, keepdim=True) + eps).sqrt() * norm.double()).view_as(x)
+    mag = x.abs()
+    if cos is not None:
+        h = x.shape[-1] // 2
+        c, s = cos.double()[pos.long()][:, None], sin.double()[pos.long()][:, None]
+        a, b = x[..., :h], x[..., h:]
+        x = torch.cat([a * c - b * s, b * c + a * s], -1)
+        ma, mb = mag[..., :h], mag[..., h:]
+        mag = torch.cat([ma * c.abs() + mb * s.abs(), mb * c.abs() + ma * s.abs()], -1)
+    return x, mag
+
+
+@pytest.mark.parametrize("src, dst", [("f32", "bf16"), ("f32", "f32"), ("bf16", "bf16"), ("bf16", "f32")])
+@pytest.mark.parametrize("heads, kvh, hd", [(16, 16, 128), (6, 2, 64), (1, 1, 64), (40, 8, 128), (7, 7, 128)])
+@pytest.mark.parametrize("norm, rope", [(True, True), (False, True), (False, False)])
+def test_append_matches_the_formula(src, dst, heads, kvh, hd, norm, rope):
+    from rabbit2_b200.paged import PagedKv
+    torch.manual_seed(heads * 100 + hd)
+    n, page, n_pages = 37, 16, 9
+    kc, vc = (torch.randn(n_pages, kvh, page, hd, device="cuda").to(DT[dst]) for _ in range(2))
+    k0, v0 = kc.clone(), vc.clone()
+    qkv = torch.randn(n, (heads + 2 * kvh) * hd + 24, device="cuda").to(DT[src])  # rows wider than q|k|v
+    q, k, v = (x.unflatten(1, (-1, hd)) for x in qkv[:, :-24].split([heads * hd, kvh * hd, kvh * hd], 1))
+    slot = torch.randperm(n_pages * page, device="cuda")[:n].clone()
+    slot[[4, 36]] = -1
+    pos = torch.randint(0, 500, (n,), device="cuda", dtype=torch.int32)
+    qn, kn = (1 + 0.2 * torch.randn(h * hd, device="cuda") for h in (heads, kvh)) if norm else (None, None)
+    cos, sin = angles(500, hd) if rope else (None, None)
+    q_out = torch.full((n, heads, hd), 7.0, device="cuda", dtype=DT[dst])
+    kv = PagedKv(kc, vc, heads)
+    kv.append(q, k, v, slot, pos if rope else None, q_out, cos=cos, sin=sin, q_norm=qn, k_norm=kn, eps=1e-5)
+    assert kv.status() == 0
+    real = slot >= 0
+    # f32 arithmetic: the norm's sum (a chain of at most 160 products and 13 levels, halved by the
+    # root), its root, quotient and two products, then two products and a sum of the rotation
+    f32 = 100 * U32
+    for got, x, w in ((q_out, q, qn), (None, k, kn), (None, v, None)):
+        rot = x is not v
+        want, mag = exact_append(x, w, cos if rot else None, sin if rot else None, pos, 1e-5)
+        if got is None:
+            cache = kc if x is k else vc
+            got = torch.zeros(n, kvh, hd, device="cuda", dtype=DT[dst])
+            got[real] = cache[slot[real] // page, :, slot[real] % page]
+        err = (got.double() - want)[real].abs()
+        assert (err <= STEP[dst] * want[real].abs() + f32 * (1 + STEP[dst]) * mag[real]).all(), err.max()
+    assert (q_out[~real] == 7.0).all()  # padding
+    other = torch.ones(n_pages * page, dtype=torch.bool, device="cuda")
+    other[slot[real]] = False
+    for c, c0 in ((kc, k0), (vc, v0)):
+        flat, flat0 = (t.transpose(1, 2).reshape(n_pages * page, -1)[other] for t in (c, c0))
+        assert torch.equal(flat, flat0)
+
+
+def test_append_in_place_and_bad_rows():
+    from rabbit2_b200.paged import PagedKv
+    n, heads, kvh, hd, page = 6, 4, 2, 64, 8
+    kc, vc = (torch.zeros(3, kvh, page, hd, device="cuda") for _ in range(2))
+    kv = PagedKv(kc, vc, heads)
+    cos, sin = angles(50, hd)
+    qkv = torch.randn(n, (heads + 2 * kvh) * hd, device="cuda")
+    before = qkv.clone()
+    q, k, v = (x.unflatten(1, (-1, hd)) for x in qkv.split([heads * hd, kvh * hd, kvh * hd], 1))
+    slot = dev([0, 5, 24, 11, 1 << 40, -3], torch.int64)  # 24 slots
+    pos = dev([0, 49, 3, 50, 2, -1])
+    out = torch.empty(n, heads, hd, device="cuda")
+    kv.append(q, k, v, slot, pos, out, cos=cos, sin=sin)
+    assert kv.status() in (0x811, 0x812)
+    first = kc.clone()
+    kv.append(q, k, v, slot, pos, q, cos=cos, sin=sin)  # q in place, beside k and v in the same rows
+    assert kv.status() in (0x811, 0x812)
+    assert torch.equal(kc, first) and torch.equal(q[:2], out[:2])
+    assert torch.equal(qkv[2:], before[2:]) and torch.equal(qkv[:, heads * hd:], before[:, heads * hd:])
+    used = torch.zeros(24, dtype=torch.bool)
+    used[[0, 5]] = True
+    rows = kc.transpose(1, 2).reshape(24, -1).abs().sum(1).cpu() > 0
+    assert torch.equal(rows, used)  # nothing else was written
+
+
+def test_append_refuses():
+    from rabbit2_b200.paged import PagedKv
+    kc, vc = (torch.zeros(3, 2, 8, 64, device="cuda") for _ in range(2))
+    kv = PagedKv(kc, vc, 4)
+    q, k, v = (torch.zeros(5, h, 64, device="cuda") for h in (4, 2, 2))
+    slot, pos, out = dev([0] * 5, torch.int64), dev([0] * 5), torch.zeros(5, 4, 64, device="cuda")
+    cos, sin = angles(10, 64)
+    for bad, match in (((q[:, :3], k, v, slot, pos, out), "q:"), ((q, k.bfloat16(), v, slot, pos, out), "k:"),
+                       ((q, k, v, slot.int(), pos, out), "slot"), ((q, k, v, slot, pos.long(), out), "pos"),
+                       ((q, k, v, slot, pos, out.bfloat16()), "q_out"), ((q, k, v, slot[:4], pos, out), "slot")):
+        with pytest.raises(ValueError, match=match):
+            kv.append(*bad, cos=cos, sin=sin)
+    with pytest.raises(ValueError, match="cos and sin"):
+        kv.append(q, k, v, slot, pos, out, cos=cos)
+    with pytest.raises(ValueError, match="cos"):
+        kv.append(q, k, v, slot, pos, out, cos=cos[:, :16], sin=sin)
+    with pytest.raises(moe.RbtMoeError, match="positions"):
+        kv.append(q, k, v, slot, None, out, cos=cos, sin=sin)
+    with pytest.raises(moe.RbtMoeError, match="both"):
+        kv.append(q, k, v, slot, pos, out, q_norm=torch.ones(256, device="cuda"))
+    with pytest.raises(moe.RbtMoeError, match="aligned"):
+        wide = torch.zeros(5, 4 * 64 + 2, device="cuda")
+        kv.append(wide[:, 2:].unflatten(1, (4, 64)), k, v, slot, pos, out)
+    with pytest.raises(moe.RbtMoeError, match="overlaps"):
+        both = torch.zeros(9, 4, 64, device="cuda")
+        kv.append(both[:5], k, v, slot, pos, both[4:])
+    with pytest.raises(moe.RbtMoeError, match="layer"):
+        kv.append(q, k, v, slot, pos, out, layer=1)
+    none = torch.zeros(0, 4, 64, device="cuda")
+    kv.append(none, none[:, :2], none[:, :2], dev([], torch.int64), dev([]), none.clone())
+    assert kv.status() == 0
+
+
+# ---------------------------------------------------------------- attention
+class Batch:
+    """Sequences of given (cached, new) counts over shuffled pages; pages beyond a sequence's
+    length and the tails of its last page hold NaN."""
+
+    def __init__(self, seqs, heads, kvh, hd, page, dtype, seed=0, spread=1.0):
+        g = torch.Generator("cuda").manual_seed(seed)
+        self.seqs, self.heads, self.kvh, self.hd, self.page, self.dtype = seqs, heads, kvh, hd, page, DT[dtype]
+        self.step = STEP[dtype]
+        total = [c + n for c, n in seqs]
+        blocks = [-(-t // page) for t in total]
+        n_pages = sum(blocks) + 2
+        ids = torch.randperm(n_pages, generator=g, device="cuda").tolist()
+        rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+        self.k = torch.full((n_pages, kvh, page, hd), math.nan, device="cuda", dtype=self.dtype)
+        self.v = self.k.clone()
+        self.rows = [n for _, n in seqs]
+        width = max(blocks + [1]) + 1
+        table = np.full((len(seqs), width), -1, np.int32)
+        self.dense, at = [], 0
+        for i, (t, b) in enumerate(zip(total, blocks)):
+            mine = ids[at:at + b]
+            at += b
+            table[i, :b] = mine
+            k, v = rnd(t, kvh, hd).to(self.dtype), rnd(t, kvh, hd).to(self.dtype)
+            self.dense.append((k, v))
+            p = torch.arange(t, device="cuda")
+            pg = torch.tensor(mine, device="cuda", dtype=torch.int64)
+            if t:
+                self.k[pg[p // page], :, p % page] = k
+                self.v[pg[p // page], :, p % page] = v
+        self.table, self.length = torch.from_numpy(table).cuda(), dev(total)
+        self.cu = dev(np.concatenate([[0], np.cumsum(self.rows)]).tolist())
+        self.n = sum(self.rows)
+        self.q = (rnd(self.n, heads, hd) * spread).to(self.dtype)
+
+    def exact(self, causal=True, window=0, scale=None):
+        """out, lse, and bounds of the kernel's error on both."""
+        scale = 1 / math.sqrt(self.hd) if scale is None else scale
+        group = self.heads // self.kvh
+        outs = [torch.zeros(self.n, self.heads, self.hd, dtype=torch.float64, device="cuda") for _ in range(2)]
+        lses = [torch.zeros(self.n, self.heads, dtype=torch.float64, device="cuda") for _ in range(2)]
+        at = 0
+        for (c, n), (k, v) in zip(self.seqs, self.dense):
+            t = c + n
+            if n == 0:
+                continue
+            q = self.q[at:at + n].double().view(n, self.kvh, group, self.hd)
+            k, v = k.double(), v.double()
+            x = torch.einsum("tjgd,kjd->tjgk", q, k) * scale
+            xm = torch.einsum("tjgd,kjd->tjgk", q.abs(), k.abs()) * abs(scale)
+            pos = torch.arange(c, t, device="cuda")[:, None]
+            key = torch.arange(t, device="cuda")
+            seen = key <= pos if causal else torch.ones(n, t, dtype=torch.bool, device="cuda")
+            if window:
+                seen = seen & (key > pos - window)
+            x = x.masked_fill(~seen[:, None, None], -math.inf)
+            xm = xm.masked_fill(~seen[:, None, None], 0)
+            p = torch.softmax(x, -1).nan_to_num(0)
+            o = torch.einsum("tjgk,kjd->tjgd", p, v)
+            mag = torch.einsum("tjgk,kjd->tjgd", p, v.abs())
+            # a score is off by head_dim roundings of its terms (the sum) and 4 of itself (scale,
+            # base 2, difference from the maximum); exp2 is off by 2^-22, and twice that for the
+            # rescaling; the sums of weights and outputs by one rounding a position.  Weights
+            # rounded to the type for the product with v: half a step (bf16 only).
+            off = ((self.hd + 8) * U32 * xm).amax(-1, keepdim=True) + 2.0 ** -20
+            wide = (t + 16) * U32
+            b = mag * (2 * off + wide + (self.step if self.step > U32 else 0)) + self.step * o.abs()
+            outs[0][at:at + n], outs[1][at:at + n] = o.reshape(n, self.heads, -1), b.reshape(n, self.heads, -1)
+            lses[0][at:at + n] = torch.logsumexp(x, -1).reshape(n, -1)
+            lses[1][at:at + n] = (2 * off + wide).reshape(n, -1)
+            at += n
+        return outs, lses
+
+    def run(self, kv=None, out=None, lse=None, causal=True, window=0, scale=None, max_new=None, stream=None):
+        from rabbit2_b200.paged import PagedKv
+        kv = kv or PagedKv(self.k, self.v, self.heads)
+        out = torch.full((self.n, self.heads, self.hd), 5.0, device="cuda", dtype=self.dtype) if out is None else out
+        lse = torch.full((self.n, self.heads), 5.0, device="cuda") if lse is None else lse
+        kv.attention(self.q, out, self.cu, self.length, self.table, max(self.rows + [0]) if max_new is None else max_new,
+                     lse=lse, causal=causal, window=window, scale=scale, stream=stream)
+        return kv, out, lse
+
+    def check(self, **how):
+        run = {k: how.pop(k) for k in ("max_new",) if k in how}
+        kv, out, lse = self.run(**how, **run)
+        assert kv.status() == 0
+        (o, ob), (l, lb) = self.exact(**how)
+        err = (out.double() - o).abs()
+        assert torch.isfinite(out).all()
+        assert (err <= ob).all(), ((err - ob).max().item(), (err / ob.clamp_min(1e-30)).max().item())
+        empty = l == -math.inf
+        assert torch.equal(lse == -math.inf, empty)
+        lerr = (lse.double() - l).abs()[~empty]
+        assert (lerr <= lb[~empty] + U32 * l[~empty].abs()).all(), lerr.max()
+        return out, lse
+
+
+HEADS = [(16, 16, 128), (8, 2, 64), (32, 4, 128), (3, 1, 64), (12, 1, 128)]
+EDGES = {
+    "one token, lengths around the pages": [(c, 1) for c in (0, 1, 7, 15, 16, 17, 63, 64, 65, 255, 256, 1000)],
+    "chunks, some empty": [(0, 1), (0, 5), (3, 0), (0, 0), (100, 33), (17, 64), (0, 129), (250, 17)],
+    "one long sequence": [(4095, 1)],
+    "a long chunk": [(77, 301)],
+}
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads, kvh, hd", HEADS)
+@pytest.mark.parametrize("edge", list(EDGES))
+def test_attention_matches_the_formula(dtype, heads, kvh, hd, edge):
+    for page in (8, 64):
+        Batch(EDGES[edge], heads, kvh, hd, page, dtype, seed=hd + page).check()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("page", [8, 16, 32, 64, 128, 256])
+@pytest.mark.parametrize("window", [0, 1, 16, 100, 5000])
+def test_attention_pages_and_windows(dtype, page, window):
+    Batch([(500, 1), (0, 40), (129, 3), (700, 90)], 4, 2, 64, page, dtype, seed=page).check(window=window)
+    Batch([(300, 1), (999, 1), (31, 1)], 8, 2, 128, page, dtype, seed=page).check(window=window)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads, kvh, hd", [(8, 2, 64), (5, 5, 128)])
+def test_attention_without_the_causal_mask(dtype, heads, kvh, hd):
+    Batch([(0, 30), (200, 1), (90, 140), (5, 0)], heads, kvh, hd, 32, dtype).check(causal=False)
+    Batch([(64, 1), (1, 1), (777, 2)], heads, kvh, hd, 32, dtype).check(causal=False)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("seqs", [[(1500, 1)] * 3, [(300, 200), (1500, 1)]])
+def test_attention_large_and_negative_scores(dtype, seqs):
+    """Scores far apart (the running maximum moves by hundreds) and a scale of its own."""
+    Batch(seqs, 4, 2, 128, 16, dtype, spread=30.0).check()
+    Batch(seqs, 4, 2, 64, 16, dtype).check(scale=-0.7)
+    Batch(seqs, 4, 2, 64, 16, dtype).check(scale=0.0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("new", [1, 150])
+def test_attention_rows_before_the_cache_see_nothing(dtype, new):
+    """A length below the number of new tokens: the first rows stand before position 0."""
+    b = Batch([(40, new), (0, 6)], 4, 2, 64, 16, dtype)
+    b.length[1] = 2
+    kv, out, lse = b.run()
+    assert kv.status() == 0
+    assert (out[new:new + 4] == 0).all() and (lse[new:new + 4] == -math.inf).all()
+    assert (out[new + 4:] != 0).any() and torch.isfinite(lse[new + 4:]).all()
+    one = Batch([(0, 2)], 4, 2, 64, 16, dtype)
+    one.q, one.k, one.v, one.table, one.dense = b.q[new + 4:].clone(), b.k, b.v, b.table[1:].contiguous(), b.dense[1:]
+    _, o2, l2 = one.run()
+    assert torch.allclose(out[new + 4:].float(), o2.float(), rtol=0, atol=2 * b.step * 5) and torch.allclose(lse[new + 4:], l2)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("seqs", [[(70, 1), (9, 1)], [(70, 60), (9, 1)]])
+def test_attention_leaves_other_rows_and_takes_strides(dtype, seqs):
+    """Rows behind the last sequence stay; q and out rows of a wider buffer; lse optional."""
+    from rabbit2_b200.paged import PagedKv
+    b = Batch(seqs, 6, 2, 64, 16, dtype)
+    kv, want, lse = b.run()
+    n = b.n + 3
+    q = torch.full((n, 6 * 64 + 40), math.nan, device="cuda", dtype=b.dtype)
+    q[:b.n, 8:8 + 384] = b.q.flatten(1)
+    out = torch.full((n, 6 * 64 + 16), 3.0, device="cuda", dtype=b.dtype)
+    lse2 = torch.full((n, 6), 3.0, device="cuda")
+    rows = lambda t, o: t[:, o:o + 384].unflatten(1, (6, 64))  # noqa: E731
+    kv.attention(rows(q, 8), rows(out, 8), b.cu, b.length, b.table, max(b.rows), lse=lse2)
+    assert kv.status() == 0
+    assert torch.equal(rows(out, 8)[:b.n], want) and torch.equal(lse2[:b.n], lse)
+    assert (out[b.n:] == 3).all() and (out[:, :8] == 3).all() and (out[:, 392:] == 3).all() and (lse2[b.n:] == 3).all()
+    kv2 = PagedKv(b.k, b.v, 6)
+    o3 = torch.zeros_like(want)
+    kv2.attention(b.q, o3, b.cu, b.length, b.table, max(b.rows))
+    assert torch.equal(o3, want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_bound_of_new_tokens_may_be_wrong(dtype):
+    """max_new only chooses kernels: smaller and larger bounds give the same values."""
+    b = Batch([(30, 90), (200, 1), (0, 20)], 8, 2, 64, 16, dtype)
+    for most in (0, 1, 20, 90, 4000):
+        b.check(max_new=most)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("new", [1, 80])
+def test_attention_reports_bad_lengths_offsets_and_pages(dtype, new):
+    b = Batch([(70, new), (9, 1)], 4, 2, 64, 16, dtype)
+    kv, want, _ = b.run()
+    assert kv.status() == 0
+    for code, change in ((0x822, lambda x: x.length.__setitem__(0, 10000)), (0x822, lambda x: x.length.__setitem__(0, -1)),
+                         (0x821, lambda x: x.cu.__setitem__(2, 10000)), (0x821, lambda x: x.cu.__setitem__(0, -5)),
+                         (0x823, lambda x: x.table.__setitem__((0, 1), -1)),
+                         (0x823, lambda x: x.table.__setitem__((0, 1), 1 << 30))):
+        c = Batch([(70, new), (9, 1)], 4, 2, 64, 16, dtype)
+        change(c)
+        c.run(kv=kv)
+        # kv's caches hold the same pages: both batches are made from one seed
+        assert kv.status() == code
+    _, again, _ = b.run(kv=kv)
+    assert kv.status() == 0 and torch.equal(again, want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_of_many_sequences(dtype):
+    rng = np.random.default_rng(0)
+    Batch([(int(rng.integers(0, 60)), int(rng.integers(0, 3))) for _ in range(2048)], 2, 1, 64, 8, dtype).check()
+    Batch([(int(rng.integers(0, 90)), int(rng.choice([0, 1, 1, 1, 50]))) for _ in range(700)], 4, 2, 64, 16, dtype).check()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("seqs", [[(700, 1)] * 5, [(100, 260), (700, 1)]])
+def test_attention_is_repeatable_and_captured(dtype, seqs):
+    """The same bits twice, on another stream, and from a replayed graph whose lengths change."""
+    from rabbit2_b200.paged import PagedKv
+    b = Batch(seqs, 8, 2, 128, 16, dtype)
+    kv, want, lse = b.run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    out2, lse2 = torch.zeros_like(want), torch.zeros_like(lse)
+    b.run(kv=kv, out=out2, lse=lse2, stream=side)
+    side.synchronize()
+    assert torch.equal(out2, want) and torch.equal(lse2, lse)
+    out3, lse3 = torch.zeros_like(want), torch.zeros_like(lse)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        b.run(kv=kv, out=out3, lse=lse3)
+    for _ in range(2):
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out3, want) and torch.equal(lse3, lse)
+    b.length.sub_(5)  # the same graph, other lengths
+    g.replay()
+    _, short, _ = b.run(kv=PagedKv(b.k, b.v, 8))
+    assert torch.equal(out3, short) and not torch.equal(short, want)
+    assert kv.status() == 0
+
+
+def test_attention_refuses():
+    from rabbit2_b200.paged import PagedKv
+    b = Batch([(20, 3)], 4, 2, 64, 16, "bf16")
+    kv = PagedKv(b.k, b.v, 4)
+    out = torch.zeros_like(b.q)
+    with pytest.raises(moe.RbtMoeError, match="window"):
+        kv.attention(b.q, out, b.cu, b.length, b.table, 3, causal=False, window=4)
+    with pytest.raises(moe.RbtMoeError, match="window"):
+        kv.attention(b.q, out, b.cu, b.length, b.table, 3, window=-1)
+    with pytest.raises(moe.RbtMoeError, match="scale"):
+        kv.attention(b.q, out, b.cu, b.length, b.table, 3, scale=math.inf)
+    with pytest.raises(moe.RbtMoeError, match="overlaps"):
+        kv.attention(b.q, b.q, b.cu, b.length, b.table, 3)
+    with pytest.raises(moe.RbtMoeError, match="layer"):
+        kv.attention(b.q, out, b.cu, b.length, b.table, 3, layer=1)
+    with pytest.raises(ValueError, match="q:"):
+        kv.attention(b.q.float(), out, b.cu, b.length, b.table, 3)
+    with pytest.raises(ValueError, match="out:"):
+        kv.attention(b.q, out[:2], b.cu, b.length, b.table, 3)
+    with pytest.raises(ValueError, match="cu"):
+        kv.attention(b.q, out, b.cu[:1], b.length, b.table, 3)
+    with pytest.raises(ValueError, match="table"):
+        kv.attention(b.q, out, b.cu, b.length, b.table.long(), 3)
+    with pytest.raises(ValueError, match="lse"):
+        kv.attention(b.q, out, b.cu, b.length, b.table, 3, lse=torch.zeros(3, 2, device="cuda"))
+    with pytest.raises(ValueError, match="caches"):
+        PagedKv(b.k, b.v[:1], 4)
+    with pytest.raises(moe.RbtMoeError, match="n_kv_heads"):
+        PagedKv(b.k, b.v, 5)
+    with pytest.raises(ValueError, match="caches"):
+        PagedKv(b.k.half(), b.v.half(), 4)
+    none = torch.zeros(0, 4, 64, device="cuda", dtype=torch.bfloat16)
+    kv.attention(none, none.clone(), dev([0, 0]), b.length, b.table, 0)
+    assert kv.status() == 0
+
+
+# ---------------------------------------------------------------- together
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_server_of_paged_sequences(dtype):
+    """Requests come, grow by chunks and tokens, end, and give their pages to others: every step's
+    attention of every layer equals that over the sequence's own dense rows."""
+    from rabbit2_b200.paged import PagedKv
+    rng, page, n_pages, heads, kvh, hd, layers, n, width = np.random.default_rng(3), 16, 40, 4, 2, 64, 2, 5, 24
+    torch.manual_seed(1)
+    caches = [torch.full((layers, n_pages, kvh, page, hd), math.nan, device="cuda", dtype=DT[dtype]) for _ in range(2)]
+    kv = PagedKv(caches[0], caches[1], heads)
+    cos, sin = angles(512, hd)
+    length, n_free = dev([0] * n), dev([n_pages])
+    table, free = torch.full((n, width), -1, dtype=torch.int32, device="cuda"), torch.arange(n_pages, dtype=torch.int32, device="cuda")
+    dense = [[[] for _ in range(n)] for _ in range(layers)]
+    for step in range(14):
+        done = [int(length[i].item() > 90 and rng.random() < 0.6) for i in range(n)]
+        held, n_mid, after, n_left = torch.zeros_like(length), torch.zeros_like(n_free), torch.zeros_like(length), torch.zeros_like(n_free)
+        kv.release(length, dev(done), table, free, n_free, held, n_mid)
+        room = n_mid.item() * page - 8 * n
+        new = []
+        for i in range(n):
+            m = int(rng.choice([0, 1, 1, 1, 20, 45])) if held[i] else int(rng.integers(1, 60))
+            new.append(m if m < room else 0)
+            room -= new[-1]
+            if done[i]:
+                for d in dense:
+                    d[i] = []
+        rows = sum(new) + 2
+        cu, slot, pos = dev([0] * (n + 1)), dev([0] * rows, torch.int64), dev([0] * rows)
+        kv.plan(held, dev(new), table, free, n_mid, after, n_left, cu, slot, pos)
+        length, n_free = after, n_left
+        assert kv.status() == 0
+        for l in range(layers):
+            qkv = torch.randn(rows, (heads + 2 * kvh) * hd, device="cuda")
+            q, k, v = (x.unflatten(1, (-1, hd)) for x in qkv.split([heads * hd, kvh * hd, kvh * hd], 1))
+            q_out = torch.zeros(rows, heads, hd, device="cuda", dtype=DT[dtype])
+            out = torch.zeros_like(q_out)
+            kv.append(q, k, v, slot, pos, q_out, cos=cos, sin=sin, layer=l)
+            kv.attention(q_out, out, cu, length, table, max(new), layer=l)
+            at = 0
+            for i, m in enumerate(new):
+                if not m:
+                    continue
+                dense[l][i].append((*exact_append(k[at:at + m], None, cos, sin, pos[at:at + m], 0), v[at:at + m]))
+                want, mag, vals = (torch.cat([x[j] for x in dense[l][i]]) for j in range(3))
+                ids = table[i, :-(-want.shape[0] // page)].long()
+                K, V = (c[l][ids].transpose(1, 2).reshape(-1, kvh, hd)[:want.shape[0]] for c in caches)
+                assert torch.equal(V, vals.to(DT[dtype]))
+                assert ((K.double() - want).abs() <= STEP[dtype] * want.abs() + 8 * U32 * mag).all()
+                b = Batch([(K.shape[0] - m, m)], heads, kvh, hd, page, dtype)
+                b.q, b.dense = q_out[at:at + m], [(K, V)]
+                (o, ob), _ = b.exact()
+                assert ((out[at:at + m].double() - o).abs() <= ob).all(), (step, l, i)
+                at += m
+            assert (out[at:] == 0).all()
+        assert kv.status() == 0
