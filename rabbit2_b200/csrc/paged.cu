@@ -21,6 +21,7 @@ struct RbtPaged {
     int device = 0, sm_count = 0, page_shift = 0;
     struct Layer {
         void *k = nullptr, *v = nullptr;
+        rbt::PagedMaps maps;  // bf16 caches
     };
     std::vector<Layer> layers;
     unsigned* status = nullptr;
@@ -144,7 +145,7 @@ int rbt_paged_create(RbtPaged** out, const RbtPagedConfig* cfg, int device) {
     if (e == cudaSuccess) e = cudaMalloc((void**)&p->status, sizeof(unsigned));
     if (e == cudaSuccess) e = cudaMemset(p->status, 0, sizeof(unsigned));
     if (e == cudaSuccess && c.n_layers > 0) {
-        const size_t tile = (size_t)64 * (2 + c.head_dim) * sizeof(float);
+        const size_t tile = (size_t)paged_part_floats(64, c.head_dim) * sizeof(float);
         e = cudaMalloc((void**)&p->part, (size_t)attn_ctas(p) * 2 * tile);
         if (e == cudaSuccess) e = cudaMalloc((void**)&p->join, (size_t)attn_ctas(p) * sizeof(PagedJoin));
     }
@@ -169,9 +170,16 @@ int rbt_paged_bind_layer(RbtPaged* p, int layer, void* d_k, void* d_v) {
     if (!p) return fail("null context");
     if (layer < 0 || layer >= p->cfg.n_layers) return fail("layer %d out of range [0, %d)", layer, p->cfg.n_layers);
     if (!d_k || !d_v) return fail("null cache pointer");
+    ON_DEVICE(p);
     if (!aligned16(d_k) || !aligned16(d_v)) return fail("the caches must be 16-byte aligned");
-    p->layers[layer].k = d_k;
-    p->layers[layer].v = d_v;
+    RbtPaged::Layer& L = p->layers[layer];
+    const RbtPagedConfig& c = p->cfg;
+    L.k = L.v = nullptr;
+    if (c.dtype == RBT_MOE_DT_BF16 && !paged_decode_maps(&L.maps, d_k, d_v, c.head_dim, c.page_size,
+                                                         (uint64_t)c.n_pages * c.n_kv_heads * c.page_size))
+        return fail("cannot encode the caches' tensor maps");
+    L.k = d_k;
+    L.v = d_v;
     return 1;
 }
 
@@ -361,12 +369,29 @@ int rbt_paged_attention_device(RbtPaged* p, int layer, const RbtPagedAttention* 
     a.part = p->part;
     a.join = p->join;
     a.status = p->status;
-    a.rows_lo = 0;
-    a.rows_hi = INT32_MAX;
     cudaStream_t s = (cudaStream_t)stream;
-    const int ctas = attn_ctas(p);
-    CU(launch_paged_attn_rows(c.dtype, c.head_dim, a, ctas, s));
-    CU(launch_paged_join(c.dtype, c.head_dim, 64, a, ctas, s));
+    // Few query rows per kv head: the kernel that streams the cache; more: the tile kernel.
+    // A batch of both kinds takes both, each its own sequences.
+    const bool bf = c.dtype == RBT_MOE_DT_BF16;
+    const int few = bf ? kPagedDecRowsBf16 : kPagedDecRowsF32;
+    const int64_t most = (int64_t)x.max_new * a.group;
+    int dec_rows = few;
+    if (!bf)
+        while (dec_rows > 1 && dec_rows / 2 >= most) dec_rows /= 2;
+    const PagedMaps& maps = p->layers[layer].maps;
+    if (most <= few || x.n_seq > 1) {
+        a.rows_lo = 0;
+        a.rows_hi = most <= few ? INT32_MAX : few;
+        CU(launch_paged_decode(c.dtype, c.head_dim, dec_rows, maps, a, p->sm_count, s));
+        CU(launch_paged_join(c.dtype, c.head_dim, dec_rows, a, p->sm_count, s));
+    }
+    if (most > few) {
+        a.rows_lo = x.n_seq > 1 ? few : 0;
+        a.rows_hi = INT32_MAX;
+        const int ctas = attn_ctas(p);
+        CU(launch_paged_attn_rows(c.dtype, c.head_dim, a, ctas, s));
+        CU(launch_paged_join(c.dtype, c.head_dim, 64, a, ctas, s));
+    }
     return 1;
 }
 

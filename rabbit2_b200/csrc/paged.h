@@ -34,6 +34,10 @@ struct PagedJoin {
     int tok0, kvh;      // row of the sequence's first token, kv head
 };
 
+// One partial tile in floats: max[rows], sum[rows], then o[rows][hd] on a 16-byte boundary.
+__host__ __device__ constexpr int paged_part_o(int rows) { return rows < 2 ? 4 : 2 * rows; }
+__host__ __device__ constexpr int paged_part_floats(int rows, int hd) { return paged_part_o(rows) + rows * hd; }
+
 struct PagedAttnArgs {
     const void *q, *k, *v;
     void* out;
@@ -45,16 +49,21 @@ struct PagedAttnArgs {
     int causal, window;
     int rows_lo, rows_hi;  // sequences with rows_lo < new tokens * group <= rows_hi are this launch's
     float scale;
-    float* part;           // [ctas][2] partial tiles: max[rows], sum[rows], o[rows][head_dim]
+    float* part;           // [ctas][2] partial tiles
     PagedJoin* join;       // [ctas]
     unsigned* status;
 };
 
-// One attention launch of up to `ctas` CTAs, its partial tiles and its joins.
-struct PagedAttnPlan {
-    int ctas;
-    int tile_rows;
+// Rows of a tile of the kernels for few rows (f32: 1, 2, 4 or 8, chosen by the call).
+constexpr int kPagedDecRowsBf16 = 16, kPagedDecRowsF32 = 8;
+
+// Tensor maps of one layer's bf16 caches as rows [page][kv head][position] of head_dim.
+struct PagedMaps {
+    CUtensorMap k_dec, v_dec;  // boxes of one page's run of positions, both 64-dim halves
 };
+bool paged_decode_maps(PagedMaps* maps, const void* k, const void* v, int hd, int page_size, uint64_t rows);
+cudaError_t launch_paged_decode(int dtype, int hd, int tile_rows, const PagedMaps& maps, const PagedAttnArgs& a, int ctas,
+                                cudaStream_t s);
 
 cudaError_t launch_paged_attn_rows(int dtype, int hd, const PagedAttnArgs& a, int ctas, cudaStream_t s);
 cudaError_t launch_paged_join(int dtype, int hd, int tile_rows, const PagedAttnArgs& a, int ctas, cudaStream_t s);

@@ -20,14 +20,6 @@ namespace {
 
 using namespace paged;
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 __device__ __forceinline__ void store4(float* p, const float (&f)[4]) {
     *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
 }
@@ -47,7 +39,7 @@ struct RowsCfg {
     static constexpr int kKN = HD == 64 ? 4 : 2, kBlock = 16 * kKN;
     static constexpr int kLd = HD + 4, kLdP = kBlock + 4;
     static constexpr int kFloats = kRows * kLd + 2 * kBlock * kLd + kRows * kLdP;
-    static constexpr int kPart = kRows * (2 + HD);  // floats of one partial tile
+    static constexpr int kPart = paged_part_floats(kRows, HD);
 };
 
 template <typename T, int HD>
@@ -229,7 +221,7 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedAtt
                 }
 #pragma unroll
                 for (int k = 0; k < DV; k++)
-                    *reinterpret_cast<float4*>(part + 2 * C::kRows + (size_t)r * HD + 4 * tx + 64 * k) = o[i][k];
+                    *reinterpret_cast<float4*>(part + paged_part_o(C::kRows) + (size_t)r * HD + 4 * tx + 64 * k) = o[i][k];
             }
             if (w.head && tid == 0)
                 a.join[blockIdx.x] = PagedJoin{w.finisher(), t.r0, t.rows, t.s.row0, t.kvh};
@@ -249,7 +241,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAtt
     const int c0 = blockIdx.x;
     if (j.last <= c0) return;
     constexpr int DL = HD / 32;
-    const int lane = threadIdx.x & 31, part_floats = tile_rows * (2 + HD);
+    const int lane = threadIdx.x & 31, part_floats = paged_part_floats(tile_rows, HD);
     for (int r = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5); r < j.n_rows;
          r += kJoinSplit * (kJoinThreads / 32)) {
         float M = -INFINITY, L = 0.0f, o[DL];
@@ -258,7 +250,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAtt
         for (int c = c0; c <= j.last; c++) {
             const float* p = a.part + ((size_t)c * 2 + (c == c0)) * part_floats;
             const float m = p[r], l = p[tile_rows + r];
-            const float* po = p + 2 * tile_rows + (size_t)r * HD + lane * DL;
+            const float* po = p + paged_part_o(tile_rows) + (size_t)r * HD + lane * DL;
             const float mn = fmaxf(M, m), base = mn == -INFINITY ? 0.0f : mn;
             const float x = ex2(M - base), y = ex2(m - base);
             L = L * x + l * y;

@@ -1,0 +1,615 @@
+// paged_decode.cu -- attention over a paged KV cache for sequences with few query rows:
+// one new token, or a few, times the heads that share a kv head (at most 16 rows in
+// bf16, 8 in f32).  Bound by the bytes of k and v, which are read once each.
+//
+// Both kernels have the same shape.  One CTA per SM takes an equal share of all units
+// (paged_sched.cuh).  Warp 4 is the producer: it walks the share ahead of the others and
+// fills a ring of 16 KB stages (k and v of one block of positions) by bulk copies, across
+// the borders of tiles, so that up to 128 KB per SM are in flight.  Warps 0-3 take the
+// blocks in turn, each with a running maximum, sum and output of its own, and add the four
+// up at the end of a tile through shared memory; nothing inside a tile waits for another
+// warp.
+//
+// bf16: 16 rows are the M side of mma.sync m16n8k16 (the 128 rows of a tcgen05 tile would
+// be mostly padding, and the tensor work here is a small part of the copies' time);
+// k and v come by tensor copies in the 128-byte swizzle, so that ldmatrix reads them
+// without bank conflicts, v transposed on the way.
+// f32: products and sums in f32 on the CUDA cores.  Eight lanes share a position (dims
+// jj, jj + 8, ... in 16-byte groups), four positions at a time; the weights go through
+// shared memory and each lane keeps its own dims of the output.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "../../include/rbt_moe.h"
+#include "common.cuh"
+#include "kernels.h"
+#include "paged.h"
+#include "paged_sched.cuh"
+#include "tc_ptx.cuh"
+
+namespace rbt {
+namespace {
+
+using namespace paged;
+using namespace tc;
+
+constexpr int kDecWarps = 4, kDecThreads = 32 * (kDecWarps + 1);
+constexpr int kDecStages = 8;           // a multiple of kDecWarps: a stage always belongs to one warp
+constexpr int kDecStage = 16384;        // bytes: k | v
+constexpr int kDecMinUnits = kDecWarps; // a CTA with less would leave warps idle
+constexpr uint64_t kDecWaitNs = 2000000000ull;
+static_assert(kDecStages % kDecWarps == 0, "stages are dealt to warps");
+
+// ---------------------------------------------------------------- both kernels
+struct Ring {
+    uint64_t full[kDecStages], empty[kDecStages];
+};
+
+__device__ __forceinline__ void ring_init(Ring* r) {
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kDecStages; i++) {
+            mbar_init(&r->full[i], 1);
+            mbar_init(&r->empty[i], 1);
+        }
+        fence_mbar_init();
+    }
+}
+
+// The producer warp.  copy(id, off, box, stage, bar) starts the copies of positions
+// [off, off + box rows) of page id into box `box` of the stage (one lane per box).
+template <int kRows, int kBlock, typename Copy>
+__device__ __forceinline__ void produce(const PagedAttnArgs& a, const Share& share, const int* starts, Ring* ring,
+                                        uint8_t* stages, int box_rows, uint32_t row_bytes, Copy copy) {
+    const int lane = threadIdx.x & 31;
+    Walk<kRows, kBlock> w(share, starts);
+    uint32_t j = 0;
+    bool ok = true;
+    while (ok && w.next(a)) {
+        const int32_t* table = a.table + (size_t)w.t.seq * a.table_stride;
+        int chunk = -1, ids = 0;  // 32 entries of the table row, one per lane
+        for (int b = w.first; b < w.first + w.n; b++, j++) {
+            const int p0 = b * kBlock, left = min(kBlock, w.t.hi - p0);
+            const int boxes = left > 0 ? (left + box_rows - 1) / box_rows : 0;
+            const int page0 = p0 >> a.page_shift;
+            if ((page0 >> 5) != chunk) {
+                chunk = page0 >> 5;
+                const int at = chunk * 32 + lane;
+                ids = at < a.table_stride ? table[at] : 0;
+            }
+            const uint32_t st = j % kDecStages;
+            if (j >= kDecStages && !mbar_wait_bounded(&ring->empty[st], (j / kDecStages - 1) & 1, kDecWaitNs)) ok = false;
+            ok = __all_sync(FULL_MASK, ok);
+            if (!ok) {
+                if (lane == 0) atomicCAS(a.status, 0u, (unsigned)kPagedWait);
+                break;
+            }
+            if (lane == 0) mbar_arrive_expect_tx(&ring->full[st], boxes * box_rows * row_bytes * 2);
+            __syncwarp();
+            const int p = p0 + lane * box_rows;  // this lane's box
+            int id = __shfl_sync(FULL_MASK, ids, (p >> a.page_shift) & 31);
+            if (lane < boxes) {
+                if ((unsigned)id >= (unsigned)a.n_pages) {  // no page: any valid memory, and no result
+                    atomicCAS(a.status, 0u, (unsigned)kPagedTable);
+                    id = 0;
+                }
+                copy(id, w.t.kvh, p & ((1 << a.page_shift) - 1), lane, stages + st * kDecStage, &ring->full[st]);
+            }
+        }
+    }
+    // every copy has landed before the CTA may exit
+    for (uint32_t i = j > kDecStages ? j - kDecStages : 0; i < j; i++)
+        if (!mbar_wait_bounded(&ring->full[i % kDecStages], (i / kDecStages) & 1, kDecWaitNs) && lane == 0)
+            atomicCAS(a.status, 0u, (unsigned)kPagedWait);
+}
+
+// A consumer's wait for block j; after one that ran out it waits no more (the results are
+// void, the barriers are still met).
+__device__ __forceinline__ void await(const PagedAttnArgs& a, Ring* ring, uint32_t j, bool& ok) {
+    if (ok) ok = __all_sync(FULL_MASK, mbar_wait_bounded(&ring->full[j % kDecStages], (j / kDecStages) & 1, kDecWaitNs));
+    if (!ok && (threadIdx.x & 31) == 0) atomicCAS(a.status, 0u, (unsigned)kPagedWait);
+}
+
+// The four warps' parts of a segment, in shared memory: two sets of maxima and sums (the
+// next segment's are written while this one's are read), one of outputs.
+template <int kRows, int HD>
+struct Parts {
+    static constexpr int kPitch = HD + 8;
+    float m[2][kDecWarps][kRows], l[2][kDecWarps][kRows];
+    float o[kDecWarps][kRows][kPitch];
+};
+
+template <typename T>
+__device__ __forceinline__ void put4(T* dst, float4 f) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(dst) = f;
+    } else {
+        const __nv_bfloat162 x = __floats2bfloat162_rn(f.x, f.y), y = __floats2bfloat162_rn(f.z, f.w);
+        *reinterpret_cast<uint2*>(dst) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+    }
+}
+
+// Adds up the warps' parts (their o already scaled to the common maximum by their owners)
+// and writes the rows, or the CTA's part of them.
+template <typename T, int kRows, int HD, typename W>
+__device__ __forceinline__ void finish(const PagedAttnArgs& a, const W& w, const Parts<kRows, HD>* s, int set) {
+    const Tile& t = w.t;
+    float* part = a.part + ((size_t)blockIdx.x * 2 + (w.head ? 1 : 0)) * paged_part_floats(kRows, HD);
+    for (int e = threadIdx.x; e < t.rows * (HD / 4); e += 32 * kDecWarps) {
+        const int r = e / (HD / 4), c = 4 * (e - r * (HD / 4));
+        float M = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kDecWarps; i++) M = fmaxf(M, s->m[set][i][r]);
+        const float base = M == -INFINITY ? 0.0f : M;
+        float L = 0.0f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < kDecWarps; i++) {
+            const float m = s->m[set][i][r];
+            if (m == -INFINITY && s->l[set][i][r] == 0.0f) continue;  // that warp saw nothing of this row: no output either
+            L += s->l[set][i][r] * ex2(m - base);
+            const float4 f = *reinterpret_cast<const float4*>(&s->o[i][r][c]);
+            o.x += f.x;
+            o.y += f.y;
+            o.z += f.z;
+            o.w += f.w;
+        }
+        if (w.whole) {
+            const int tok = (t.r0 + r) / a.group, h = t.kvh * a.group + (t.r0 + r) - tok * a.group;
+            const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;
+            put4(static_cast<T*>(a.out) + (t.s.row0 + tok) * a.out_stride + (size_t)h * HD + c,
+                 make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+            if (a.lse && c == 0)
+                a.lse[(size_t)(t.s.row0 + tok) * a.n_heads + h] = L == 0.0f ? -INFINITY : M * kLn2 + logf(L);
+        } else {
+            if (c == 0) {
+                part[r] = M;
+                part[kRows + r] = L;
+            }
+            *reinterpret_cast<float4*>(part + paged_part_o(kRows) + (size_t)r * HD + c) = o;
+        }
+    }
+    if (!w.whole && w.head && threadIdx.x == 0)
+        a.join[blockIdx.x] = PagedJoin{w.finisher(), t.r0, t.rows, t.s.row0, t.kvh};
+}
+
+// ---------------------------------------------------------------- bf16
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&x)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <int HD>
+struct DecBf16 {
+    static constexpr int kRows = kPagedDecRowsBf16;
+    static constexpr int kBlock = kDecStage / (4 * HD);  // positions of a stage: 32 (head_dim 128) or 64
+    static constexpr int kHalf = kDecStage / 2;          // bytes of k
+    static constexpr int kSmem = kDecStages * kDecStage + (int)sizeof(Parts<kRows, HD>) + 1024;
+};
+
+template <int HD>
+__global__ void __launch_bounds__(kDecThreads, 1)
+    paged_decode_bf16_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                             const PagedAttnArgs a) {
+    using C = DecBf16<HD>;
+    constexpr int KB = C::kBlock, NT = KB / 8, KS = HD / 16;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    Parts<C::kRows, HD>* parts = reinterpret_cast<Parts<C::kRows, HD>*>(smem + kDecStages * kDecStage);
+    int* starts = reinterpret_cast<int*>(parts + 1);
+    __shared__ Ring ring;
+    __shared__ Share share;
+    ring_init(&ring);
+    if (threadIdx.x == 0) {
+        prefetch_tmap(&tm_k);
+        prefetch_tmap(&tm_v);
+        a.join[blockIdx.x].last = blockIdx.x;
+    }
+    find_share<kDecThreads, C::kRows, KB, kDecMinUnits>(a, starts, &share);  // (its barriers publish the ring's too)
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int page = 1 << a.page_shift, box = min(page, KB);
+    if (warp == kDecWarps) {
+        produce<C::kRows, KB>(a, share, starts, &ring, smem, box, HD * 2,
+                              [&](int id, int kvh, int off, int i, uint8_t* stage, uint64_t* bar) {
+                                  const int y = ((id * a.n_kv + kvh) << a.page_shift) + off;
+                                  tma_load_3d(stage + i * box * HD * 2, &tm_k, bar, 0, y, 0);
+                                  tma_load_3d(stage + C::kHalf + i * box * HD * 2, &tm_v, bar, 0, y, 0);
+                              });
+        return;
+    }
+    const int g = lane >> 2, tq = lane & 3;
+    const float k2 = a.scale * kLog2e;
+    const int box_shift = min(a.page_shift, HD == 128 ? 5 : 6);
+    // byte offset of 16-byte chunk `c` (of HD / 8) of position r of a block: boxes of [half][box
+    // rows][64 dims] in the 128-byte swizzle
+    const auto at = [&](int r, int c) -> uint32_t {
+        const uint32_t b = r >> box_shift, rr = r & (box - 1);
+        return b * (box * HD * 2) + (c >> 3) * (box * 128) + rr * 128 + ((uint32_t)((c & 7) ^ (rr & 7)) << 4);
+    };
+    Walk<C::kRows, KB> w(share, starts);
+    uint32_t j = 0;
+    bool ok = true;
+    for (int set = 0; w.next(a); set ^= 1) {
+        const Tile& t = w.t;
+        uint32_t q[KS][4];  // rows g and g + 8 as A fragments
+        int to[2], from[2];
+        const uint16_t* qp[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int r = g + 8 * i, tok = (t.r0 + r) / a.group, pos = t.off + tok;
+            to[i] = r >= t.rows ? 0 : a.causal ? min(t.s.len, pos + 1) : t.s.len;
+            from[i] = a.window ? max(0, pos - a.window + 1) : 0;
+            qp[i] = r >= t.rows ? nullptr
+                                : static_cast<const uint16_t*>(a.q) + (t.s.row0 + tok) * a.q_stride +
+                                      (size_t)(t.kvh * a.group + (t.r0 + r) - tok * a.group) * HD;
+        }
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                q[k][i] = qp[i] ? *reinterpret_cast<const uint32_t*>(qp[i] + 16 * k + 2 * tq) : 0u;
+                q[k][i + 2] = qp[i] ? *reinterpret_cast<const uint32_t*>(qp[i] + 16 * k + 8 + 2 * tq) : 0u;
+            }
+        // blocks that every row of the tile sees whole need no mask
+        const int sure_to = a.causal ? min(t.s.len, t.off + t.r0 / a.group + 1) : t.s.len;
+        const int sure_from = a.window ? t.off + (t.r0 + t.rows - 1) / a.group - a.window + 1 : 0;
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[HD / 8][4];
+#pragma unroll
+        for (int n = 0; n < HD / 8; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[n][i] = 0.0f;
+        const uint32_t skip = (warp - j) & (kDecWarps - 1);
+        for (int i = skip; i < w.n; i += kDecWarps) {
+            const uint32_t jj = j + i, st = jj % kDecStages;
+            const int p0 = (w.first + i) * KB;
+            await(a, &ring, jj, ok);
+            const uint32_t ks = smem_u32(smem + st * kDecStage), vs = ks + C::kHalf;
+            float s[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[n][e] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < KS; k += 2) {  // positions 8 n .., dims 16 k .. + 32
+                    uint32_t b[4];
+                    ldsm4(ks + at(8 * n + (lane & 7), 2 * k + (lane >> 3)), b);
+                    mma16816(s[n], q[k], b[0], b[1]);
+                    mma16816(s[n], q[k + 1], b[2], b[3]);
+                }
+            }
+            const bool edge = p0 + KB > sure_to || p0 < sure_from;
+            float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float x = s[n][e] * k2;
+                    if (edge) {
+                        const int p = p0 + 8 * n + 2 * tq + (e & 1);
+                        if (p >= to[e >> 1] || p < from[e >> 1]) x = -INFINITY;
+                    }
+                    s[n][e] = x;
+                    top[e >> 1] = fmaxf(top[e >> 1], x);
+                }
+            float alpha[2], base[2];
+#pragma unroll
+            for (int i2 = 0; i2 < 2; i2++) {
+                top[i2] = fmaxf(top[i2], __shfl_xor_sync(FULL_MASK, top[i2], 1));
+                top[i2] = fmaxf(top[i2], __shfl_xor_sync(FULL_MASK, top[i2], 2));
+                const float mn = fmaxf(m[i2], top[i2]);
+                base[i2] = mn == -INFINITY ? 0.0f : mn;
+                alpha[i2] = ex2(m[i2] - base[i2]);
+                m[i2] = mn;
+                l[i2] *= alpha[i2];
+            }
+            if (__any_sync(FULL_MASK, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
+#pragma unroll
+                for (int n = 0; n < HD / 8; n++) {
+                    o[n][0] *= alpha[0];
+                    o[n][1] *= alpha[0];
+                    o[n][2] *= alpha[1];
+                    o[n][3] *= alpha[1];
+                }
+            }
+            uint32_t pa[NT / 2][4];  // the weights as A fragments, rounded to bf16 (half a step each, summed in f32)
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const float x0 = ex2(s[n][0] - base[0]), x1 = ex2(s[n][1] - base[0]);
+                const float y0 = ex2(s[n][2] - base[1]), y1 = ex2(s[n][3] - base[1]);
+                l[0] += x0 + x1;
+                l[1] += y0 + y1;
+                pa[n >> 1][(n & 1) * 2] = pack2(x0, x1);
+                pa[n >> 1][(n & 1) * 2 + 1] = pack2(y0, y1);
+            }
+            const bool tail = p0 + KB > t.hi;
+            if (tail) {  // what lies behind the last position is not a number, perhaps: no weight of 0 hides that
+                for (int e = lane; e < KB * (HD / 8); e += 32) {
+                    const int r = e / (HD / 8), c = e - r * (HD / 8);
+                    if (p0 + r >= t.hi)
+                        *reinterpret_cast<uint4*>(smem + st * kDecStage + C::kHalf + at(r, c)) = make_uint4(0, 0, 0, 0);
+                }
+                __syncwarp();
+            }
+#pragma unroll
+            for (int k = 0; k < NT / 2; k++)
+#pragma unroll
+                for (int n = 0; n < HD / 8; n += 2) {  // positions 16 k .., dims 8 n .. + 16
+                    uint32_t b[4];
+                    ldsm4_t(vs + at(16 * k + (lane & 15), n + (lane >> 4)), b);
+                    mma16816(o[n], pa[k], b[0], b[1]);
+                    mma16816(o[n + 1], pa[k], b[2], b[3]);
+                }
+            if (tail) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the copies write there again
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ring.empty[st]);
+        }
+        j += w.n;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            l[i] += __shfl_xor_sync(FULL_MASK, l[i], 1);
+            l[i] += __shfl_xor_sync(FULL_MASK, l[i], 2);
+            if (tq == 0) {
+                parts->m[set][warp][g + 8 * i] = m[i];
+                parts->l[set][warp][g + 8 * i] = l[i];
+            }
+        }
+        named_sync(1, 32 * kDecWarps);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int r = g + 8 * i;
+            if (r >= t.rows) continue;
+            float M = -INFINITY;
+#pragma unroll
+            for (int x = 0; x < kDecWarps; x++) M = fmaxf(M, parts->m[set][x][r]);
+            const float f = ex2(m[i] - (M == -INFINITY ? 0.0f : M));
+#pragma unroll
+            for (int n = 0; n < HD / 8; n++)
+                *reinterpret_cast<float2*>(&parts->o[warp][r][8 * n + 2 * tq]) =
+                    make_float2(o[n][2 * i] * f, o[n][2 * i + 1] * f);
+        }
+        named_sync(1, 32 * kDecWarps);
+        finish<uint16_t, C::kRows, HD>(a, w, parts, set);
+    }
+}
+
+// ---------------------------------------------------------------- f32
+template <int HD, int R>
+struct DecF32 {
+    static constexpr int kBlock = kDecStage / (8 * HD);  // 16 (head_dim 128) or 32
+    static constexpr int kHalf = kDecStage / 2;
+    static constexpr int kSmem = kDecStages * kDecStage + (int)sizeof(Parts<R, HD>) + kDecWarps * kBlock * R * 4 + 128;
+};
+
+template <int HD, int R>
+__global__ void __launch_bounds__(kDecThreads, 1) paged_decode_f32_kernel(const PagedAttnArgs a) {
+    using C = DecF32<HD, R>;
+    constexpr int KB = C::kBlock, NI = KB / 4, NC = HD / 32, DL = HD / 32;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
+    Parts<R, HD>* parts = reinterpret_cast<Parts<R, HD>*>(smem + kDecStages * kDecStage);
+    float* weights = reinterpret_cast<float*>(parts + 1);  // [warp][KB][R]
+    int* starts = reinterpret_cast<int*>(weights + kDecWarps * KB * R);
+    __shared__ Ring ring;
+    __shared__ Share share;
+    ring_init(&ring);
+    if (threadIdx.x == 0) a.join[blockIdx.x].last = blockIdx.x;
+    find_share<kDecThreads, R, KB, kDecMinUnits>(a, starts, &share);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int page = 1 << a.page_shift, box = min(page, KB);
+    if (warp == kDecWarps) {
+        produce<R, KB>(a, share, starts, &ring, smem, box, HD * 4,
+                       [&](int id, int kvh, int off, int i, uint8_t* stage, uint64_t* bar) {
+                           const size_t row = (((size_t)id * a.n_kv + kvh) << a.page_shift) + off;
+                           const uint32_t bytes = box * HD * 4;
+                           bulk_load(stage + i * bytes, static_cast<const float*>(a.k) + row * HD, bytes, bar);
+                           bulk_load(stage + C::kHalf + i * bytes, static_cast<const float*>(a.v) + row * HD, bytes, bar);
+                       });
+        return;
+    }
+    const int kg = lane >> 3, jj = lane & 7;
+    const float k2 = a.scale * kLog2e;
+    float* wp = weights + warp * KB * R;
+    Walk<R, KB> w(share, starts);
+    uint32_t j = 0;
+    bool ok = true;
+    for (int set = 0; w.next(a); set ^= 1) {
+        const Tile& t = w.t;
+        float4 q[R][NC];
+        int to[R], from[R];
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const int tok = (t.r0 + r) / a.group, pos = t.off + tok;
+            to[r] = r >= t.rows ? 0 : a.causal ? min(t.s.len, pos + 1) : t.s.len;
+            from[r] = a.window ? max(0, pos - a.window + 1) : 0;
+            const float* src = static_cast<const float*>(a.q) + (t.s.row0 + tok) * a.q_stride +
+                               (size_t)(t.kvh * a.group + (t.r0 + r) - tok * a.group) * HD;
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+                q[r][c] = r < t.rows ? *reinterpret_cast<const float4*>(src + 4 * (jj + 8 * c))
+                                     : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        float m[R], l[R], o[R][DL];
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            m[r] = -INFINITY;
+            l[r] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < DL; d++) o[r][d] = 0.0f;
+        }
+        const uint32_t skip = (warp - j) & (kDecWarps - 1);
+        for (int b = skip; b < w.n; b += kDecWarps) {
+            const uint32_t jb = j + b, st = jb % kDecStages;
+            const int p0 = (w.first + b) * KB, nv = min(KB, t.hi - p0);
+            await(a, &ring, jb, ok);
+            const float* Ks = reinterpret_cast<const float*>(smem + st * kDecStage);
+            const float* Vs = reinterpret_cast<const float*>(smem + st * kDecStage + C::kHalf);
+            float s[NI][R];
+#pragma unroll
+            for (int i = 0; i < NI; i++) {
+                float4 k4[NC];
+#pragma unroll
+                for (int c = 0; c < NC; c++)
+                    k4[c] = *reinterpret_cast<const float4*>(Ks + (4 * i + kg) * HD + 4 * (jj + 8 * c));
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    float x = 0.0f;
+#pragma unroll
+                    for (int c = 0; c < NC; c++) {
+                        x = fmaf(q[r][c].x, k4[c].x, x);
+                        x = fmaf(q[r][c].y, k4[c].y, x);
+                        x = fmaf(q[r][c].z, k4[c].z, x);
+                        x = fmaf(q[r][c].w, k4[c].w, x);
+                    }
+                    s[i][r] = x;
+                }
+            }
+#pragma unroll
+            for (int d = 1; d < 8; d <<= 1)
+#pragma unroll
+                for (int i = 0; i < NI; i++)
+#pragma unroll
+                    for (int r = 0; r < R; r++) s[i][r] += __shfl_xor_sync(FULL_MASK, s[i][r], d);
+            float alpha[R];
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < NI; i++) {
+                    const int p = p0 + 4 * i + kg;
+                    s[i][r] = p >= from[r] && p < to[r] ? s[i][r] * k2 : -INFINITY;
+                    top = fmaxf(top, s[i][r]);
+                }
+                top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, 8));
+                top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, 16));
+                const float mn = fmaxf(m[r], top), base = mn == -INFINITY ? 0.0f : mn;
+                alpha[r] = ex2(m[r] - base);
+                m[r] = mn;
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < NI; i++) {
+                    s[i][r] = ex2(s[i][r] - base);
+                    sum += s[i][r];
+                }
+                l[r] = l[r] * alpha[r] + sum;
+            }
+            if (jj == 0) {
+#pragma unroll
+                for (int i = 0; i < NI; i++)
+#pragma unroll
+                    for (int r = 0; r < R; r++) wp[(4 * i + kg) * R + r] = s[i][r];
+            }
+            __syncwarp();
+#pragma unroll
+            for (int r = 0; r < R; r++)
+#pragma unroll
+                for (int d = 0; d < DL; d++) o[r][d] *= alpha[r];
+#pragma unroll 4
+            for (int p = 0; p < nv; p++) {
+                float v[DL], x[R];
+#pragma unroll
+                for (int d = 0; d < DL; d += 2)
+                    *reinterpret_cast<float2*>(v + d) = *reinterpret_cast<const float2*>(Vs + p * HD + lane * DL + d);
+#pragma unroll
+                for (int r = 0; r < R; r++) x[r] = wp[p * R + r];
+#pragma unroll
+                for (int r = 0; r < R; r++)
+#pragma unroll
+                    for (int d = 0; d < DL; d++) o[r][d] = fmaf(x[r], v[d], o[r][d]);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ring.empty[st]);
+        }
+        j += w.n;
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            l[r] += __shfl_xor_sync(FULL_MASK, l[r], 8);
+            l[r] += __shfl_xor_sync(FULL_MASK, l[r], 16);
+            if (lane == 0) {
+                parts->m[set][warp][r] = m[r];
+                parts->l[set][warp][r] = l[r];
+            }
+        }
+        named_sync(1, 32 * kDecWarps);
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            if (r >= t.rows) continue;
+            float M = -INFINITY;
+#pragma unroll
+            for (int x = 0; x < kDecWarps; x++) M = fmaxf(M, parts->m[set][x][r]);
+            const float f = ex2(m[r] - (M == -INFINITY ? 0.0f : M));
+#pragma unroll
+            for (int d = 0; d < DL; d++) parts->o[warp][r][lane * DL + d] = o[r][d] * f;
+        }
+        named_sync(1, 32 * kDecWarps);
+        finish<float, R, HD>(a, w, parts, set);
+    }
+}
+
+template <typename K>
+cudaError_t set_smem(K kernel, int bytes) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes + (kPagedMaxSeq + 1) * 4);
+}
+
+template <int HD>
+cudaError_t bf16_case(const PagedMaps& maps, const PagedAttnArgs& a, int ctas, cudaStream_t s) {
+    const int smem = DecBf16<HD>::kSmem;
+    cudaError_t e = set_smem(paged_decode_bf16_kernel<HD>, smem);
+    if (e != cudaSuccess) return e;
+    paged_decode_bf16_kernel<HD><<<ctas, kDecThreads, smem + (a.n_seq + 1) * 4, s>>>(maps.k_dec, maps.v_dec, a);
+    return cudaGetLastError();
+}
+
+template <int HD, int R>
+cudaError_t f32_case(const PagedAttnArgs& a, int ctas, cudaStream_t s) {
+    const int smem = DecF32<HD, R>::kSmem;
+    cudaError_t e = set_smem(paged_decode_f32_kernel<HD, R>, smem);
+    if (e != cudaSuccess) return e;
+    paged_decode_f32_kernel<HD, R><<<ctas, kDecThreads, smem + (a.n_seq + 1) * 4, s>>>(a);
+    return cudaGetLastError();
+}
+
+template <int HD>
+cudaError_t f32_rows(int rows, const PagedAttnArgs& a, int ctas, cudaStream_t s) {
+    switch (rows) {
+        case 1: return f32_case<HD, 1>(a, ctas, s);
+        case 2: return f32_case<HD, 2>(a, ctas, s);
+        case 4: return f32_case<HD, 4>(a, ctas, s);
+        default: return f32_case<HD, 8>(a, ctas, s);
+    }
+}
+
+}  // namespace
+
+bool paged_decode_maps(PagedMaps* maps, const void* k, const void* v, int hd, int page_size, uint64_t rows) {
+    const uint64_t dims[3] = {64, rows, (uint64_t)hd / 64}, strides[2] = {(uint64_t)hd * 2, 128};
+    const int block = hd == 128 ? DecBf16<128>::kBlock : DecBf16<64>::kBlock;
+    const uint32_t box[3] = {64, (uint32_t)(page_size < block ? page_size : block), (uint32_t)hd / 64};
+    return make_map_sw128(&maps->k_dec, k, 3, dims, strides, box) && make_map_sw128(&maps->v_dec, v, 3, dims, strides, box);
+}
+
+cudaError_t launch_paged_decode(int dtype, int hd, int tile_rows, const PagedMaps& maps, const PagedAttnArgs& a, int ctas,
+                                cudaStream_t s) {
+    if (dtype == RBT_MOE_DT_BF16) return hd == 64 ? bf16_case<64>(maps, a, ctas, s) : bf16_case<128>(maps, a, ctas, s);
+    return hd == 64 ? f32_rows<64>(tile_rows, a, ctas, s) : f32_rows<128>(tile_rows, a, ctas, s);
+}
+
+}  // namespace rbt

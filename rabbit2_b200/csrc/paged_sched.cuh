@@ -17,6 +17,15 @@
 namespace rbt {
 namespace paged {
 
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// 2^x of the special-function unit (relative error 2^-22; below 2^-126 it gives 0)
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 struct Seq {
     int row0, count, len;  // first row, new tokens, positions; count 0: not of this launch
 };
