@@ -101,8 +101,6 @@ int check_rows(const char* name, const void* ptr, int64_t stride, int width, int
     return 1;
 }
 
-int attn_ctas(const RbtPaged* p) { return p->sm_count * 2; }
-
 }  // namespace
 
 extern "C" {
@@ -145,9 +143,10 @@ int rbt_paged_create(RbtPaged** out, const RbtPagedConfig* cfg, int device) {
     if (e == cudaSuccess) e = cudaMalloc((void**)&p->status, sizeof(unsigned));
     if (e == cudaSuccess) e = cudaMemset(p->status, 0, sizeof(unsigned));
     if (e == cudaSuccess && c.n_layers > 0) {
-        const size_t tile = (size_t)paged_part_floats(64, c.head_dim) * sizeof(float);
-        e = cudaMalloc((void**)&p->part, (size_t)attn_ctas(p) * 2 * tile);
-        if (e == cudaSuccess) e = cudaMalloc((void**)&p->join, (size_t)attn_ctas(p) * sizeof(PagedJoin));
+        // two partial tiles per CTA of the largest launch: 256 rows on every SM, or 64 rows on twice as many CTAs
+        const int rows = c.dtype == RBT_MOE_DT_BF16 ? kPagedTcRows : 2 * kPagedF32Rows;
+        e = cudaMalloc((void**)&p->part, (size_t)p->sm_count * 2 * paged_part_floats(rows, c.head_dim) * sizeof(float));
+        if (e == cudaSuccess) e = cudaMalloc((void**)&p->join, (size_t)2 * p->sm_count * sizeof(PagedJoin));
     }
     if (e != cudaSuccess) {
         rbt_paged_destroy(p);
@@ -175,8 +174,9 @@ int rbt_paged_bind_layer(RbtPaged* p, int layer, void* d_k, void* d_v) {
     RbtPaged::Layer& L = p->layers[layer];
     const RbtPagedConfig& c = p->cfg;
     L.k = L.v = nullptr;
-    if (c.dtype == RBT_MOE_DT_BF16 && !paged_decode_maps(&L.maps, d_k, d_v, c.head_dim, c.page_size,
-                                                         (uint64_t)c.n_pages * c.n_kv_heads * c.page_size))
+    const uint64_t rows = (uint64_t)c.n_pages * c.n_kv_heads * c.page_size;
+    if (c.dtype == RBT_MOE_DT_BF16 && (!paged_decode_maps(&L.maps, d_k, d_v, c.head_dim, c.page_size, rows) ||
+                                       !paged_tc_maps(&L.maps, d_k, d_v, c.head_dim, c.page_size, rows)))
         return fail("cannot encode the caches' tensor maps");
     L.k = d_k;
     L.v = d_v;
@@ -388,9 +388,9 @@ int rbt_paged_attention_device(RbtPaged* p, int layer, const RbtPagedAttention* 
     if (most > few) {
         a.rows_lo = x.n_seq > 1 ? few : 0;
         a.rows_hi = INT32_MAX;
-        const int ctas = attn_ctas(p);
-        CU(launch_paged_attn_rows(c.dtype, c.head_dim, a, ctas, s));
-        CU(launch_paged_join(c.dtype, c.head_dim, 64, a, ctas, s));
+        if (bf) CU(launch_paged_tc(c.head_dim, maps, a, p->sm_count, s));
+        else CU(launch_paged_rows(c.head_dim, a, 2 * p->sm_count, s));
+        CU(launch_paged_join(c.dtype, c.head_dim, bf ? kPagedTcRows : kPagedF32Rows, a, bf ? p->sm_count : 2 * p->sm_count, s));
     }
     return 1;
 }

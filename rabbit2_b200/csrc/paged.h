@@ -56,16 +56,22 @@ struct PagedAttnArgs {
 
 // Rows of a tile of the kernels for few rows (f32: 1, 2, 4 or 8, chosen by the call).
 constexpr int kPagedDecRowsBf16 = 16, kPagedDecRowsF32 = 8;
+constexpr int kPagedTcRows = 256;  // rows of a unit of the tensor-core kernel (two MMA tiles)
+constexpr int kPagedF32Rows = 64;     // rows of a tile of the f32 kernel for chunks
 
 // Tensor maps of one layer's bf16 caches as rows [page][kv head][position] of head_dim.
 struct PagedMaps {
     CUtensorMap k_dec, v_dec;  // boxes of one page's run of positions, both 64-dim halves
+    CUtensorMap k_tc, v_tc;    // one 64-dim half of it
 };
 bool paged_decode_maps(PagedMaps* maps, const void* k, const void* v, int hd, int page_size, uint64_t rows);
 cudaError_t launch_paged_decode(int dtype, int hd, int tile_rows, const PagedMaps& maps, const PagedAttnArgs& a, int ctas,
                                 cudaStream_t s);
 
-cudaError_t launch_paged_attn_rows(int dtype, int hd, const PagedAttnArgs& a, int ctas, cudaStream_t s);
+bool paged_tc_maps(PagedMaps* maps, const void* k, const void* v, int hd, int page_size, uint64_t rows);
+cudaError_t launch_paged_tc(int hd, const PagedMaps& maps, const PagedAttnArgs& a, int ctas, cudaStream_t s);
+
+cudaError_t launch_paged_rows(int hd, const PagedAttnArgs& a, int ctas, cudaStream_t s);
 cudaError_t launch_paged_join(int dtype, int hd, int tile_rows, const PagedAttnArgs& a, int ctas, cudaStream_t s);
 
 struct PagedTablesArgs {

@@ -1,4 +1,4 @@
-// paged_attn.cu -- attention over a paged KV cache: the CUDA-core kernel and the
+// paged_attn.cu -- attention over a paged KV cache: the f32 kernel for chunks and the
 // kernel that joins the parts of tiles shared by several CTAs.
 //
 //   o_r = sum_p exp(x_rp - m_r) v_p / l_r,  x_rp = scale q_r . k_p,
@@ -20,14 +20,6 @@ namespace {
 
 using namespace paged;
 
-__device__ __forceinline__ void store4(float* p, const float (&f)[4]) {
-    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
-}
-__device__ __forceinline__ void store4(uint16_t* p, const float (&f)[4]) {
-    const __nv_bfloat162 x = __floats2bfloat162_rn(f[0], f[1]), y = __floats2bfloat162_rn(f[2], f[3]);
-    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-}
-
 // ---------------------------------------------------------------- rows kernel
 // 16 x 16 threads: thread (ty, tx) owns rows ty kRM .. + kRM, score columns tx + 16 j and
 // output dims 4 tx + 64 k.
@@ -35,18 +27,18 @@ constexpr int kRowsThreads = 256;
 
 template <int HD>
 struct RowsCfg {
-    static constexpr int kRM = 4, kRows = 16 * kRM;
+    static constexpr int kRM = kPagedF32Rows / 16, kRows = kPagedF32Rows;
     static constexpr int kKN = HD == 64 ? 4 : 2, kBlock = 16 * kKN;
     static constexpr int kLd = HD + 4, kLdP = kBlock + 4;
     static constexpr int kFloats = kRows * kLd + 2 * kBlock * kLd + kRows * kLdP;
     static constexpr int kPart = paged_part_floats(kRows, HD);
 };
 
-template <typename T, int HD>
+template <int HD>
 __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedAttnArgs a) {
     using C = RowsCfg<HD>;
     constexpr int RM = C::kRM, KN = C::kKN, KB = C::kBlock, LD = C::kLd, LDP = C::kLdP, DV = HD / 64;
-    constexpr int V = WeightTraits<T>::kVec, CH = HD / V;
+    constexpr int V = 4, CH = HD / V;
     extern __shared__ __align__(16) float sm[];
     float* Qs = sm;
     float* Ks = Qs + C::kRows * LD;
@@ -64,18 +56,13 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedAtt
         const Tile& t = w.t;
         for (int e = tid; e < C::kRows * CH; e += kRowsThreads) {
             const int r = e / CH, c = (e - r * CH) * V;
-            float f[V];
+            float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
             if (r < t.rows) {
                 const int tok = (t.r0 + r) / a.group, g = (t.r0 + r) - tok * a.group;
-                const T* src = static_cast<const T*>(a.q) + (t.s.row0 + tok) * a.q_stride +
-                               (size_t)(t.kvh * a.group + g) * HD + c;
-                WeightTraits<T>::unpack(*reinterpret_cast<const uint4*>(src), f);
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; i++) f[i] = 0.0f;
+                f = *reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + (t.s.row0 + tok) * a.q_stride +
+                                                     (size_t)(t.kvh * a.group + g) * HD + c);
             }
-#pragma unroll
-            for (int i = 0; i < V; i++) Qs[r * LD + c + i] = f[i];
+            *reinterpret_cast<float4*>(Qs + r * LD + c) = f;
         }
         int from[RM], to[RM];  // positions [from, to) that the thread's rows see
         float m[RM], l[RM];
@@ -96,24 +83,19 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedAtt
             __syncthreads();  // the block before is consumed (and Qs written, on the first pass)
             for (int e = tid; e < KB * CH; e += kRowsThreads) {
                 const int r = e / CH, c = (e - r * CH) * V, p = p0 + r;
-                float fk[V], fv[V];
-#pragma unroll
-                for (int i = 0; i < V; i++) fk[i] = fv[i] = 0.0f;
+                float4 k4 = make_float4(0.f, 0.f, 0.f, 0.f), v4 = k4;
                 if (p < t.hi) {
                     const int id = table[p >> a.page_shift];
                     if ((unsigned)id < (unsigned)a.n_pages) {
                         const size_t at = ((((size_t)id * a.n_kv + t.kvh) << a.page_shift) + (p & (page - 1))) * HD + c;
-                        WeightTraits<T>::unpack(ld_stream16(static_cast<const T*>(a.k) + at), fk);
-                        WeightTraits<T>::unpack(ld_stream16(static_cast<const T*>(a.v) + at), fv);
+                        k4 = *reinterpret_cast<const float4*>(static_cast<const float*>(a.k) + at);
+                        v4 = *reinterpret_cast<const float4*>(static_cast<const float*>(a.v) + at);
                     } else {
                         atomicCAS(a.status, 0u, (unsigned)kPagedTable);
                     }
                 }
-#pragma unroll
-                for (int i = 0; i < V; i++) {
-                    Ks[r * LD + c + i] = fk[i];
-                    Vs[r * LD + c + i] = fv[i];
-                }
+                *reinterpret_cast<float4*>(Ks + r * LD + c) = k4;
+                *reinterpret_cast<float4*>(Vs + r * LD + c) = v4;
             }
             __syncthreads();
             float s[RM][KN];
@@ -200,12 +182,11 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedAtt
                 if (r >= t.rows) continue;
                 const int tok = (t.r0 + r) / a.group, h = t.kvh * a.group + (t.r0 + r) - tok * a.group;
                 const float inv = l[i] > 0.0f || l[i] != l[i] ? 1.0f / l[i] : 0.0f;
-                T* dst = static_cast<T*>(a.out) + (t.s.row0 + tok) * a.out_stride + (size_t)h * HD;
+                float* dst = static_cast<float*>(a.out) + (t.s.row0 + tok) * a.out_stride + (size_t)h * HD;
 #pragma unroll
-                for (int k = 0; k < DV; k++) {
-                    const float f[4] = {o[i][k].x * inv, o[i][k].y * inv, o[i][k].z * inv, o[i][k].w * inv};
-                    store4(dst + 4 * tx + 64 * k, f);
-                }
+                for (int k = 0; k < DV; k++)
+                    *reinterpret_cast<float4*>(dst + 4 * tx + 64 * k) =
+                        make_float4(o[i][k].x * inv, o[i][k].y * inv, o[i][k].z * inv, o[i][k].w * inv);
                 if (a.lse && tx == 0)
                     a.lse[(size_t)(t.s.row0 + tok) * a.n_heads + h] = l[i] == 0.0f ? -INFINITY : m[i] * kLn2 + logf(l[i]);
             }
@@ -281,22 +262,21 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAtt
     }
 }
 
-template <typename T, int HD>
+template <int HD>
 cudaError_t rows_case(const PagedAttnArgs& a, int ctas, cudaStream_t s) {
     using C = RowsCfg<HD>;
     const int smem = C::kFloats * 4 + (a.n_seq + 1) * 4;
-    cudaError_t e = cudaFuncSetAttribute(paged_rows_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaError_t e = cudaFuncSetAttribute(paged_rows_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          C::kFloats * 4 + (kPagedMaxSeq + 1) * 4);
     if (e != cudaSuccess) return e;
-    paged_rows_kernel<T, HD><<<ctas, kRowsThreads, smem, s>>>(a);
+    paged_rows_kernel<HD><<<ctas, kRowsThreads, smem, s>>>(a);
     return cudaGetLastError();
 }
 
 }  // namespace
 
-cudaError_t launch_paged_attn_rows(int dtype, int hd, const PagedAttnArgs& a, int ctas, cudaStream_t s) {
-    if (dtype == RBT_MOE_DT_BF16) return hd == 64 ? rows_case<uint16_t, 64>(a, ctas, s) : rows_case<uint16_t, 128>(a, ctas, s);
-    return hd == 64 ? rows_case<float, 64>(a, ctas, s) : rows_case<float, 128>(a, ctas, s);
+cudaError_t launch_paged_rows(int hd, const PagedAttnArgs& a, int ctas, cudaStream_t s) {
+    return hd == 64 ? rows_case<64>(a, ctas, s) : rows_case<128>(a, ctas, s);
 }
 
 cudaError_t launch_paged_join(int dtype, int hd, int tile_rows, const PagedAttnArgs& a, int ctas, cudaStream_t s) {
