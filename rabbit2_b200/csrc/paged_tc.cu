@@ -14,8 +14,8 @@
 // the weights stay below 2^8.  v is the B operand as it lies in the pages (positions x
 // dims, "MN-major"), k likewise K-major: no transposed copy of the cache is made.
 //
-// Warps 0-3 and 4-7: the softmax of tiles 0 and 1; warp 8 issues the MMAs; warp 9 the
-// copies.  Every wait is bounded; one that runs out leaves a code, and every role goes on
+// Warps 0-3 and 4-7: the softmax of tiles 0 and 1; warps 8 and 9 issue their MMAs; warp 10
+// the copies.  Every wait is bounded; one that runs out leaves a code, and every role goes on
 // without waiting, so that the CTA ends.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -38,9 +38,10 @@ using namespace tc;
 
 constexpr int kTcTile = 128;               // rows of one MMA tile
 constexpr int kTcRows = kPagedTcRows;      // two tiles
-constexpr int kTcBlock = 128;              // positions of a block
-constexpr int kTcThreads = 320;
-constexpr uint64_t kTcWaitNs = 2000000000ull;
+constexpr int kTcBlock = 128;              // positions of a block: one stage of k and v
+constexpr int kTcStep = 64;                // positions of a softmax step
+constexpr int kTcThreads = 352;
+constexpr long long kTcWaitClocks = 4000000000ll;  // 2 s and more: far beyond any legitimate wait
 constexpr float kTcRescale = 8.0f;         // log2 of the largest weight before the maximum moves
 
 template <int HD>
@@ -57,9 +58,9 @@ struct TcCfg {
 };
 
 struct TcBars {
-    uint64_t q_full[2], s_full[2], p_full[2], pv_done[2];
+    uint64_t q_full[2], s_full[2][2], p_full[2][2], pv_done[2];  // [tile][buffer]
     uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
-    uint64_t drain;
+    uint64_t v_tail, drain;
     uint32_t tmem;
 };
 
@@ -87,20 +88,156 @@ __device__ __forceinline__ uint32_t sw128(int r, int c) {  // 16-byte chunk c of
     return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4));
 }
 
+// Two f32 values as one operand of the packed instructions.
+__device__ __forceinline__ uint64_t pair2(float x, float y) {
+    return (uint64_t)__float_as_uint(x) | (uint64_t)__float_as_uint(y) << 32;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(x), "l"(y), "l"(z));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
+    return d;
+}
+
+// Two weights (0 .. 2^8) as bf16, to nearest with ties upwards: two integer adds and a byte
+// permute.  The conversion instruction shares the special-function pipe with ex2, which
+// bounds the softmax.  (NaN may become a number here; the row's sum keeps it.)
+__device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
+    return __byte_perm(__float_as_uint(x) + 0x8000u, __float_as_uint(y) + 0x8000u, 0x7632);
+}
+
 // A wait that gives up once, for good: the softmax then passes its other barriers at once.
 struct Waiter {
     bool ok = true;
     unsigned* status;
     __device__ __forceinline__ void operator()(uint64_t* bar, uint32_t parity) {
-        if (ok && !mbar_wait_bounded(bar, parity, kTcWaitNs)) {
-            ok = false;
-            atomicCAS(status, 0u, (unsigned)kPagedWait);
-        }
+        if (!ok || mbar_try_wait(bar, parity)) return;
+        const long long t0 = clock64();
+        while (!mbar_try_wait(bar, parity))
+            if (clock64() - t0 > kTcWaitClocks) {
+                ok = false;
+                atomicCAS(status, 0u, (unsigned)kPagedWait);
+                return;
+            }
+    }
+    __device__ __forceinline__ bool one(uint64_t* bar, uint32_t parity) {
+        (*this)(bar, parity);
+        return ok;
     }
     // for a whole warp, which goes on only if every lane may
     __device__ __forceinline__ bool warp(uint64_t* bar, uint32_t parity) {
         (*this)(bar, parity);
         return ok = __all_sync(FULL_MASK, ok);
+    }
+};
+
+// Softmax steps of tile i in blocks [first, first + n) of a unit's range: up to the last
+// position that a row of the tile sees.  rows: those of the tile (<= 0: none).
+__device__ __forceinline__ int tile_steps(const PagedAttnArgs& a, const Tile& t, int i, int first, int n, int& rows) {
+    rows = min(kTcTile, t.rows - i * kTcTile);
+    if (rows <= 0) return 0;
+    const int hi = a.causal ? min(t.hi, t.off + (t.r0 + i * kTcTile + rows - 1) / a.group + 1) : t.hi;
+    return max(0, min(n * (kTcBlock / kTcStep), (hi - first * kTcBlock + kTcStep - 1) / kTcStep));
+}
+
+// The thread that issues tile I's MMAs.  One thread per tile: an issue waits until the
+// tensor cores have room, and the waits and commits between two groups of MMAs of one tile
+// leave room for the other's.
+template <int HD, int I>
+struct Issuer {
+    using C = TcCfg<HD>;
+    static constexpr uint32_t kIdS = idesc_bf16_f32(kTcTile, kTcStep);
+    static constexpr uint32_t kIdO = idesc_bf16_f32(kTcTile, HD) | (1u << 16);  // B is MN-major
+    static constexpr uint32_t kHalfStep = kTcStep * 128;  // bytes from a block's first 64 positions to its second
+    const PagedAttnArgs& a;
+    TcBars& bars;
+    Waiter& wait;
+    uint32_t tmem, q, k, v;              // descriptors' lower halves (stage 0 of k and v)
+    uint32_t j0 = 0, n_q = 0, n_s = 0;   // blocks, phases of q_full and steps before this segment
+    int steps, k_seen, v_seen;           // of this segment; blocks whose copies have been waited for
+
+    __device__ __forceinline__ Issuer(const PagedAttnArgs& a, TcBars& bars, uint8_t* smem, uint32_t tmem, Waiter& wait)
+        : a(a), bars(bars), wait(wait), tmem(tmem) {
+        q = (uint32_t)sw128_kmajor_desc(smem_u32(smem + C::oQ + I * C::kTileBytes));
+        k = (uint32_t)sw128_kmajor_desc(smem_u32(smem + C::oK));
+        v = (uint32_t)mn_desc(smem_u32(smem + C::oV), C::kHalf);
+    }
+    static __device__ __forceinline__ uint64_t desc(uint32_t lo) {
+        return (uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29)) << 32 | lo;
+    }
+    __device__ __forceinline__ uint32_t stage(int block) const { return (j0 + block) % C::kStages; }
+    __device__ __forceinline__ bool need(int block, int& seen, uint64_t* full) {
+        if (block < seen) return true;
+        seen = block + 1;
+        return wait.one(&full[stage(block)], ((j0 + block) / C::kStages) & 1);
+    }
+    // Scores of step s into its buffer (steps so far) & 1.
+    __device__ __forceinline__ bool scores(int s) {
+        if (!need(s >> 1, k_seen, bars.k_full)) return false;
+        const uint32_t u = n_s + s, d = tmem + C::cS + I * 128 + (u & 1) * 64;
+        const uint32_t kb = k + ((stage(s >> 1) * C::kTileBytes + (s & 1) * kHalfStep) >> 4);
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; kk++) {
+            const uint32_t o = ((kk >> 2) * C::kHalf + (kk & 3) * 32) >> 4;
+            mma_bf16(d, desc(q + o), desc(kb + o), kIdS, kk != 0);
+        }
+        mma_commit(&bars.s_full[I][u & 1]);
+        if ((s & 1) || s + 1 == steps) mma_commit(&bars.k_empty[stage(s >> 1)]);
+        return true;
+    }
+    // O += P v of step s.
+    __device__ __forceinline__ bool product(int s) {
+        if (!need(s >> 1, v_seen, bars.v_full)) return false;
+        const uint32_t u = n_s + s, p = tmem + C::cS + I * 128 + (u & 1) * 64;
+        const uint32_t vb = v + ((stage(s >> 1) * C::kTileBytes + (s & 1) * kHalfStep) >> 4);
+        if (!wait.one(&bars.p_full[I][u & 1], (u >> 1) & 1)) return false;
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < kTcStep / 16; kk++)
+            mma_bf16_ts(tmem + C::cO + I * 128, p + kk * 8, desc(vb + (kk * 2048 >> 4)), kIdO, (s | kk) != 0);
+        mma_commit(&bars.pv_done[I]);
+        if ((s & 1) || s + 1 == steps) mma_commit(&bars.v_empty[stage(s >> 1)]);
+        return true;
+    }
+    template <typename W>
+    __device__ __forceinline__ bool segment(const W& w) {
+        int rows;
+        steps = tile_steps(a, w.t, I, w.first, w.n, rows);
+        k_seen = v_seen = 0;
+        if (rows > 0 && !wait.one(&bars.q_full[I], n_q++ & 1)) return false;
+        for (int s = 0; s < min(2, steps); s++)  // (the buffers are free: all products of the segment before were waited for)
+            if (!scores(s)) return false;
+        for (int s = 0; s < steps; s++) {
+            if (!product(s)) return false;
+            // the scores after next take the place of the weights that this product reads
+            if (!wait.one(&bars.pv_done[I], (n_s + s) & 1)) return false;
+            if (s + 2 < steps && !scores(s + 2)) return false;
+        }
+        // Blocks that this tile has no step in are freed in turn, too: each when it has come, so that
+        // an arrival never counts for the block that was in the stage before.
+        for (int b = (steps + 1) / 2; b < w.n; b++) {
+            if (!need(b, k_seen, bars.k_full)) return false;
+            mbar_arrive(&bars.k_empty[stage(b)]);
+            if (!need(b, v_seen, bars.v_full)) return false;
+            mbar_arrive(&bars.v_empty[stage(b)]);
+        }
+        n_s += steps;
+        j0 += w.n;
+        return true;
+    }
+    template <typename W>
+    __device__ __forceinline__ void run(W& w) {
+        while (w.next(a))
+            if (!segment(w)) break;
+        // every MMA has completed before TMEM is freed
+        mma_commit(&bars.drain);
+        wait.ok = true;
+        wait(&bars.drain, 0);
     }
 };
 
@@ -118,17 +255,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; i++) {
             mbar_init(&bars.q_full[i], kTcTile);
-            mbar_init(&bars.s_full[i], 1);
-            mbar_init(&bars.p_full[i], kTcTile);
             mbar_init(&bars.pv_done[i], 1);
+            for (int b = 0; b < 2; b++) {
+                mbar_init(&bars.s_full[i][b], 1);
+                mbar_init(&bars.p_full[i][b], kTcTile);
+            }
         }
         for (int i = 0; i < C::kStages; i++) {
             mbar_init(&bars.k_full[i], 1);
-            mbar_init(&bars.k_empty[i], 1);
+            mbar_init(&bars.k_empty[i], 2);
             mbar_init(&bars.v_full[i], 1);
-            mbar_init(&bars.v_empty[i], 1);
+            mbar_init(&bars.v_empty[i], 2);
         }
-        mbar_init(&bars.drain, 1);
+        mbar_init(&bars.v_tail, 1);
+        mbar_init(&bars.drain, 2);
         fence_mbar_init();
         prefetch_tmap(&tm_k);
         prefetch_tmap(&tm_v);
@@ -146,10 +286,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     Waiter wait;
     wait.status = a.status;
 
-    if (warp == 9) {
+    if (warp == 10) {
         // ------------------------------------------------ copies
         const int box = min(1 << a.page_shift, kTcBlock), n_box = kTcBlock / box, box_shift = min(a.page_shift, 7);
-        uint32_t j = 0;
+        uint32_t j = 0, n_tail = 0;
         while (w.next(a)) {
             const int32_t* table = a.table + (size_t)w.t.seq * a.table_stride;
             for (int b = w.first; b < w.first + w.n; b++, j++) {
@@ -181,9 +321,28 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     wait.ok = false;
                     break;
                 }
-                if (lane == 0) mbar_arrive_expect_tx(&bars.v_full[st], bytes);
+                const bool tail = p0 + kTcBlock > w.t.hi;
+                uint64_t* bar = tail ? &bars.v_tail : &bars.v_full[st];
+                if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
                 __syncwarp();
-                if (on) tma_load_3d(smem + C::oV + st * C::kTileBytes + at, &tm_v, &bars.v_full[st], 0, y, half);
+                if (on) tma_load_3d(smem + C::oV + st * C::kTileBytes + at, &tm_v, bar, 0, y, half);
+                if (tail) {
+                    // what lies behind the last position is not a number, perhaps, which a weight of 0 would not hide
+                    const bool got = wait.warp(&bars.v_tail, n_tail++ & 1);
+                    const int r0 = max(0, w.t.hi - p0);
+                    for (int e = lane; e < (kTcBlock - r0) * (HD / 8); e += 32) {
+                        const int r = r0 + e / (HD / 8), c = e % (HD / 8);
+                        *reinterpret_cast<uint4*>(smem + C::oV + st * C::kTileBytes + (c >> 3) * C::kHalf + sw128(r, c & 7)) =
+                            make_uint4(0, 0, 0, 0);
+                    }
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars.v_full[st]);
+                    if (!got) {
+                        j++;
+                        break;
+                    }
+                }
             }
             if (!wait.ok) break;
         }
@@ -194,85 +353,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             wait(&bars.v_full[i % C::kStages], (i / C::kStages) & 1);
         }
     } else if (warp == 8) {
-        // ------------------------------------------------ MMAs (lane 0 issues)
-        constexpr uint32_t idS = idesc_bf16_f32(kTcTile, kTcBlock);
-        constexpr uint32_t idO = idesc_bf16_f32(kTcTile, HD) | (1u << 16);  // B is MN-major
-        uint32_t j0 = 0, nq[2] = {0, 0}, np[2] = {0, 0};  // blocks before this segment; phases used of q_full, and p_full
-        const auto issue_s = [&](int i, uint32_t st) {
-            if (lane == 0) {
-                const uint32_t sq = smem_u32(smem + C::oQ + i * C::kTileBytes);
-                const uint32_t sk = smem_u32(smem + C::oK + st * C::kTileBytes);
-#pragma unroll
-                for (int kk = 0; kk < HD / 16; kk++) {
-                    const uint32_t o = (kk >> 2) * C::kHalf + (kk & 3) * 32;
-                    mma_bf16(tmem + C::cS + i * 128, sw128_kmajor_desc(sq + o), sw128_kmajor_desc(sk + o), idS, kk != 0);
-                }
-                mma_commit(&bars.s_full[i]);
-            }
-            __syncwarp();
-        };
-        const auto segment = [&]() -> bool {
-            const int nt = w.t.rows > kTcTile ? 2 : 1;
-            for (int i = 0; i < nt; i++) {
-                if (!wait.warp(&bars.q_full[i], nq[i] & 1)) return false;
-                nq[i]++;
-                if (i == 0 && !wait.warp(&bars.k_full[j0 % C::kStages], (j0 / C::kStages) & 1)) return false;
-                tc_fence_after();
-                issue_s(i, j0 % C::kStages);  // (S_i is free: the product that read P_i was waited for)
-            }
-            if (lane == 0) mma_commit(&bars.k_empty[j0 % C::kStages]);
-            for (int n = 0; n < w.n; n++) {
-                const uint32_t j = j0 + n, st = j % C::kStages, st1 = (j + 1) % C::kStages;
-                for (int i = 0; i < nt; i++) {
-                    if (i == 0) {
-                        if (!wait.warp(&bars.v_full[st], (j / C::kStages) & 1)) return false;
-                        const int p0 = (w.first + n) * kTcBlock;
-                        if (p0 + kTcBlock > w.t.hi) {
-                            // what lies behind the last position is not a number, perhaps, which a weight of 0 would not hide
-                            const int r0 = max(0, w.t.hi - p0);
-                            for (int e = lane; e < (kTcBlock - r0) * (HD / 8); e += 32) {
-                                const int r = r0 + e / (HD / 8), c = e % (HD / 8);
-                                *reinterpret_cast<uint4*>(smem + C::oV + st * C::kTileBytes + (c >> 3) * C::kHalf +
-                                                          sw128(r, c & 7)) = make_uint4(0, 0, 0, 0);
-                            }
-                            fence_async_smem();
-                            __syncwarp();
-                        }
-                    }
-                    if (!wait.warp(&bars.p_full[i], np[i] & 1)) return false;
-                    tc_fence_after();
-                    if (lane == 0) {
-                        const uint32_t sv = smem_u32(smem + C::oV + st * C::kTileBytes);
-#pragma unroll
-                        for (int kk = 0; kk < kTcBlock / 16; kk++)
-                            mma_bf16_ts(tmem + C::cO + i * 128, tmem + C::cS + i * 128 + kk * 8, mn_desc(sv + kk * 2048, C::kHalf),
-                                        idO, (n | kk) != 0);
-                        mma_commit(&bars.pv_done[i]);
-                        if (i == nt - 1) mma_commit(&bars.v_empty[st]);
-                    }
-                    __syncwarp();
-                    // S_i of the next block takes the place of P_i: after the product that reads P_i, which the
-                    // softmax also counts on (O_i is at rest whenever s_full[i] arrives)
-                    if (!wait.warp(&bars.pv_done[i], np[i] & 1)) return false;
-                    np[i]++;
-                    if (n + 1 < w.n) {
-                        if (i == 0 && !wait.warp(&bars.k_full[st1], ((j + 1) / C::kStages) & 1)) return false;
-                        tc_fence_after();
-                        issue_s(i, st1);
-                        if (i == nt - 1 && lane == 0) mma_commit(&bars.k_empty[st1]);
-                    }
-                }
-            }
-            j0 += w.n;
-            return true;
-        };
-        while (w.next(a))
-            if (!segment()) break;
-        // every MMA has completed before TMEM is freed
-        if (lane == 0) mma_commit(&bars.drain);
+        // ------------------------------------------------ MMAs: one thread per tile
+        if (lane == 0) {
+            Issuer<HD, 0> mma(a, bars, smem, tmem, wait);
+            mma.run(w);
+        }
         __syncwarp();
-        wait.ok = true;
-        wait(&bars.drain, 0);
+    } else if (warp == 9) {
+        if (lane == 0) {
+            Issuer<HD, 1> mma(a, bars, smem, tmem, wait);
+            mma.run(w);
+        }
         __syncwarp();
     } else {
         // ------------------------------------------------ softmax: thread = row
@@ -282,7 +373,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // a negative scale turns the sign of q instead; a scale of 0 stays above it, so that -inf stays -inf
         const float k2 = fmaxf(fabsf(a.scale) * kLog2e, 1e-37f);
         const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
-        uint32_t ns = 0;  // phases used of s_full and pv_done
+        uint32_t ns = 0;  // steps so far
         while (w.next(a)) {
             const Tile& t = w.t;
             const int row = i * kTcTile + r;  // in the unit
@@ -310,28 +401,30 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 mbar_arrive(&bars.q_full[i]);
             }
             float m = -INFINITY, l = 0.0f;
-            for (int n = 0; n < w.n; n++) {
-                const int p0 = (w.first + n) * kTcBlock;
-                wait(&bars.s_full[i], ns & 1);
-                ns++;
+            int tile_rows;
+            const int steps = tile_steps(a, t, i, w.first, w.n, tile_rows);
+            for (int n = 0; n < steps; n++, ns++) {
+                const int p0 = w.first * kTcBlock + n * kTcStep;
+                const uint32_t buf = tS + (ns & 1) * 64;
+                wait(&bars.s_full[i][ns & 1], (ns >> 1) & 1);
                 __syncwarp();
                 tc_fence_after();
-                uint32_t v[128];
-#pragma unroll
-                for (int c = 0; c < 4; c++) tmem_ld_32x32b_x32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&v[32 * c]));
+                uint32_t v[64];
+                tmem_ld_32x32b_x32(buf, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+                tmem_ld_32x32b_x32(buf + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
                 tmem_ld_wait();
-                float top = -INFINITY;
                 const int c0 = from - p0, c1 = to - p0;  // columns [c0, c1) are seen
-                if (__all_sync(FULL_MASK, c0 <= 0 && c1 >= kTcBlock)) {
+                if (!__all_sync(FULL_MASK, c0 <= 0 && c1 >= kTcStep)) {
 #pragma unroll
-                    for (int c = 0; c < 128; c++) top = fmaxf(top, __uint_as_float(v[c]));
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 128; c++) {
+                    for (int c = 0; c < 64; c++)
                         if (c < c0 || c >= c1) v[c] = 0xff800000u;
-                        top = fmaxf(top, __uint_as_float(v[c]));
-                    }
                 }
+                float part4[4];  // four chains of maxima
+#pragma unroll
+                for (int c = 0; c < 4; c++) part4[c] = __uint_as_float(v[c]);
+#pragma unroll
+                for (int c = 4; c < 64; c++) part4[c & 3] = fmaxf(part4[c & 3], __uint_as_float(v[c]));
+                const float top = fmaxf(fmaxf(part4[0], part4[1]), fmaxf(part4[2], part4[3]));
                 // (equal infinities need no step; m = -inf until the row sees something)
                 const bool move = top > m && (m == -INFINITY || (top - m) * k2 > kTcRescale);
                 float alpha = 1.0f;
@@ -341,6 +434,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     l *= alpha;
                 }
                 if (n > 0 && __any_sync(FULL_MASK, move)) {
+                    wait(&bars.pv_done[i], (ns - 1) & 1);  // O is at rest then: the next product needs this step's weights
+                    __syncwarp();
+                    tc_fence_after();
 #pragma unroll 1
                     for (int c = 0; c < HD; c += 32) {
                         uint32_t o[32];
@@ -352,26 +448,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                 }
                 const float mk = m == -INFINITY ? 0.0f : m * k2;
+                const uint64_t kk = pair2(k2, k2), mm = pair2(-mk, -mk);
+                uint64_t sum[2] = {0, 0};
+                uint32_t p[32];
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    uint32_t p[32];
-                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int c = 0; c < 32; c++) {
-                        const float x = ex2(fmaf(__uint_as_float(v[64 * h + 2 * c]), k2, -mk));
-                        const float y = ex2(fmaf(__uint_as_float(v[64 * h + 2 * c + 1]), k2, -mk));
-                        sum[c & 3] += x + y;
-                        const __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
-                        p[c] = *reinterpret_cast<const uint32_t*>(&b);
-                    }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                    tmem_st_32x32b_x32(tS + 32 * h, p);
+                for (int c = 0; c < 32; c++) {
+                    const uint64_t z = fma2((uint64_t)v[2 * c] | (uint64_t)v[2 * c + 1] << 32, kk, mm);
+                    const float x = ex2(__uint_as_float((uint32_t)z)), y = ex2(__uint_as_float((uint32_t)(z >> 32)));
+                    sum[c & 1] = add2(sum[c & 1], pair2(x, y));
+                    p[c] = pack_bf16(x, y);
                 }
+                tmem_st_32x32b_x32(buf, p);
+                sum[0] = add2(sum[0], sum[1]);
+                l += __uint_as_float((uint32_t)sum[0]) + __uint_as_float((uint32_t)(sum[0] >> 32));
                 tmem_st_wait();
                 tc_fence_before();
-                mbar_arrive(&bars.p_full[i]);
+                // Each product is seen over before the next is let start: a barrier's parity tells only
+                // one phase from the next, and the MMA warp counts on the same.
+                if (n > 0) wait(&bars.pv_done[i], (ns - 1) & 1);
+                mbar_arrive(&bars.p_full[i][ns & 1]);
             }
-            wait(&bars.pv_done[i], (ns - 1) & 1);
+            if (steps) wait(&bars.pv_done[i], (ns - 1) & 1);
             __syncwarp();
             tc_fence_after();
             const float scale = w.whole ? (l > 0.0f || l != l ? 1.0f / l : 0.0f) : 1.0f;
@@ -392,6 +489,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 uint32_t o[32];
                 tmem_ld_32x32b_x32(tO + c, o);
                 tmem_ld_wait();
+                if (!steps) {  // no product has written O
+#pragma unroll
+                    for (int e = 0; e < 32; e++) o[e] = 0;
+                }
                 if (!live) continue;
                 if (w.whole) {
 #pragma unroll
