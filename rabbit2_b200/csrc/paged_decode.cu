@@ -110,6 +110,7 @@ __device__ __forceinline__ void produce(const PagedAttnArgs& a, const Share& sha
 __device__ __forceinline__ void await(const PagedAttnArgs& a, Ring* ring, uint32_t j, bool& ok) {
     if (ok) ok = __all_sync(FULL_MASK, mbar_wait_bounded(&ring->full[j % kDecStages], (j / kDecStages) & 1, kDecWaitNs));
     if (!ok && (threadIdx.x & 31) == 0) atomicCAS(a.status, 0u, (unsigned)kPagedWait);
+    __syncwarp();
 }
 
 // The four warps' parts of a segment, in shared memory: two sets of maxima and sums (the

@@ -110,6 +110,79 @@ __device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
     return __byte_perm(__float_as_uint(x) + 0x8000u, __float_as_uint(y) + 0x8000u, 0x7632);
 }
 
+// Values that a wait made valid: what uses them stays behind it.
+template <int N>
+__device__ __forceinline__ void tie(uint32_t (&v)[N]) {
+#pragma unroll
+    for (int c = 0; c < N; c++) asm volatile("" : "+r"(v[c]));
+}
+__device__ __forceinline__ void load_scores(uint32_t at, uint32_t (&v)[64]) {
+    tmem_ld_32x32b_x32(at, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+    tmem_ld_32x32b_x32(at + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+    tmem_ld_wait();
+    tie(v);
+}
+// the scores outside columns [c0, c1) as -inf
+__device__ __forceinline__ void mask_scores(uint32_t (&v)[64], int c0, int c1) {
+    if (!__all_sync(FULL_MASK, c0 <= 0 && c1 >= 64)) {
+#pragma unroll
+        for (int c = 0; c < 64; c++)
+            if (c < c0 || c >= c1) v[c] = 0xff800000u;
+    }
+}
+
+__device__ __forceinline__ float max3(float x, float y, float z) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(x), "f"(y), "f"(z));
+    return d;
+}
+__device__ __forceinline__ float max64(const uint32_t (&v)[64]) {  // four chains of three-way maxima
+    float t[4];
+#pragma unroll
+    for (int c = 0; c < 4; c++) t[c] = __uint_as_float(v[c]);
+#pragma unroll
+    for (int c = 4; c < 60; c += 8)
+#pragma unroll
+        for (int e = 0; e < 4; e++) t[e] = max3(t[e], __uint_as_float(v[c + e]), __uint_as_float(v[c + 4 + e]));
+#pragma unroll
+    for (int e = 0; e < 4; e++) t[e] = fmaxf(t[e], __uint_as_float(v[60 + e]));
+    return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+}
+
+// A row's softmax: maximum m of the scores so far (or one within 2^kTcRescale of it) and sum l
+// of the weights 2^((s - m) k2).
+struct Row {
+    float k2, m = -INFINITY, l = 0.0f;
+    __device__ __forceinline__ explicit Row(float k2) : k2(k2) {}
+    // (equal infinities need no step; m = -inf until the row sees something)
+    __device__ __forceinline__ bool too_large(float top) const {
+        return top > m && (m == -INFINITY || (top - m) * k2 > kTcRescale);
+    }
+    // m for scores up to `top`; the factor of what was summed before
+    __device__ __forceinline__ float raise(float top) {
+        if (!too_large(top)) return 1.0f;
+        const float alpha = m == -INFINITY ? 0.0f : ex2((m - top) * k2);
+        m = top;
+        l *= alpha;
+        return alpha;
+    }
+    // the weights as bf16 pairs, and their sum
+    __device__ __forceinline__ float weights(const uint32_t (&v)[64], uint32_t (&p)[32]) const {
+        const float mk = m == -INFINITY ? 0.0f : m * k2;
+        const uint64_t kk = pair2(k2, k2), mm = pair2(-mk, -mk);
+        uint64_t sum[2] = {0, 0};
+#pragma unroll
+        for (int c = 0; c < 32; c++) {
+            const uint64_t z = fma2((uint64_t)v[2 * c] | (uint64_t)v[2 * c + 1] << 32, kk, mm);
+            const float x = ex2(__uint_as_float((uint32_t)z)), y = ex2(__uint_as_float((uint32_t)(z >> 32)));
+            sum[c & 1] = add2(sum[c & 1], pair2(x, y));
+            p[c] = pack_bf16(x, y);
+        }
+        sum[0] = add2(sum[0], sum[1]);
+        return __uint_as_float((uint32_t)sum[0]) + __uint_as_float((uint32_t)(sum[0] >> 32));
+    }
+};
+
 // A wait that gives up once, for good: the softmax then passes its other barriers at once.
 struct Waiter {
     bool ok = true;
@@ -209,7 +282,7 @@ struct Issuer {
         int rows;
         steps = tile_steps(a, w.t, I, w.first, w.n, rows);
         k_seen = v_seen = 0;
-        if (rows > 0 && !wait.one(&bars.q_full[I], n_q++ & 1)) return false;
+        if (steps && !wait.one(&bars.q_full[I], n_q++ & 1)) return false;
         for (int s = 0; s < min(2, steps); s++)  // (the buffers are free: all products of the segment before were waited for)
             if (!scores(s)) return false;
         for (int s = 0; s < steps; s++) {
@@ -383,7 +456,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const int pos = t.off + tok;
             const int to = !live ? 0 : a.causal ? min(t.s.len, pos + 1) : t.s.len;
             const int from = a.window ? max(0, pos - a.window + 1) : 0;
-            {
+            int tile_rows;
+            const int steps = tile_steps(a, t, i, w.first, w.n, tile_rows);
+            if (steps) {  // (without a step nobody waits for q, and a second arrival could pass for the first)
                 const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
                                                                   (t.s.row0 + tok) * a.q_stride + (size_t)head * HD);
                 uint8_t* dst = smem + C::oQ + i * C::kTileBytes;
@@ -400,74 +475,59 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 tc_fence_before();
                 mbar_arrive(&bars.q_full[i]);
             }
-            float m = -INFINITY, l = 0.0f;
-            int tile_rows;
-            const int steps = tile_steps(a, t, i, w.first, w.n, tile_rows);
+            Row row_state(k2);
             for (int n = 0; n < steps; n++, ns++) {
                 const int p0 = w.first * kTcBlock + n * kTcStep;
                 const uint32_t buf = tS + (ns & 1) * 64;
+                uint32_t v[64], p[32];
+                float sum = 0.0f;
                 wait(&bars.s_full[i][ns & 1], (ns >> 1) & 1);
                 __syncwarp();
                 tc_fence_after();
-                uint32_t v[64];
-                tmem_ld_32x32b_x32(buf, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
-                tmem_ld_32x32b_x32(buf + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
-                tmem_ld_wait();
-                const int c0 = from - p0, c1 = to - p0;  // columns [c0, c1) are seen
-                if (!__all_sync(FULL_MASK, c0 <= 0 && c1 >= kTcStep)) {
-#pragma unroll
-                    for (int c = 0; c < 64; c++)
-                        if (c < c0 || c >= c1) v[c] = 0xff800000u;
+                load_scores(buf, v);
+                mask_scores(v, from - p0, to - p0);
+                // The weights with the maximum so far, while another pipe looks for a larger one; where that is
+                // larger by too much (hardly ever after a row's first steps), again with the new one.
+                bool again = n == 0;
+                if (!again) {
+                    sum = row_state.weights(v, p);
+                    again = __any_sync(FULL_MASK, row_state.too_large(max64(v)));
                 }
-                float part4[4];  // four chains of maxima
-#pragma unroll
-                for (int c = 0; c < 4; c++) part4[c] = __uint_as_float(v[c]);
-#pragma unroll
-                for (int c = 4; c < 64; c++) part4[c & 3] = fmaxf(part4[c & 3], __uint_as_float(v[c]));
-                const float top = fmaxf(fmaxf(part4[0], part4[1]), fmaxf(part4[2], part4[3]));
-                // (equal infinities need no step; m = -inf until the row sees something)
-                const bool move = top > m && (m == -INFINITY || (top - m) * k2 > kTcRescale);
-                float alpha = 1.0f;
-                if (move) {
-                    alpha = m == -INFINITY ? 0.0f : ex2((m - top) * k2);
-                    m = top;
-                    l *= alpha;
-                }
-                if (n > 0 && __any_sync(FULL_MASK, move)) {
-                    wait(&bars.pv_done[i], (ns - 1) & 1);  // O is at rest then: the next product needs this step's weights
-                    __syncwarp();
-                    tc_fence_after();
-#pragma unroll 1
-                    for (int c = 0; c < HD; c += 32) {
-                        uint32_t o[32];
-                        tmem_ld_32x32b_x32(tO + c, o);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                        tmem_st_32x32b_x32(tO + c, o);
+                if (again) {
+                    if (n > 0) {
+                        load_scores(buf, v);
+                        mask_scores(v, from - p0, to - p0);
                     }
-                }
-                const float mk = m == -INFINITY ? 0.0f : m * k2;
-                const uint64_t kk = pair2(k2, k2), mm = pair2(-mk, -mk);
-                uint64_t sum[2] = {0, 0};
-                uint32_t p[32];
+                    const float alpha = row_state.raise(max64(v));
+                    __syncwarp();
+                    if (n > 0) {
+                        wait(&bars.pv_done[i], (ns - 1) & 1);  // O is at rest then: the next product needs this step's weights
+                        __syncwarp();
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < HD; c += 32) {
+                            uint32_t o[32];
+                            tmem_ld_32x32b_x32(tO + c, o);
+                            tmem_ld_wait();
+                            tie(o);
 #pragma unroll
-                for (int c = 0; c < 32; c++) {
-                    const uint64_t z = fma2((uint64_t)v[2 * c] | (uint64_t)v[2 * c + 1] << 32, kk, mm);
-                    const float x = ex2(__uint_as_float((uint32_t)z)), y = ex2(__uint_as_float((uint32_t)(z >> 32)));
-                    sum[c & 1] = add2(sum[c & 1], pair2(x, y));
-                    p[c] = pack_bf16(x, y);
+                            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                            tmem_st_32x32b_x32(tO + c, o);
+                        }
+                    }
+                    sum = row_state.weights(v, p);
                 }
+                __syncwarp();
                 tmem_st_32x32b_x32(buf, p);
-                sum[0] = add2(sum[0], sum[1]);
-                l += __uint_as_float((uint32_t)sum[0]) + __uint_as_float((uint32_t)(sum[0] >> 32));
+                row_state.l += sum;
                 tmem_st_wait();
                 tc_fence_before();
                 // Each product is seen over before the next is let start: a barrier's parity tells only
-                // one phase from the next, and the MMA warp counts on the same.
+                // one phase from the next, and the MMA warps count on the same.
                 if (n > 0) wait(&bars.pv_done[i], (ns - 1) & 1);
                 mbar_arrive(&bars.p_full[i][ns & 1]);
             }
+            const float m = row_state.m, l = row_state.l;
             if (steps) wait(&bars.pv_done[i], (ns - 1) & 1);
             __syncwarp();
             tc_fence_after();
@@ -487,14 +547,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
             for (int c = 0; c < HD; c += 32) {
                 uint32_t o[32];
+                __syncwarp();  // the rows of a warp part ways below, and tcgen05.ld is the whole warp's
                 tmem_ld_32x32b_x32(tO + c, o);
                 tmem_ld_wait();
+                tie(o);
                 if (!steps) {  // no product has written O
 #pragma unroll
                     for (int e = 0; e < 32; e++) o[e] = 0;
                 }
-                if (!live) continue;
-                if (w.whole) {
+                if (live && w.whole) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 8) {
                         uint32_t b[4];
@@ -506,12 +567,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         }
                         *reinterpret_cast<uint4*>(out + c + e) = make_uint4(b[0], b[1], b[2], b[3]);
                     }
-                } else {
+                } else if (live) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 4)
                         *reinterpret_cast<uint4*>(po + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                 }
             }
+            __syncwarp();
             tc_fence_before();
             if (!w.whole && w.head && threadIdx.x == 0)
                 a.join[blockIdx.x] = PagedJoin{w.finisher(), t.r0, t.rows, t.s.row0, t.kvh};
