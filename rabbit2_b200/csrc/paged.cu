@@ -27,6 +27,7 @@ struct RbtPaged {
     unsigned* status = nullptr;
     float* part = nullptr;          // partial tiles of the attention
     rbt::PagedJoin* join = nullptr;
+    unsigned* arrived = nullptr;
 };
 
 namespace {
@@ -140,13 +141,28 @@ int rbt_paged_create(RbtPaged** out, const RbtPagedConfig* cfg, int device) {
         return fail("out of host memory");
     }
     cudaError_t e = cudaDeviceGetAttribute(&p->sm_count, cudaDevAttrMultiProcessorCount, device);
-    if (e == cudaSuccess) e = cudaMalloc((void**)&p->status, sizeof(unsigned));
-    if (e == cudaSuccess) e = cudaMemset(p->status, 0, sizeof(unsigned));
-    if (e == cudaSuccess && c.n_layers > 0) {
-        // two partial tiles per CTA of the largest launch: 256 rows on every SM, or 64 rows on twice as many CTAs
+    // one block: the status word and the arrival counters, the joins, and two partial tiles per CTA of
+    // the largest launch: 256 rows on every SM, or 64 rows on twice as many CTAs
+    size_t words = 64, joins = 0, parts = 0;
+    if (c.n_layers > 0) {
+        words += (size_t)2 * p->sm_count;
+        joins = (size_t)2 * p->sm_count * sizeof(PagedJoin);
         const int rows = c.dtype == RBT_MOE_DT_BF16 ? kPagedTcRows : 2 * kPagedF32Rows;
-        e = cudaMalloc((void**)&p->part, (size_t)p->sm_count * 2 * paged_part_floats(rows, c.head_dim) * sizeof(float));
-        if (e == cudaSuccess) e = cudaMalloc((void**)&p->join, (size_t)2 * p->sm_count * sizeof(PagedJoin));
+        parts = (size_t)p->sm_count * 2 * paged_part_floats(rows, c.head_dim) * sizeof(float);
+    }
+    words = (words * 4 + 255) / 256 * 256;
+    joins = (joins + 255) / 256 * 256;
+    if (e == cudaSuccess) e = cudaMalloc((void**)&p->status, words + joins + parts);
+    if (e == cudaSuccess) e = cudaMemset(p->status, 0, words);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(0);  // before calls on streams that do not wait for this one
+    if (e == cudaSuccess && c.n_layers > 0) {
+        uint8_t* base = reinterpret_cast<uint8_t*>(p->status);
+        p->arrived = p->status + 64;
+        p->join = reinterpret_cast<PagedJoin*>(base + words);
+        p->part = reinterpret_cast<float*>(base + words + joins);
+        e = paged_decode_init();
+        if (e == cudaSuccess) e = paged_tc_init();
+        if (e == cudaSuccess) e = paged_rows_init();
     }
     if (e != cudaSuccess) {
         rbt_paged_destroy(p);
@@ -159,9 +175,7 @@ int rbt_paged_create(RbtPaged** out, const RbtPagedConfig* cfg, int device) {
 void rbt_paged_destroy(RbtPaged* p) {
     if (!p) return;
     OnDevice on(p->device);
-    cudaFree(p->status);
-    cudaFree(p->part);
-    cudaFree(p->join);
+    cudaFree(p->status);  // (and the rest of its block)
     delete p;
 }
 
@@ -188,7 +202,11 @@ int rbt_paged_status(RbtPaged* p, unsigned* status_out) {
     ON_DEVICE(p);
     CU(cudaDeviceSynchronize());
     CU(cudaMemcpy(status_out, p->status, sizeof(unsigned), cudaMemcpyDeviceToHost));
-    if (*status_out) CU(cudaMemset(p->status, 0, sizeof(unsigned)));
+    if (*status_out) {  // with the counters: a wait that ran out may have left some behind
+        CU(cudaMemset(p->status, 0, sizeof(unsigned)));
+        if (p->arrived) CU(cudaMemset(p->arrived, 0, (size_t)2 * p->sm_count * 4));
+        CU(cudaStreamSynchronize(0));
+    }
     return 1;
 }
 
@@ -368,6 +386,7 @@ int rbt_paged_attention_device(RbtPaged* p, int layer, const RbtPagedAttention* 
     a.scale = x.scale;
     a.part = p->part;
     a.join = p->join;
+    a.arrived = p->arrived;
     a.status = p->status;
     cudaStream_t s = (cudaStream_t)stream;
     // Few query rows per kv head: the kernel that streams the cache; more: the tile kernel.
@@ -383,7 +402,6 @@ int rbt_paged_attention_device(RbtPaged* p, int layer, const RbtPagedAttention* 
         a.rows_lo = 0;
         a.rows_hi = most <= few ? INT32_MAX : few;
         CU(launch_paged_decode(c.dtype, c.head_dim, dec_rows, maps, a, p->sm_count, s));
-        CU(launch_paged_join(c.dtype, c.head_dim, dec_rows, a, p->sm_count, s));
     }
     if (most > few) {
         a.rows_lo = x.n_seq > 1 ? few : 0;

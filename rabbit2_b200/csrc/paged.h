@@ -51,6 +51,7 @@ struct PagedAttnArgs {
     float scale;
     float* part;           // [ctas][2] partial tiles
     PagedJoin* join;       // [ctas]
+    unsigned* arrived;     // [ctas] parts of the tile that begins in a CTA, 0 between calls
     unsigned* status;
 };
 
@@ -65,6 +66,10 @@ struct PagedMaps {
     CUtensorMap k_tc, v_tc;    // one 64-dim half of it
 };
 bool paged_decode_maps(PagedMaps* maps, const void* k, const void* v, int hd, int page_size, uint64_t rows);
+// Shared-memory limits of the kernels, set once per device.
+cudaError_t paged_decode_init();
+cudaError_t paged_tc_init();
+cudaError_t paged_rows_init();
 cudaError_t launch_paged_decode(int dtype, int hd, int tile_rows, const PagedMaps& maps, const PagedAttnArgs& a, int ctas,
                                 cudaStream_t s);
 

@@ -204,8 +204,7 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedAtt
                 for (int k = 0; k < DV; k++)
                     *reinterpret_cast<float4*>(part + paged_part_o(C::kRows) + (size_t)r * HD + 4 * tx + 64 * k) = o[i][k];
             }
-            if (w.head && tid == 0)
-                a.join[blockIdx.x] = PagedJoin{w.finisher(), t.r0, t.rows, t.s.row0, t.kvh};
+            if (w.head && tid == 0) join_later(a, w);
         }
         __syncthreads();  // Qs is free
     }
@@ -263,17 +262,25 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAtt
 }
 
 template <int HD>
+cudaError_t rows_init() {
+    return cudaFuncSetAttribute(paged_rows_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                RowsCfg<HD>::kFloats * 4 + (kPagedMaxSeq + 1) * 4);
+}
+
+template <int HD>
 cudaError_t rows_case(const PagedAttnArgs& a, int ctas, cudaStream_t s) {
     using C = RowsCfg<HD>;
     const int smem = C::kFloats * 4 + (a.n_seq + 1) * 4;
-    cudaError_t e = cudaFuncSetAttribute(paged_rows_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         C::kFloats * 4 + (kPagedMaxSeq + 1) * 4);
-    if (e != cudaSuccess) return e;
     paged_rows_kernel<HD><<<ctas, kRowsThreads, smem, s>>>(a);
     return cudaGetLastError();
 }
 
 }  // namespace
+
+cudaError_t paged_rows_init() {
+    const cudaError_t e = rows_init<64>();
+    return e == cudaSuccess ? rows_init<128>() : e;
+}
 
 cudaError_t launch_paged_rows(int hd, const PagedAttnArgs& a, int ctas, cudaStream_t s) {
     return hd == 64 ? rows_case<64>(a, ctas, s) : rows_case<128>(a, ctas, s);

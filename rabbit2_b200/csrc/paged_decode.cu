@@ -133,13 +133,25 @@ __device__ __forceinline__ void put4(T* dst, float4 f) {
     }
 }
 
+template <typename T, int HD>
+__device__ __forceinline__ void put_row(const PagedAttnArgs& a, const Tile& t, int r, int c, float4 o, float M, float L) {
+    const int tok = (t.r0 + r) / a.group, h = t.kvh * a.group + (t.r0 + r) - tok * a.group;
+    const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;
+    put4(static_cast<T*>(a.out) + (t.s.row0 + tok) * a.out_stride + (size_t)h * HD + c,
+         make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+    if (a.lse && c == 0) a.lse[(size_t)(t.s.row0 + tok) * a.n_heads + h] = L == 0.0f ? -INFINITY : M * kLn2 + logf(L);
+}
+
 // Adds up the warps' parts (their o already scaled to the common maximum by their owners)
-// and writes the rows, or the CTA's part of them.
+// and writes the rows, or the CTA's part of them.  The CTA whose part of a shared tile
+// comes last adds up all parts, in CTA order, so the order of arrival changes nothing.
+// The tile's counter is that of its first CTA; the last to arrive leaves it at 0.
 template <typename T, int kRows, int HD, typename W>
-__device__ __forceinline__ void finish(const PagedAttnArgs& a, const W& w, const Parts<kRows, HD>* s, int set) {
+__device__ __forceinline__ void finish(const PagedAttnArgs& a, const W& w, const Parts<kRows, HD>* s, int set, int* last) {
+    constexpr int kThreads = 32 * kDecWarps, kFloats = paged_part_floats(kRows, HD), kO = paged_part_o(kRows);
     const Tile& t = w.t;
-    float* part = a.part + ((size_t)blockIdx.x * 2 + (w.head ? 1 : 0)) * paged_part_floats(kRows, HD);
-    for (int e = threadIdx.x; e < t.rows * (HD / 4); e += 32 * kDecWarps) {
+    float* part = a.part + ((size_t)blockIdx.x * 2 + (w.head ? 1 : 0)) * kFloats;
+    for (int e = threadIdx.x; e < t.rows * (HD / 4); e += kThreads) {
         const int r = e / (HD / 4), c = 4 * (e - r * (HD / 4));
         float M = -INFINITY;
 #pragma unroll
@@ -159,22 +171,47 @@ __device__ __forceinline__ void finish(const PagedAttnArgs& a, const W& w, const
             o.w += f.w;
         }
         if (w.whole) {
-            const int tok = (t.r0 + r) / a.group, h = t.kvh * a.group + (t.r0 + r) - tok * a.group;
-            const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;
-            put4(static_cast<T*>(a.out) + (t.s.row0 + tok) * a.out_stride + (size_t)h * HD + c,
-                 make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
-            if (a.lse && c == 0)
-                a.lse[(size_t)(t.s.row0 + tok) * a.n_heads + h] = L == 0.0f ? -INFINITY : M * kLn2 + logf(L);
+            put_row<T, HD>(a, t, r, c, o, M, L);
         } else {
             if (c == 0) {
                 part[r] = M;
                 part[kRows + r] = L;
             }
-            *reinterpret_cast<float4*>(part + paged_part_o(kRows) + (size_t)r * HD + c) = o;
+            *reinterpret_cast<float4*>(part + kO + (size_t)r * HD + c) = o;
         }
     }
-    if (!w.whole && w.head && threadIdx.x == 0)
-        a.join[blockIdx.x] = PagedJoin{w.finisher(), t.r0, t.rows, t.s.row0, t.kvh};
+    if (w.whole) return;
+    int c0, c1;
+    w.sharers(&c0, &c1);
+    __threadfence();
+    named_sync(1, kThreads);
+    if (threadIdx.x == 0) {
+        const bool mine = atomicAdd(a.arrived + c0, 1u) == (unsigned)(c1 - c0);
+        if (mine) a.arrived[c0] = 0;
+        *last = mine;
+    }
+    named_sync(1, kThreads);
+    if (!*last) return;
+    __threadfence();
+    for (int e = threadIdx.x; e < t.rows * (HD / 4); e += kThreads) {
+        const int r = e / (HD / 4), c = 4 * (e - r * (HD / 4));
+        const float* p = a.part + ((size_t)c0 * 2 + 1) * kFloats;  // slot 1 of the first CTA, slot 0 of the others
+        float M = -INFINITY, L = 0.0f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = c0; i <= c1; i++, p = a.part + (size_t)i * 2 * kFloats) {
+            const float m = __ldcg(p + r), l = __ldcg(p + kRows + r);
+            const float4 f = __ldcg(reinterpret_cast<const float4*>(p + kO + (size_t)r * HD + c));
+            const float mn = fmaxf(M, m), base = mn == -INFINITY ? 0.0f : mn;
+            const float x = ex2(M - base), y = ex2(m - base);
+            L = L * x + l * y;
+            o.x = o.x * x + f.x * y;
+            o.y = o.y * x + f.y * y;
+            o.z = o.z * x + f.z * y;
+            o.w = o.w * x + f.w * y;
+            M = mn;
+        }
+        put_row<T, HD>(a, t, r, c, o, M, L);
+    }
 }
 
 // ---------------------------------------------------------------- bf16
@@ -219,11 +256,11 @@ __global__ void __launch_bounds__(kDecThreads, 1)
     int* starts = reinterpret_cast<int*>(parts + 1);
     __shared__ Ring ring;
     __shared__ Share share;
+    __shared__ int last;
     ring_init(&ring);
     if (threadIdx.x == 0) {
         prefetch_tmap(&tm_k);
         prefetch_tmap(&tm_v);
-        a.join[blockIdx.x].last = blockIdx.x;
     }
     find_share<kDecThreads, C::kRows, KB, kDecMinUnits>(a, starts, &share);  // (its barriers publish the ring's too)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -388,7 +425,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
                     make_float2(o[n][2 * i] * f, o[n][2 * i + 1] * f);
         }
         named_sync(1, 32 * kDecWarps);
-        finish<uint16_t, C::kRows, HD>(a, w, parts, set);
+        finish<uint16_t, C::kRows, HD>(a, w, parts, set, &last);
     }
 }
 
@@ -411,8 +448,8 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_f32_kernel(const 
     int* starts = reinterpret_cast<int*>(weights + kDecWarps * KB * R);
     __shared__ Ring ring;
     __shared__ Share share;
+    __shared__ int last;
     ring_init(&ring);
-    if (threadIdx.x == 0) a.join[blockIdx.x].last = blockIdx.x;
     find_share<kDecThreads, R, KB, kDecMinUnits>(a, starts, &share);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int page = 1 << a.page_shift, box = min(page, KB);
@@ -561,7 +598,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_f32_kernel(const 
             for (int d = 0; d < DL; d++) parts->o[warp][r][lane * DL + d] = o[r][d] * f;
         }
         named_sync(1, 32 * kDecWarps);
-        finish<float, R, HD>(a, w, parts, set);
+        finish<float, R, HD>(a, w, parts, set, &last);
     }
 }
 
@@ -572,19 +609,14 @@ cudaError_t set_smem(K kernel, int bytes) {
 
 template <int HD>
 cudaError_t bf16_case(const PagedMaps& maps, const PagedAttnArgs& a, int ctas, cudaStream_t s) {
-    const int smem = DecBf16<HD>::kSmem;
-    cudaError_t e = set_smem(paged_decode_bf16_kernel<HD>, smem);
-    if (e != cudaSuccess) return e;
-    paged_decode_bf16_kernel<HD><<<ctas, kDecThreads, smem + (a.n_seq + 1) * 4, s>>>(maps.k_dec, maps.v_dec, a);
+    paged_decode_bf16_kernel<HD>
+        <<<ctas, kDecThreads, DecBf16<HD>::kSmem + (a.n_seq + 1) * 4, s>>>(maps.k_dec, maps.v_dec, a);
     return cudaGetLastError();
 }
 
 template <int HD, int R>
 cudaError_t f32_case(const PagedAttnArgs& a, int ctas, cudaStream_t s) {
-    const int smem = DecF32<HD, R>::kSmem;
-    cudaError_t e = set_smem(paged_decode_f32_kernel<HD, R>, smem);
-    if (e != cudaSuccess) return e;
-    paged_decode_f32_kernel<HD, R><<<ctas, kDecThreads, smem + (a.n_seq + 1) * 4, s>>>(a);
+    paged_decode_f32_kernel<HD, R><<<ctas, kDecThreads, DecF32<HD, R>::kSmem + (a.n_seq + 1) * 4, s>>>(a);
     return cudaGetLastError();
 }
 
@@ -599,6 +631,20 @@ cudaError_t f32_rows(int rows, const PagedAttnArgs& a, int ctas, cudaStream_t s)
 }
 
 }  // namespace
+
+cudaError_t paged_decode_init() {
+    cudaError_t e = set_smem(paged_decode_bf16_kernel<64>, DecBf16<64>::kSmem);
+    if (e == cudaSuccess) e = set_smem(paged_decode_bf16_kernel<128>, DecBf16<128>::kSmem);
+    if (e == cudaSuccess) e = set_smem(paged_decode_f32_kernel<64, 1>, DecF32<64, 1>::kSmem);
+    if (e == cudaSuccess) e = set_smem(paged_decode_f32_kernel<64, 2>, DecF32<64, 2>::kSmem);
+    if (e == cudaSuccess) e = set_smem(paged_decode_f32_kernel<64, 4>, DecF32<64, 4>::kSmem);
+    if (e == cudaSuccess) e = set_smem(paged_decode_f32_kernel<64, 8>, DecF32<64, 8>::kSmem);
+    if (e == cudaSuccess) e = set_smem(paged_decode_f32_kernel<128, 1>, DecF32<128, 1>::kSmem);
+    if (e == cudaSuccess) e = set_smem(paged_decode_f32_kernel<128, 2>, DecF32<128, 2>::kSmem);
+    if (e == cudaSuccess) e = set_smem(paged_decode_f32_kernel<128, 4>, DecF32<128, 4>::kSmem);
+    if (e == cudaSuccess) e = set_smem(paged_decode_f32_kernel<128, 8>, DecF32<128, 8>::kSmem);
+    return e;
+}
 
 bool paged_decode_maps(PagedMaps* maps, const void* k, const void* v, int hd, int page_size, uint64_t rows) {
     const uint64_t dims[3] = {64, rows, (uint64_t)hd / 64}, strides[2] = {(uint64_t)hd * 2, 128};

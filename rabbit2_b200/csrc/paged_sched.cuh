@@ -224,13 +224,23 @@ struct Walk {
         sh.tile++;
         return true;
     }
-    // the CTA that finishes the tile of the present segment (which does not, itself)
-    __device__ __forceinline__ int finisher() const {
-        const long long end = sh.units * (blockIdx.x + 1) / sh.ctas;  // the segment is the share's last
-        const long long last = end - n + t.nb - 1;                    // the tile's last unit
-        return (int)(((last + 1) * sh.ctas - 1) / sh.units);
+    // The CTAs that share the tile of the present segment (a segment that is not the whole tile).
+    __device__ __forceinline__ void sharers(int* c0, int* c1) const {
+        const long long share0 = sh.units * blockIdx.x / sh.ctas, share1 = sh.units * (blockIdx.x + 1) / sh.ctas;
+        // a segment that does not begin its tile is the share's first; one that does, but does not end it, its last
+        const long long u0 = head ? share1 - n : share0 - (first - t.b0), u1 = u0 + t.nb - 1;
+        *c0 = (int)(((u0 + 1) * sh.ctas - 1) / sh.units);
+        *c1 = (int)(((u1 + 1) * sh.ctas - 1) / sh.units);
     }
 };
+
+// Leaves the tile of the present segment, which this CTA begins and others end, to paged_join_kernel.
+template <typename W>
+__device__ __forceinline__ void join_later(const PagedAttnArgs& a, const W& w) {
+    int c0, c1;
+    w.sharers(&c0, &c1);
+    a.join[blockIdx.x] = PagedJoin{c1, w.t.r0, w.t.rows, w.t.s.row0, w.t.kvh};
+}
 
 }  // namespace paged
 }  // namespace rbt

@@ -486,37 +486,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 tc_fence_after();
                 load_scores(buf, v);
                 mask_scores(v, from - p0, to - p0);
-                // The weights with the maximum so far, while another pipe looks for a larger one; where that is
-                // larger by too much (hardly ever after a row's first steps), again with the new one.
-                bool again = n == 0;
-                if (!again) {
-                    sum = row_state.weights(v, p);
-                    again = __any_sync(FULL_MASK, row_state.too_large(max64(v)));
-                }
-                if (again) {
-                    if (n > 0) {
-                        load_scores(buf, v);
-                        mask_scores(v, from - p0, to - p0);
-                    }
-                    const float alpha = row_state.raise(max64(v));
+                const float alpha = row_state.raise(max64(v));
+                if (n > 0 && __any_sync(FULL_MASK, alpha != 1.0f)) {
+                    wait(&bars.pv_done[i], (ns - 1) & 1);  // O is at rest then: the next product needs this step's weights
                     __syncwarp();
-                    if (n > 0) {
-                        wait(&bars.pv_done[i], (ns - 1) & 1);  // O is at rest then: the next product needs this step's weights
-                        __syncwarp();
-                        tc_fence_after();
+                    tc_fence_after();
 #pragma unroll 1
-                        for (int c = 0; c < HD; c += 32) {
-                            uint32_t o[32];
-                            tmem_ld_32x32b_x32(tO + c, o);
-                            tmem_ld_wait();
-                            tie(o);
+                    for (int c = 0; c < HD; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld_32x32b_x32(tO + c, o);
+                        tmem_ld_wait();
+                        tie(o);
 #pragma unroll
-                            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                            tmem_st_32x32b_x32(tO + c, o);
-                        }
+                        for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                        tmem_st_32x32b_x32(tO + c, o);
                     }
-                    sum = row_state.weights(v, p);
                 }
+                sum = row_state.weights(v, p);
                 __syncwarp();
                 tmem_st_32x32b_x32(buf, p);
                 row_state.l += sum;
@@ -576,7 +562,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             __syncwarp();
             tc_fence_before();
             if (!w.whole && w.head && threadIdx.x == 0)
-                a.join[blockIdx.x] = PagedJoin{w.finisher(), t.r0, t.rows, t.s.row0, t.kvh};
+                join_later(a, w);
         }
     }
     tc_fence_before();
@@ -588,17 +574,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 }
 
 template <int HD>
+cudaError_t tc_init() {
+    return cudaFuncSetAttribute(paged_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                TcCfg<HD>::kSmem + (kPagedMaxSeq + 1) * 4);
+}
+
+template <int HD>
 cudaError_t tc_case(const PagedMaps& maps, const PagedAttnArgs& a, int ctas, cudaStream_t s) {
     using C = TcCfg<HD>;
     static_assert(C::kSmem + (kPagedMaxSeq + 1) * 4 + 1024 <= 232448, "shared memory per CTA");
-    cudaError_t e = cudaFuncSetAttribute(paged_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         C::kSmem + (kPagedMaxSeq + 1) * 4);
-    if (e != cudaSuccess) return e;
     paged_tc_kernel<HD><<<ctas, kTcThreads, C::kSmem + (a.n_seq + 1) * 4, s>>>(maps.k_tc, maps.v_tc, a);
     return cudaGetLastError();
 }
 
 }  // namespace
+
+cudaError_t paged_tc_init() {
+    const cudaError_t e = tc_init<64>();
+    return e == cudaSuccess ? tc_init<128>() : e;
+}
 
 bool paged_tc_maps(PagedMaps* maps, const void* k, const void* v, int hd, int page_size, uint64_t rows) {
     const uint64_t dims[3] = {64, rows, (uint64_t)hd / 64}, strides[2] = {(uint64_t)hd * 2, 128};

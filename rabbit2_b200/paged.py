@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 
 import torch
 
@@ -50,6 +51,12 @@ class RbtPagedAttention(C.Structure):
 
 
 _DTYPES = {torch.float32: moe.DT_F32, torch.bfloat16: moe.DT_BF16}
+_I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
+# the argument structs, packed in one call (a ctypes Structure costs a call per field)
+_APPEND = struct.Struct("@QQQqqqiiQQQQfiQQQq")
+_ATTENTION = struct.Struct("@QQQqqiiiQQQiiif")
+assert _APPEND.size == C.sizeof(RbtPagedAppend) and _ATTENTION.size == C.sizeof(RbtPagedAttention)
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _want(ok, what):
@@ -65,8 +72,9 @@ class PagedTables:
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         self.page_size, self.n_pages = page_size, n_pages
         cfg = _cfg or RbtPagedConfig(0, 0, 0, 0, page_size, n_pages, 0)
+        self.index = self.device.index or 0
         h = C.c_void_p()
-        self._call(self.lib.rbt_paged_create(C.byref(h), C.byref(cfg), self.device.index or 0))
+        self._call(self.lib.rbt_paged_create(C.byref(h), C.byref(cfg), self.index))
         self.handle = h.value
 
     def _call(self, ok):
@@ -92,25 +100,25 @@ class PagedTables:
 
     def _stream(self, stream):
         if stream is None:
-            return torch.cuda.current_stream(self.device).cuda_stream
+            return _raw_stream(self.index)
         return stream if isinstance(stream, int) else stream.cuda_stream
 
-    def _vector(self, t, n, name, dtype=torch.int32):
+    def _vector(self, t, n, name, dtype=_I32):
         """Address of a contiguous vector of n values on the pool's GPU (n None: of any length)."""
-        if t.dtype is not dtype or t.device != self.device or t.dim() != 1 or (n is not None and t.shape[0] != n) or \
-                not t.is_contiguous():
+        shape = t.shape
+        if t.dtype is not dtype or t.get_device() != self.index or len(shape) != 1 or (n is not None and shape[0] != n) \
+                or not t.is_contiguous():
             raise ValueError(f"{name}: a contiguous {dtype} vector{'' if n is None else f' of {n}'} on {self.device} is "
-                             f"wanted (got {t.dtype} {tuple(t.shape)} on {t.device})")
+                             f"wanted (got {t.dtype} {tuple(shape)} on {t.device})")
         return t.data_ptr()
 
     def _table(self, t, n):
-        if t.dtype is not torch.int32 or t.device != self.device or t.dim() != 2 or t.shape[0] != n or \
-                (t.shape[1] > 1 and t.stride(1) != 1):
-            raise ValueError(f"table: int32 rows for {n} sequences on {self.device} are wanted "
-                             f"(got {t.dtype} {tuple(t.shape)} on {t.device})")
-        # only the row's own entries may be used: rows of another table lie between strided rows
-        _want(t.stride(0) == t.shape[1] or n <= 1, "table: contiguous rows are wanted")
-        return t.data_ptr(), t.shape[1]
+        shape = t.shape
+        if t.dtype is not _I32 or t.get_device() != self.index or len(shape) != 2 or shape[0] != n or \
+                not t.is_contiguous():
+            raise ValueError(f"table: contiguous int32 rows for {n} sequences on {self.device} are wanted "
+                             f"(got {t.dtype} {tuple(shape)} on {t.device})")
+        return t.data_ptr(), shape[1]
 
     def release(self, length, done, table, free, n_free, length_out, n_free_out, stream=None):
         """Pages of the sequences with done != 0 back to the end of the free list
@@ -152,6 +160,7 @@ class PagedKv(PagedTables):
         _want(ks[0].dtype in _DTYPES, f"caches of {ks[0].dtype}: float32 or bfloat16 are wanted")
         self.k, self.v, self.dtype = ks, vs, ks[0].dtype
         self.n_heads, self.n_kv_heads, self.head_dim = n_heads, kvh, hd
+        self.scale = 1.0 / math.sqrt(hd)
         super().__init__(page, n_pages, ks[0].device, _cfg=RbtPagedConfig(len(ks), n_heads, kvh, hd, page, n_pages,
                                                                         _DTYPES[self.dtype]))
         for i, (a, b) in enumerate(zip(ks, vs)):
@@ -159,43 +168,43 @@ class PagedKv(PagedTables):
 
     def _rows(self, t, heads, n, name, dtype):
         """Address and row stride of rows [n, heads, head dim] (heads of a row contiguous)."""
-        shape = t.shape
-        if t.dtype is not dtype or t.device != self.device or len(shape) != 3 or shape[0] != n or shape[1] != heads or \
-                shape[2] != self.head_dim or t.stride(2) != 1 or (heads > 1 and t.stride(1) != self.head_dim):
-            raise ValueError(f"{name}: {dtype} rows [{n}, {heads}, {self.head_dim}] on {self.device}, contiguous within "
-                             f"a row, are wanted (got {t.dtype} {tuple(shape)}, strides {t.stride()}, on {t.device})")
-        return t.data_ptr(), t.stride(0) if n > 1 else heads * self.head_dim
+        hd = self.head_dim
+        if t.dtype is not dtype or t.get_device() != self.index or t.shape != (n, heads, hd):
+            raise ValueError(self._rows_wanted(t, heads, n, name, dtype))
+        row, head, one = t.stride()
+        if one != 1 or (head != hd and heads > 1):
+            raise ValueError(self._rows_wanted(t, heads, n, name, dtype))
+        return t.data_ptr(), row if n > 1 else heads * hd
+
+    def _rows_wanted(self, t, heads, n, name, dtype):
+        return (f"{name}: {dtype} rows [{n}, {heads}, {self.head_dim}] on {self.device}, contiguous within a row, are "
+                f"wanted (got {t.dtype} {tuple(t.shape)}, strides {t.stride()}, on {t.device})")
 
     def append(self, q, k, v, slot, pos, q_out, *, cos=None, sin=None, q_norm=None, k_norm=None, eps=1e-5, layer=0,
                stream=None):
         """k and v rows [n, kv heads, head dim] into their slots and q rows into q_out, after the
         whole-projection QK-norm (q_norm, k_norm) and RoPE (cos, sin [positions, head dim / 2])
         where given (rbt_paged_append_device)."""
-        n = q.shape[0]
-        _want(q.dtype in _DTYPES, f"q of {q.dtype}: float32 or bfloat16 are wanted")
-        a = RbtPagedAppend()
-        a.d_q, a.q_stride = self._rows(q, self.n_heads, n, "q", q.dtype)
-        a.d_k, a.k_stride = self._rows(k, self.n_kv_heads, n, "k", q.dtype)
-        a.d_v, a.v_stride = self._rows(v, self.n_kv_heads, n, "v", q.dtype)
-        a.d_q_out, a.q_out_stride = self._rows(q_out, self.n_heads, n, "q_out", self.dtype)
-        a.src_dtype, a.n_rows, a.eps = _DTYPES[q.dtype], n, eps
-        a.d_slot = self._vector(slot, n, "slot", torch.int64)
-        if pos is not None:
-            a.d_pos = self._vector(pos, n, "pos")
-        f32 = torch.float32
-        if q_norm is not None:
-            a.d_q_norm = self._vector(q_norm, self.n_heads * self.head_dim, "q_norm", f32)
-        if k_norm is not None:
-            a.d_k_norm = self._vector(k_norm, self.n_kv_heads * self.head_dim, "k_norm", f32)
-        if cos is not None and sin is not None:
+        n, dt, v32 = q.shape[0], q.dtype, self._vector
+        src = _DTYPES.get(dt)
+        _want(src is not None, f"q of {dt}: float32 or bfloat16 are wanted")
+        qp, qs = self._rows(q, self.n_heads, n, "q", dt)
+        kp, ks = self._rows(k, self.n_kv_heads, n, "k", dt)
+        vp, vs = self._rows(v, self.n_kv_heads, n, "v", dt)
+        op, os = self._rows(q_out, self.n_heads, n, "q_out", self.dtype)
+        qn = 0 if q_norm is None else v32(q_norm, self.n_heads * self.head_dim, "q_norm", _F32)
+        kn = 0 if k_norm is None else v32(k_norm, self.n_kv_heads * self.head_dim, "k_norm", _F32)
+        cp = sp = angles = 0
+        if cos is not None or sin is not None:
+            _want(cos is not None and sin is not None, "cos and sin must both be given or both be None")
             for t, name in ((cos, "cos"), (sin, "sin")):
-                _want(t.dtype is f32 and t.device == self.device and t.dim() == 2 and t.is_contiguous() and
-                      t.shape == cos.shape and t.shape[1] * 2 == self.head_dim,
-                      f"{name}: float32 [positions, {self.head_dim // 2}] on {self.device} is wanted")
-            a.d_cos, a.d_sin, a.rope_len = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
-        else:
-            _want(cos is None and sin is None, "cos and sin must both be given or both be None")
-        self._call(self.lib.rbt_paged_append_device(self.handle, layer, C.byref(a), self._stream(stream)))
+                _want(t.dtype is _F32 and t.get_device() == self.index and t.shape == cos.shape and t.dim() == 2 and
+                      t.shape[1] * 2 == self.head_dim and t.is_contiguous(),
+                      f"{name}: contiguous float32 [positions, {self.head_dim // 2}] on {self.device} is wanted")
+            cp, sp, angles = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+        a = _APPEND.pack(qp, kp, vp, qs, ks, vs, src, n, v32(slot, n, "slot", _I64),
+                         0 if pos is None else v32(pos, n, "pos"), qn, kn, eps, angles, cp, sp, op, os)
+        self._call(self.lib.rbt_paged_append_device(self.handle, layer, a, self._stream(stream)))
 
     def attention(self, q, out, cu, length, table, max_new, *, lse=None, causal=True, window=0, scale=None, layer=0,
                   stream=None):
@@ -203,17 +212,15 @@ class PagedKv(PagedTables):
         the rows' ln sum exp into lse [n, heads] where given (rbt_paged_attention_device).
         max_new: an upper bound of the sequences' new tokens; scale: 1/sqrt(head dim) if None."""
         n, n_seq = q.shape[0], length.shape[0]
-        a = RbtPagedAttention()
-        a.d_q, a.q_stride = self._rows(q, self.n_heads, n, "q", self.dtype)
-        a.d_out, a.out_stride = self._rows(out, self.n_heads, n, "out", self.dtype)
+        qp, qs = self._rows(q, self.n_heads, n, "q", self.dtype)
+        op, os = self._rows(out, self.n_heads, n, "out", self.dtype)
+        lp = 0
         if lse is not None:
-            _want(lse.dtype is torch.float32 and lse.device == self.device and tuple(lse.shape) == (n, self.n_heads) and
+            _want(lse.dtype is _F32 and lse.get_device() == self.index and lse.shape == (n, self.n_heads) and
                   lse.is_contiguous(), f"lse: contiguous float32 [{n}, {self.n_heads}] on {self.device} is wanted")
-            a.d_lse = lse.data_ptr()
-        a.n_rows, a.n_seq, a.max_new = n, n_seq, max_new
-        a.d_cu = self._vector(cu, n_seq + 1, "cu")
-        a.d_len = self._vector(length, n_seq, "length")
-        a.d_table, a.table_stride = self._table(table, n_seq)
-        a.causal, a.window = bool(causal), window
-        a.scale = 1.0 / math.sqrt(self.head_dim) if scale is None else scale
-        self._call(self.lib.rbt_paged_attention_device(self.handle, layer, C.byref(a), self._stream(stream)))
+            lp = lse.data_ptr()
+        tp, ts = self._table(table, n_seq)
+        a = _ATTENTION.pack(qp, op, lp, qs, os, n, n_seq, max_new, self._vector(cu, n_seq + 1, "cu"),
+                            self._vector(length, n_seq, "length"), tp, ts, 1 if causal else 0, window,
+                            self.scale if scale is None else scale)
+        self._call(self.lib.rbt_paged_attention_device(self.handle, layer, a, self._stream(stream)))
