@@ -70,7 +70,7 @@ bool paged_decode_maps(PagedMaps* maps, const void* k, const void* v, int hd, in
 cudaError_t paged_decode_init();
 cudaError_t paged_tc_init();
 cudaError_t paged_rows_init();
-cudaError_t launch_paged_decode(int dtype, int hd, int tile_rows, const PagedMaps& maps, const PagedAttnArgs& a, int ctas,
+cudaError_t launch_paged_decode(int dtype, int hd, int tile_rows, const PagedMaps& maps, const PagedAttnArgs& a, int sms,
                                 cudaStream_t s);
 
 bool paged_tc_maps(PagedMaps* maps, const void* k, const void* v, int hd, int page_size, uint64_t rows);

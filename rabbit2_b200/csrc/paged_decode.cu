@@ -2,10 +2,11 @@
 // one new token, or a few, times the heads that share a kv head (at most 16 rows in
 // bf16, 8 in f32).  Bound by the bytes of k and v, which are read once each.
 //
-// Both kernels have the same shape.  One CTA per SM takes an equal share of all units
-// (paged_sched.cuh).  Warp 4 is the producer: it walks the share ahead of the others and
-// fills a ring of 16 KB stages (k and v of one block of positions) by bulk copies, across
-// the borders of tiles, so that up to 128 KB per SM are in flight.  Warps 0-3 take the
+// Both kernels have the same shape.  One or two CTAs per SM each take an equal share of all units
+// (paged_sched.cuh).  Warps 4 and 5 are the producers, of k and of v (one warp alone could
+// not start copies fast enough): they walk the share ahead of the others and fill a ring of
+// 16 KB stages (k and v of one block of positions) by bulk copies, across the borders of
+// tiles, so that up to 128 KB per SM are in flight.  Warps 0-3 take the
 // blocks in turn, each with a running maximum, sum and output of its own, and add the four
 // up at the end of a tile through shared memory; nothing inside a tile waits for another
 // warp.
@@ -36,38 +37,47 @@ namespace {
 using namespace paged;
 using namespace tc;
 
-constexpr int kDecWarps = 4, kDecThreads = 32 * (kDecWarps + 1);
-constexpr int kDecStages = 8;           // a multiple of kDecWarps: a stage always belongs to one warp
+constexpr int kDecWarps = 4, kDecThreads = 32 * (kDecWarps + 2);
+// Stages of the ring and CTAs per SM.  Two CTAs of four stages overlap one's turn from a tile to
+// the next (its q, its sums) with the other's copies; against one CTA of eight stages: 96
+// sequences to 16384 positions in pages of 16 682 -> 545 us, 64 at 2048 in f32 360 -> 310 us.
+// The f32 kernel of 8 rows needs the registers of one CTA (with two it spills: 164 -> 246 us).
+template <bool kOne>
+struct DecShape {
+    static constexpr int kStages = kOne ? 8 : 4, kCtas = kOne ? 1 : 2;
+};
 constexpr int kDecStage = 16384;        // bytes: k | v
 constexpr int kDecMinUnits = kDecWarps; // a CTA with less would leave warps idle
-constexpr uint64_t kDecWaitNs = 2000000000ull;
-static_assert(kDecStages % kDecWarps == 0, "stages are dealt to warps");
 
 // ---------------------------------------------------------------- both kernels
+template <int kStages>
 struct Ring {
-    uint64_t full[kDecStages], empty[kDecStages];
+    uint64_t full[kStages], empty[kStages];
 };
 
-__device__ __forceinline__ void ring_init(Ring* r) {
+template <int kStages>
+__device__ __forceinline__ void ring_init(Ring<kStages>* r) {
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kDecStages; i++) {
-            mbar_init(&r->full[i], 1);
+        for (int i = 0; i < kStages; i++) {
+            mbar_init(&r->full[i], 2);
             mbar_init(&r->empty[i], 1);
         }
         fence_mbar_init();
     }
 }
 
-// The producer warp.  copy(id, off, box, stage, bar) starts the copies of positions
-// [off, off + box rows) of page id into box `box` of the stage (one lane per box).
-template <int kRows, int kBlock, typename Copy>
-__device__ __forceinline__ void produce(const PagedAttnArgs& a, const Share& share, const int* starts, Ring* ring,
+// A producer warp, of k or of v.  copy(id, kvh, off, box, stage, bar) starts the copy of
+// positions [off, off + box rows) of page id into box `box` of its half of the stage (one
+// lane per box).
+template <int kRows, int kBlock, int kStages, typename Copy>
+__device__ __forceinline__ void produce(const PagedAttnArgs& a, const Share& share, const int* starts, Ring<kStages>* ring,
                                         uint8_t* stages, int box_rows, uint32_t row_bytes, Copy copy) {
     const int lane = threadIdx.x & 31;
     Walk<kRows, kBlock> w(share, starts);
     uint32_t j = 0;
-    bool ok = true;
-    while (ok && w.next(a)) {
+    Waiter wait;
+    wait.status = a.status;
+    while (wait.ok && w.next(a)) {
         const int32_t* table = a.table + (size_t)w.t.seq * a.table_stride;
         int chunk = -1, ids = 0;  // 32 entries of the table row, one per lane
         for (int b = w.first; b < w.first + w.n; b++, j++) {
@@ -79,14 +89,9 @@ __device__ __forceinline__ void produce(const PagedAttnArgs& a, const Share& sha
                 const int at = chunk * 32 + lane;
                 ids = at < a.table_stride ? table[at] : 0;
             }
-            const uint32_t st = j % kDecStages;
-            if (j >= kDecStages && !mbar_wait_bounded(&ring->empty[st], (j / kDecStages - 1) & 1, kDecWaitNs)) ok = false;
-            ok = __all_sync(FULL_MASK, ok);
-            if (!ok) {
-                if (lane == 0) atomicCAS(a.status, 0u, (unsigned)kPagedWait);
-                break;
-            }
-            if (lane == 0) mbar_arrive_expect_tx(&ring->full[st], boxes * box_rows * row_bytes * 2);
+            const uint32_t st = j % kStages;
+            if (j >= kStages && !wait.warp(&ring->empty[st], (j / kStages - 1) & 1)) break;
+            if (lane == 0) mbar_arrive_expect_tx(&ring->full[st], boxes * box_rows * row_bytes);
             __syncwarp();
             const int p = p0 + lane * box_rows;  // this lane's box
             int id = __shfl_sync(FULL_MASK, ids, (p >> a.page_shift) & 31);
@@ -100,17 +105,9 @@ __device__ __forceinline__ void produce(const PagedAttnArgs& a, const Share& sha
         }
     }
     // every copy has landed before the CTA may exit
-    for (uint32_t i = j > kDecStages ? j - kDecStages : 0; i < j; i++)
-        if (!mbar_wait_bounded(&ring->full[i % kDecStages], (i / kDecStages) & 1, kDecWaitNs) && lane == 0)
-            atomicCAS(a.status, 0u, (unsigned)kPagedWait);
-}
-
-// A consumer's wait for block j; after one that ran out it waits no more (the results are
-// void, the barriers are still met).
-__device__ __forceinline__ void await(const PagedAttnArgs& a, Ring* ring, uint32_t j, bool& ok) {
-    if (ok) ok = __all_sync(FULL_MASK, mbar_wait_bounded(&ring->full[j % kDecStages], (j / kDecStages) & 1, kDecWaitNs));
-    if (!ok && (threadIdx.x & 31) == 0) atomicCAS(a.status, 0u, (unsigned)kPagedWait);
-    __syncwarp();
+    wait.ok = true;
+    for (uint32_t i = j > kStages ? j - kStages : 0; i < j; i++)
+        wait(&ring->full[i % kStages], (i / kStages) & 1);
 }
 
 // The four warps' parts of a segment, in shared memory: two sets of maxima and sums (the
@@ -241,20 +238,21 @@ struct DecBf16 {
     static constexpr int kRows = kPagedDecRowsBf16;
     static constexpr int kBlock = kDecStage / (4 * HD);  // positions of a stage: 32 (head_dim 128) or 64
     static constexpr int kHalf = kDecStage / 2;          // bytes of k
-    static constexpr int kSmem = kDecStages * kDecStage + (int)sizeof(Parts<kRows, HD>) + 1024;
+    static constexpr int kStages = DecShape<false>::kStages, kCtas = DecShape<false>::kCtas;
+    static constexpr int kSmem = kStages * kDecStage + (int)sizeof(Parts<kRows, HD>) + 1024;
 };
 
 template <int HD>
-__global__ void __launch_bounds__(kDecThreads, 1)
+__global__ void __launch_bounds__(kDecThreads, DecBf16<HD>::kCtas)
     paged_decode_bf16_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                              const PagedAttnArgs a) {
     using C = DecBf16<HD>;
     constexpr int KB = C::kBlock, NT = KB / 8, KS = HD / 16;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    Parts<C::kRows, HD>* parts = reinterpret_cast<Parts<C::kRows, HD>*>(smem + kDecStages * kDecStage);
+    Parts<C::kRows, HD>* parts = reinterpret_cast<Parts<C::kRows, HD>*>(smem + C::kStages * kDecStage);
     int* starts = reinterpret_cast<int*>(parts + 1);
-    __shared__ Ring ring;
+    __shared__ Ring<C::kStages> ring;
     __shared__ Share share;
     __shared__ int last;
     ring_init(&ring);
@@ -265,27 +263,33 @@ __global__ void __launch_bounds__(kDecThreads, 1)
     find_share<kDecThreads, C::kRows, KB, kDecMinUnits>(a, starts, &share);  // (its barriers publish the ring's too)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int page = 1 << a.page_shift, box = min(page, KB);
-    if (warp == kDecWarps) {
-        produce<C::kRows, KB>(a, share, starts, &ring, smem, box, HD * 2,
+    if (warp >= kDecWarps) {
+        const bool is_v = warp > kDecWarps;
+        produce<C::kRows, KB>(a, share, starts, &ring, smem + (is_v ? C::kHalf : 0), box, HD * 2,
                               [&](int id, int kvh, int off, int i, uint8_t* stage, uint64_t* bar) {
                                   const int y = ((id * a.n_kv + kvh) << a.page_shift) + off;
-                                  tma_load_3d(stage + i * box * HD * 2, &tm_k, bar, 0, y, 0);
-                                  tma_load_3d(stage + C::kHalf + i * box * HD * 2, &tm_v, bar, 0, y, 0);
+                                  tma_load_3d(stage + i * box * HD * 2, is_v ? &tm_v : &tm_k, bar, 0, y, 0);
                               });
         return;
     }
     const int g = lane >> 2, tq = lane & 3;
     const float k2 = a.scale * kLog2e;
     const int box_shift = min(a.page_shift, HD == 128 ? 5 : 6);
-    // byte offset of 16-byte chunk `c` (of HD / 8) of position r of a block: boxes of [half][box
-    // rows][64 dims] in the 128-byte swizzle
-    const auto at = [&](int r, int c) -> uint32_t {
-        const uint32_t b = r >> box_shift, rr = r & (box - 1);
-        return b * (box * HD * 2) + (c >> 3) * (box * 128) + rr * 128 + ((uint32_t)((c & 7) ^ (rr & 7)) << 4);
-    };
+    // A block lies in boxes of [64-dim half][box rows][64 dims] in the 128-byte swizzle: 16-byte chunk c of
+    // a half of row r is at row_at(r) + ((c ^ (r & 7)) << 4).  For ldmatrix lane i points to row (i & 7) of
+    // its 8 x 8 matrix, so the swizzle is one exclusive-or with a constant of the lane.
+    const uint32_t half_bytes = box * 128;
+    const auto row_at = [&](int r) -> uint32_t { return (r >> box_shift) * (box * HD * 2) + (r & (box - 1)) * 128; };
+    uint32_t k_row[NT], v_row[NT / 2];
+#pragma unroll
+    for (int n = 0; n < NT; n++) k_row[n] = row_at(8 * n + (lane & 7));
+#pragma unroll
+    for (int k = 0; k < NT / 2; k++) v_row[k] = C::kHalf + row_at(16 * k + (lane & 15));
+    const uint32_t k_swz = ((lane >> 3) ^ (lane & 7)) << 4, v_swz = ((lane >> 4) ^ (lane & 7)) << 4;
     Walk<C::kRows, KB> w(share, starts);
     uint32_t j = 0;
-    bool ok = true;
+    Waiter wait;  // (after one that ran out it waits no more: the results are void, the barriers are still met)
+    wait.status = a.status;
     for (int set = 0; w.next(a); set ^= 1) {
         const Tile& t = w.t;
         uint32_t q[KS][4];  // rows g and g + 8 as A fragments
@@ -317,10 +321,10 @@ __global__ void __launch_bounds__(kDecThreads, 1)
             for (int i = 0; i < 4; i++) o[n][i] = 0.0f;
         const uint32_t skip = (warp - j) & (kDecWarps - 1);
         for (int i = skip; i < w.n; i += kDecWarps) {
-            const uint32_t jj = j + i, st = jj % kDecStages;
+            const uint32_t jj = j + i, st = jj % C::kStages;
             const int p0 = (w.first + i) * KB;
-            await(a, &ring, jj, ok);
-            const uint32_t ks = smem_u32(smem + st * kDecStage), vs = ks + C::kHalf;
+            wait.warp(&ring.full[st], (jj / C::kStages) & 1);
+            const uint32_t stage = smem_u32(smem + st * kDecStage);
             float s[NT][4];
 #pragma unroll
             for (int n = 0; n < NT; n++) {
@@ -329,7 +333,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
 #pragma unroll
                 for (int k = 0; k < KS; k += 2) {  // positions 8 n .., dims 16 k .. + 32
                     uint32_t b[4];
-                    ldsm4(ks + at(8 * n + (lane & 7), 2 * k + (lane >> 3)), b);
+                    ldsm4(stage + k_row[n] + (k >> 2) * half_bytes + (k_swz ^ ((2 * k & 7) << 4)), b);
                     mma16816(s[n], q[k], b[0], b[1]);
                     mma16816(s[n], q[k + 1], b[2], b[3]);
                 }
@@ -383,7 +387,8 @@ __global__ void __launch_bounds__(kDecThreads, 1)
                 for (int e = lane; e < KB * (HD / 8); e += 32) {
                     const int r = e / (HD / 8), c = e - r * (HD / 8);
                     if (p0 + r >= t.hi)
-                        *reinterpret_cast<uint4*>(smem + st * kDecStage + C::kHalf + at(r, c)) = make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4*>(smem + st * kDecStage + C::kHalf + row_at(r) + (c >> 3) * half_bytes +
+                                                  (((c ^ r) & 7) << 4)) = make_uint4(0, 0, 0, 0);
                 }
                 __syncwarp();
             }
@@ -392,7 +397,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
 #pragma unroll
                 for (int n = 0; n < HD / 8; n += 2) {  // positions 16 k .., dims 8 n .. + 16
                     uint32_t b[4];
-                    ldsm4_t(vs + at(16 * k + (lane & 15), n + (lane >> 4)), b);
+                    ldsm4_t(stage + v_row[k] + (n >> 3) * half_bytes + (v_swz ^ ((n & 7) << 4)), b);
                     mma16816(o[n], pa[k], b[0], b[1]);
                     mma16816(o[n + 1], pa[k], b[2], b[3]);
                 }
@@ -434,32 +439,34 @@ template <int HD, int R>
 struct DecF32 {
     static constexpr int kBlock = kDecStage / (8 * HD);  // 16 (head_dim 128) or 32
     static constexpr int kHalf = kDecStage / 2;
-    static constexpr int kSmem = kDecStages * kDecStage + (int)sizeof(Parts<R, HD>) + kDecWarps * kBlock * R * 4 + 128;
+    static constexpr int kStages = DecShape<R == 8>::kStages, kCtas = DecShape<R == 8>::kCtas;
+    static constexpr int kSmem = kStages * kDecStage + (int)sizeof(Parts<R, HD>) + kDecWarps * kBlock * R * 4 + 128;
 };
 
 template <int HD, int R>
-__global__ void __launch_bounds__(kDecThreads, 1) paged_decode_f32_kernel(const PagedAttnArgs a) {
+__global__ void __launch_bounds__(kDecThreads, DecF32<HD, R>::kCtas) paged_decode_f32_kernel(const PagedAttnArgs a) {
     using C = DecF32<HD, R>;
     constexpr int KB = C::kBlock, NI = KB / 4, NC = HD / 32, DL = HD / 32;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
-    Parts<R, HD>* parts = reinterpret_cast<Parts<R, HD>*>(smem + kDecStages * kDecStage);
+    Parts<R, HD>* parts = reinterpret_cast<Parts<R, HD>*>(smem + C::kStages * kDecStage);
     float* weights = reinterpret_cast<float*>(parts + 1);  // [warp][KB][R]
     int* starts = reinterpret_cast<int*>(weights + kDecWarps * KB * R);
-    __shared__ Ring ring;
+    __shared__ Ring<C::kStages> ring;
     __shared__ Share share;
     __shared__ int last;
     ring_init(&ring);
     find_share<kDecThreads, R, KB, kDecMinUnits>(a, starts, &share);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int page = 1 << a.page_shift, box = min(page, KB);
-    if (warp == kDecWarps) {
-        produce<R, KB>(a, share, starts, &ring, smem, box, HD * 4,
+    if (warp >= kDecWarps) {
+        const bool is_v = warp > kDecWarps;
+        const float* src = static_cast<const float*>(is_v ? a.v : a.k);
+        produce<R, KB>(a, share, starts, &ring, smem + (is_v ? C::kHalf : 0), box, HD * 4,
                        [&](int id, int kvh, int off, int i, uint8_t* stage, uint64_t* bar) {
                            const size_t row = (((size_t)id * a.n_kv + kvh) << a.page_shift) + off;
                            const uint32_t bytes = box * HD * 4;
-                           bulk_load(stage + i * bytes, static_cast<const float*>(a.k) + row * HD, bytes, bar);
-                           bulk_load(stage + C::kHalf + i * bytes, static_cast<const float*>(a.v) + row * HD, bytes, bar);
+                           bulk_load(stage + i * bytes, src + row * HD, bytes, bar);
                        });
         return;
     }
@@ -468,7 +475,8 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_f32_kernel(const 
     float* wp = weights + warp * KB * R;
     Walk<R, KB> w(share, starts);
     uint32_t j = 0;
-    bool ok = true;
+    Waiter wait;  // (after one that ran out it waits no more: the results are void, the barriers are still met)
+    wait.status = a.status;
     for (int set = 0; w.next(a); set ^= 1) {
         const Tile& t = w.t;
         float4 q[R][NC];
@@ -495,9 +503,9 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_f32_kernel(const 
         }
         const uint32_t skip = (warp - j) & (kDecWarps - 1);
         for (int b = skip; b < w.n; b += kDecWarps) {
-            const uint32_t jb = j + b, st = jb % kDecStages;
+            const uint32_t jb = j + b, st = jb % C::kStages;
             const int p0 = (w.first + b) * KB, nv = min(KB, t.hi - p0);
-            await(a, &ring, jb, ok);
+            wait.warp(&ring.full[st], (jb / C::kStages) & 1);
             const float* Ks = reinterpret_cast<const float*>(smem + st * kDecStage);
             const float* Vs = reinterpret_cast<const float*>(smem + st * kDecStage + C::kHalf);
             float s[NI][R];
@@ -608,25 +616,25 @@ cudaError_t set_smem(K kernel, int bytes) {
 }
 
 template <int HD>
-cudaError_t bf16_case(const PagedMaps& maps, const PagedAttnArgs& a, int ctas, cudaStream_t s) {
+cudaError_t bf16_case(const PagedMaps& maps, const PagedAttnArgs& a, int sms, cudaStream_t s) {
     paged_decode_bf16_kernel<HD>
-        <<<ctas, kDecThreads, DecBf16<HD>::kSmem + (a.n_seq + 1) * 4, s>>>(maps.k_dec, maps.v_dec, a);
+        <<<sms * DecBf16<HD>::kCtas, kDecThreads, DecBf16<HD>::kSmem + (a.n_seq + 1) * 4, s>>>(maps.k_dec, maps.v_dec, a);
     return cudaGetLastError();
 }
 
 template <int HD, int R>
-cudaError_t f32_case(const PagedAttnArgs& a, int ctas, cudaStream_t s) {
-    paged_decode_f32_kernel<HD, R><<<ctas, kDecThreads, DecF32<HD, R>::kSmem + (a.n_seq + 1) * 4, s>>>(a);
+cudaError_t f32_case(const PagedAttnArgs& a, int sms, cudaStream_t s) {
+    paged_decode_f32_kernel<HD, R><<<sms * DecF32<HD, R>::kCtas, kDecThreads, DecF32<HD, R>::kSmem + (a.n_seq + 1) * 4, s>>>(a);
     return cudaGetLastError();
 }
 
 template <int HD>
-cudaError_t f32_rows(int rows, const PagedAttnArgs& a, int ctas, cudaStream_t s) {
+cudaError_t f32_rows(int rows, const PagedAttnArgs& a, int sms, cudaStream_t s) {
     switch (rows) {
-        case 1: return f32_case<HD, 1>(a, ctas, s);
-        case 2: return f32_case<HD, 2>(a, ctas, s);
-        case 4: return f32_case<HD, 4>(a, ctas, s);
-        default: return f32_case<HD, 8>(a, ctas, s);
+        case 1: return f32_case<HD, 1>(a, sms, s);
+        case 2: return f32_case<HD, 2>(a, sms, s);
+        case 4: return f32_case<HD, 4>(a, sms, s);
+        default: return f32_case<HD, 8>(a, sms, s);
     }
 }
 
@@ -653,10 +661,10 @@ bool paged_decode_maps(PagedMaps* maps, const void* k, const void* v, int hd, in
     return make_map_sw128(&maps->k_dec, k, 3, dims, strides, box) && make_map_sw128(&maps->v_dec, v, 3, dims, strides, box);
 }
 
-cudaError_t launch_paged_decode(int dtype, int hd, int tile_rows, const PagedMaps& maps, const PagedAttnArgs& a, int ctas,
+cudaError_t launch_paged_decode(int dtype, int hd, int tile_rows, const PagedMaps& maps, const PagedAttnArgs& a, int sms,
                                 cudaStream_t s) {
-    if (dtype == RBT_MOE_DT_BF16) return hd == 64 ? bf16_case<64>(maps, a, ctas, s) : bf16_case<128>(maps, a, ctas, s);
-    return hd == 64 ? f32_rows<64>(tile_rows, a, ctas, s) : f32_rows<128>(tile_rows, a, ctas, s);
+    if (dtype == RBT_MOE_DT_BF16) return hd == 64 ? bf16_case<64>(maps, a, sms, s) : bf16_case<128>(maps, a, sms, s);
+    return hd == 64 ? f32_rows<64>(tile_rows, a, sms, s) : f32_rows<128>(tile_rows, a, sms, s);
 }
 
 }  // namespace rbt

@@ -13,6 +13,7 @@
 
 #include "common.cuh"
 #include "paged.h"
+#include "tc_ptx.cuh"
 
 namespace rbt {
 namespace paged {
@@ -25,6 +26,33 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+
+constexpr long long kWaitClocks = 4000000000ll;  // 2 s and more: far beyond any legitimate wait
+
+// A wait that gives up once, for good: the softmax then passes its other barriers at once.
+struct Waiter {
+    bool ok = true;
+    unsigned* status;
+    __device__ __forceinline__ void operator()(uint64_t* bar, uint32_t parity) {
+        if (!ok || tc::mbar_try_wait(bar, parity)) return;
+        const long long t0 = clock64();
+        while (!tc::mbar_try_wait(bar, parity))
+            if (clock64() - t0 > kWaitClocks) {
+                ok = false;
+                atomicCAS(status, 0u, (unsigned)kPagedWait);
+                return;
+            }
+    }
+    __device__ __forceinline__ bool one(uint64_t* bar, uint32_t parity) {
+        (*this)(bar, parity);
+        return ok;
+    }
+    // for a whole warp, which goes on only if every lane may
+    __device__ __forceinline__ bool warp(uint64_t* bar, uint32_t parity) {
+        (*this)(bar, parity);
+        return ok = __all_sync(FULL_MASK, ok);
+    }
+};
 
 struct Seq {
     int row0, count, len;  // first row, new tokens, positions; count 0: not of this launch

@@ -41,7 +41,6 @@ constexpr int kTcRows = kPagedTcRows;      // two tiles
 constexpr int kTcBlock = 128;              // positions of a block: one stage of k and v
 constexpr int kTcStep = 64;                // positions of a softmax step
 constexpr int kTcThreads = 352;
-constexpr long long kTcWaitClocks = 4000000000ll;  // 2 s and more: far beyond any legitimate wait
 constexpr float kTcRescale = 8.0f;         // log2 of the largest weight before the maximum moves
 
 template <int HD>
@@ -180,31 +179,6 @@ struct Row {
         }
         sum[0] = add2(sum[0], sum[1]);
         return __uint_as_float((uint32_t)sum[0]) + __uint_as_float((uint32_t)(sum[0] >> 32));
-    }
-};
-
-// A wait that gives up once, for good: the softmax then passes its other barriers at once.
-struct Waiter {
-    bool ok = true;
-    unsigned* status;
-    __device__ __forceinline__ void operator()(uint64_t* bar, uint32_t parity) {
-        if (!ok || mbar_try_wait(bar, parity)) return;
-        const long long t0 = clock64();
-        while (!mbar_try_wait(bar, parity))
-            if (clock64() - t0 > kTcWaitClocks) {
-                ok = false;
-                atomicCAS(status, 0u, (unsigned)kPagedWait);
-                return;
-            }
-    }
-    __device__ __forceinline__ bool one(uint64_t* bar, uint32_t parity) {
-        (*this)(bar, parity);
-        return ok;
-    }
-    // for a whole warp, which goes on only if every lane may
-    __device__ __forceinline__ bool warp(uint64_t* bar, uint32_t parity) {
-        (*this)(bar, parity);
-        return ok = __all_sync(FULL_MASK, ok);
     }
 };
 
