@@ -120,6 +120,7 @@ int rbt_paged_create(RbtPaged** out, const RbtPagedConfig* cfg, int device) {
         if (c.n_heads <= 0 || c.n_kv_heads <= 0 || c.n_heads % c.n_kv_heads)
             return fail("n_heads %d is not a multiple of n_kv_heads %d", c.n_heads, c.n_kv_heads);
         if (c.n_heads > 1024) return fail("n_heads %d above the supported 1024", c.n_heads);
+        if (c.n_heads / c.n_kv_heads > 512) return fail("%d heads per kv head above the supported 512", c.n_heads / c.n_kv_heads);
         if ((int64_t)c.n_pages * c.n_kv_heads * c.page_size > INT32_MAX)
             return fail("n_pages %d * n_kv_heads %d * page_size %d exceeds 2^31 - 1 rows", c.n_pages, c.n_kv_heads,
                         c.page_size);
@@ -379,6 +380,10 @@ int rbt_paged_attention_device(RbtPaged* p, int layer, const RbtPagedAttention* 
     a.n_heads = c.n_heads;
     a.n_kv = c.n_kv_heads;
     a.group = c.n_heads / c.n_kv_heads;
+    a.group_inv = ((1u << 20) + a.group - 1) / a.group;
+    a.group_inv32 = a.group == 1 ? 0xffffffffu : (unsigned)(((1ull << 32) + a.group - 1) / a.group);
+    const int64_t most_len = (int64_t)x.table_stride << p->page_shift;
+    a.most_len = most_len > INT32_MAX ? INT32_MAX : (int)most_len;
     a.page_shift = p->page_shift;
     a.n_pages = c.n_pages;
     a.causal = x.causal;
@@ -397,6 +402,10 @@ int rbt_paged_attention_device(RbtPaged* p, int layer, const RbtPagedAttention* 
     int dec_rows = few;
     if (!bf)
         while (dec_rows > 1 && dec_rows / 2 >= most) dec_rows /= 2;
+    // units of one kv head (tiles of a launch times blocks, of 16 positions or more) are counted in 31 bits
+    const int tile = most <= few ? dec_rows : few;
+    if (((int64_t)x.n_rows * a.group / tile + x.n_seq) * (a.most_len / 16 + 1) > INT32_MAX)
+        return fail("%d rows over tables of %d positions are too many for one call", x.n_rows, a.most_len);
     const PagedMaps& maps = p->layers[layer].maps;
     if (most <= few || x.n_seq > 1) {
         a.rows_lo = 0;

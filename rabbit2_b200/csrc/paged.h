@@ -45,6 +45,8 @@ struct PagedAttnArgs {
     long q_stride, out_stride;
     const int32_t *cu, *len, *table;
     int table_stride, n_rows, n_seq, n_heads, n_kv, group;
+    unsigned group_inv, group_inv32;  // ceil(2^20 / group), 2^32 / group (31 bits of it count)
+    int most_len;        // positions that a row of the table holds
     int page_shift, n_pages;
     int causal, window;
     int rows_lo, rows_hi;  // sequences with rows_lo < new tokens * group <= rows_hi are this launch's

@@ -35,7 +35,7 @@ struct RowsCfg {
 };
 
 template <int HD>
-__global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedAttnArgs a) {
+__global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const __grid_constant__ PagedAttnArgs a) {
     using C = RowsCfg<HD>;
     constexpr int RM = C::kRM, KN = C::kKN, KB = C::kBlock, LD = C::kLd, LDP = C::kLdP, DV = HD / 64;
     constexpr int V = 4, CH = HD / V;
@@ -44,23 +44,24 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedAtt
     float* Ks = Qs + C::kRows * LD;
     float* Vs = Ks + KB * LD;
     float* Ps = Vs + KB * LD;
-    int* starts = reinterpret_cast<int*>(sm + C::kFloats);
+    const Plan plan(a, sm + C::kFloats);
     __shared__ Share share;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    find_share<kRowsThreads, C::kRows, KB, 4>(a, starts, &share);
-    Walk<C::kRows, KB> w(share, starts);
+    find_share<kRowsThreads, C::kRows, KB, 4>(a, plan, &share);
+    Walk<C::kRows, KB> w(share, plan);
     if (tid == 0) a.join[blockIdx.x].last = blockIdx.x;
     const float k2 = a.scale * kLog2e;
     const int page = 1 << a.page_shift;
+#pragma unroll 1
     while (w.next(a)) {
         const Tile& t = w.t;
         for (int e = tid; e < C::kRows * CH; e += kRowsThreads) {
             const int r = e / CH, c = (e - r * CH) * V;
             float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
             if (r < t.rows) {
-                const int tok = (t.r0 + r) / a.group, g = (t.r0 + r) - tok * a.group;
+                const int tok = t.token(a, r), h = t.head(a, r);
                 f = *reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + (t.s.row0 + tok) * a.q_stride +
-                                                     (size_t)(t.kvh * a.group + g) * HD + c);
+                                                     (size_t)h * HD + c);
             }
             *reinterpret_cast<float4*>(Qs + r * LD + c) = f;
         }
@@ -69,7 +70,7 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedAtt
         float4 o[RM][DV];
 #pragma unroll
         for (int i = 0; i < RM; i++) {
-            const int r = ty * RM + i, pos = t.off + (t.r0 + r) / a.group;
+            const int r = ty * RM + i, pos = t.off + t.token(a, r);
             to[i] = r >= t.rows ? 0 : a.causal ? min(t.s.len, pos + 1) : t.s.len;
             from[i] = a.window ? max(0, pos - a.window + 1) : 0;
             m[i] = -INFINITY;
@@ -78,6 +79,7 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedAtt
             for (int k = 0; k < DV; k++) o[i][k] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
         const int32_t* table = a.table + (size_t)t.seq * a.table_stride;
+#pragma unroll 1
         for (int b = w.first; b < w.first + w.n; b++) {
             const int p0 = b * KB;
             __syncthreads();  // the block before is consumed (and Qs written, on the first pass)
@@ -180,7 +182,7 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedAtt
             for (int i = 0; i < RM; i++) {
                 const int r = ty * RM + i;
                 if (r >= t.rows) continue;
-                const int tok = (t.r0 + r) / a.group, h = t.kvh * a.group + (t.r0 + r) - tok * a.group;
+                const int tok = t.token(a, r), h = t.head(a, r);
                 const float inv = l[i] > 0.0f || l[i] != l[i] ? 1.0f / l[i] : 0.0f;
                 float* dst = static_cast<float*>(a.out) + (t.s.row0 + tok) * a.out_stride + (size_t)h * HD;
 #pragma unroll
@@ -216,7 +218,7 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const PagedAtt
 constexpr int kJoinThreads = 128, kJoinSplit = 8;
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAttnArgs a, int tile_rows) {
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedAttnArgs a, int tile_rows) {
     const PagedJoin j = a.join[blockIdx.x];
     const int c0 = blockIdx.x;
     if (j.last <= c0) return;
@@ -227,6 +229,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAtt
         float M = -INFINITY, L = 0.0f, o[DL];
 #pragma unroll
         for (int d = 0; d < DL; d++) o[d] = 0.0f;
+#pragma unroll 1
         for (int c = c0; c <= j.last; c++) {
             const float* p = a.part + ((size_t)c * 2 + (c == c0)) * part_floats;
             const float m = p[r], l = p[tile_rows + r];
@@ -264,13 +267,13 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAtt
 template <int HD>
 cudaError_t rows_init() {
     return cudaFuncSetAttribute(paged_rows_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                RowsCfg<HD>::kFloats * 4 + (kPagedMaxSeq + 1) * 4);
+                                RowsCfg<HD>::kFloats * 4 + Plan::bytes(kPagedMaxSeq));
 }
 
 template <int HD>
 cudaError_t rows_case(const PagedAttnArgs& a, int ctas, cudaStream_t s) {
     using C = RowsCfg<HD>;
-    const int smem = C::kFloats * 4 + (a.n_seq + 1) * 4;
+    const int smem = C::kFloats * 4 + Plan::bytes(a.n_seq);
     paged_rows_kernel<HD><<<ctas, kRowsThreads, smem, s>>>(a);
     return cudaGetLastError();
 }

@@ -70,16 +70,17 @@ __device__ __forceinline__ void ring_init(Ring<kStages>* r) {
 // positions [off, off + box rows) of page id into box `box` of its half of the stage (one
 // lane per box).
 template <int kRows, int kBlock, int kStages, typename Copy>
-__device__ __forceinline__ void produce(const PagedAttnArgs& a, const Share& share, const int* starts, Ring<kStages>* ring,
+__device__ __forceinline__ void produce(const PagedAttnArgs& a, const Share& share, const Plan& plan, Ring<kStages>* ring,
                                         uint8_t* stages, int box_rows, uint32_t row_bytes, Copy copy) {
     const int lane = threadIdx.x & 31;
-    Walk<kRows, kBlock> w(share, starts);
+    Walk<kRows, kBlock> w(share, plan);
     uint32_t j = 0;
     Waiter wait;
-    wait.status = a.status;
+#pragma unroll 1
     while (wait.ok && w.next(a)) {
         const int32_t* table = a.table + (size_t)w.t.seq * a.table_stride;
         int chunk = -1, ids = 0;  // 32 entries of the table row, one per lane
+#pragma unroll 1
         for (int b = w.first; b < w.first + w.n; b++, j++) {
             const int p0 = b * kBlock, left = min(kBlock, w.t.hi - p0);
             const int boxes = left > 0 ? (left + box_rows - 1) / box_rows : 0;
@@ -105,9 +106,12 @@ __device__ __forceinline__ void produce(const PagedAttnArgs& a, const Share& sha
         }
     }
     // every copy has landed before the CTA may exit
+    wait.report(a.status);
     wait.ok = true;
+#pragma unroll 1
     for (uint32_t i = j > kStages ? j - kStages : 0; i < j; i++)
         wait(&ring->full[i % kStages], (i / kStages) & 1);
+    wait.report(a.status);
 }
 
 // The four warps' parts of a segment, in shared memory: two sets of maxima and sums (the
@@ -132,7 +136,7 @@ __device__ __forceinline__ void put4(T* dst, float4 f) {
 
 template <typename T, int HD>
 __device__ __forceinline__ void put_row(const PagedAttnArgs& a, const Tile& t, int r, int c, float4 o, float M, float L) {
-    const int tok = (t.r0 + r) / a.group, h = t.kvh * a.group + (t.r0 + r) - tok * a.group;
+    const int tok = t.token(a, r), h = t.head(a, r);
     const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;
     put4(static_cast<T*>(a.out) + (t.s.row0 + tok) * a.out_stride + (size_t)h * HD + c,
          make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
@@ -148,6 +152,7 @@ __device__ __forceinline__ void finish(const PagedAttnArgs& a, const W& w, const
     constexpr int kThreads = 32 * kDecWarps, kFloats = paged_part_floats(kRows, HD), kO = paged_part_o(kRows);
     const Tile& t = w.t;
     float* part = a.part + ((size_t)blockIdx.x * 2 + (w.head ? 1 : 0)) * kFloats;
+#pragma unroll 1
     for (int e = threadIdx.x; e < t.rows * (HD / 4); e += kThreads) {
         const int r = e / (HD / 4), c = 4 * (e - r * (HD / 4));
         float M = -INFINITY;
@@ -190,11 +195,13 @@ __device__ __forceinline__ void finish(const PagedAttnArgs& a, const W& w, const
     named_sync(1, kThreads);
     if (!*last) return;
     __threadfence();
+#pragma unroll 1
     for (int e = threadIdx.x; e < t.rows * (HD / 4); e += kThreads) {
         const int r = e / (HD / 4), c = 4 * (e - r * (HD / 4));
         const float* p = a.part + ((size_t)c0 * 2 + 1) * kFloats;  // slot 1 of the first CTA, slot 0 of the others
         float M = -INFINITY, L = 0.0f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
         for (int i = c0; i <= c1; i++, p = a.part + (size_t)i * 2 * kFloats) {
             const float m = __ldcg(p + r), l = __ldcg(p + kRows + r);
             const float4 f = __ldcg(reinterpret_cast<const float4*>(p + kO + (size_t)r * HD + c));
@@ -245,13 +252,13 @@ struct DecBf16 {
 template <int HD>
 __global__ void __launch_bounds__(kDecThreads, DecBf16<HD>::kCtas)
     paged_decode_bf16_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                             const PagedAttnArgs a) {
+                             const __grid_constant__ PagedAttnArgs a) {
     using C = DecBf16<HD>;
     constexpr int KB = C::kBlock, NT = KB / 8, KS = HD / 16;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     Parts<C::kRows, HD>* parts = reinterpret_cast<Parts<C::kRows, HD>*>(smem + C::kStages * kDecStage);
-    int* starts = reinterpret_cast<int*>(parts + 1);
+    const Plan plan(a, parts + 1);
     __shared__ Ring<C::kStages> ring;
     __shared__ Share share;
     __shared__ int last;
@@ -260,12 +267,12 @@ __global__ void __launch_bounds__(kDecThreads, DecBf16<HD>::kCtas)
         prefetch_tmap(&tm_k);
         prefetch_tmap(&tm_v);
     }
-    find_share<kDecThreads, C::kRows, KB, kDecMinUnits>(a, starts, &share);  // (its barriers publish the ring's too)
+    find_share<kDecThreads, C::kRows, KB, kDecMinUnits>(a, plan, &share);  // (its barriers publish the ring's too)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int page = 1 << a.page_shift, box = min(page, KB);
     if (warp >= kDecWarps) {
         const bool is_v = warp > kDecWarps;
-        produce<C::kRows, KB>(a, share, starts, &ring, smem + (is_v ? C::kHalf : 0), box, HD * 2,
+        produce<C::kRows, KB>(a, share, plan, &ring, smem + (is_v ? C::kHalf : 0), box, HD * 2,
                               [&](int id, int kvh, int off, int i, uint8_t* stage, uint64_t* bar) {
                                   const int y = ((id * a.n_kv + kvh) << a.page_shift) + off;
                                   tma_load_3d(stage + i * box * HD * 2, is_v ? &tm_v : &tm_k, bar, 0, y, 0);
@@ -286,40 +293,46 @@ __global__ void __launch_bounds__(kDecThreads, DecBf16<HD>::kCtas)
 #pragma unroll
     for (int k = 0; k < NT / 2; k++) v_row[k] = C::kHalf + row_at(16 * k + (lane & 15));
     const uint32_t k_swz = ((lane >> 3) ^ (lane & 7)) << 4, v_swz = ((lane >> 4) ^ (lane & 7)) << 4;
-    Walk<C::kRows, KB> w(share, starts);
+    Walk<C::kRows, KB> w(share, plan);
     uint32_t j = 0;
     Waiter wait;  // (after one that ran out it waits no more: the results are void, the barriers are still met)
-    wait.status = a.status;
+#pragma unroll 1
     for (int set = 0; w.next(a); set ^= 1) {
         const Tile& t = w.t;
-        uint32_t q[KS][4];  // rows g and g + 8 as A fragments
-        int to[2], from[2];
-        const uint16_t* qp[2];
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int r = g + 8 * i, tok = (t.r0 + r) / a.group, pos = t.off + tok;
-            to[i] = r >= t.rows ? 0 : a.causal ? min(t.s.len, pos + 1) : t.s.len;
-            from[i] = a.window ? max(0, pos - a.window + 1) : 0;
-            qp[i] = r >= t.rows ? nullptr
-                                : static_cast<const uint16_t*>(a.q) + (t.s.row0 + tok) * a.q_stride +
-                                      (size_t)(t.kvh * a.group + (t.r0 + r) - tok * a.group) * HD;
+        // q as A fragments (rows g and g + 8), through shared memory: each warp its own copy, 16-byte
+        // chunk c of row r at chunk c ^ (r & 7) of the row
+        uint32_t q[KS][4];
+        uint8_t* qw = reinterpret_cast<uint8_t*>(&parts->o[warp][0][0]);  // (free between two segments' sums)
+#pragma unroll 1
+        for (int e = lane; e < C::kRows * (HD / 8); e += 32) {
+            const int r = e / (HD / 8), c = e - r * (HD / 8);
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (r < t.rows)
+                x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
+                                                    (t.s.row0 + t.token(a, r)) * a.q_stride + (size_t)t.head(a, r) * HD + 8 * c);
+            *reinterpret_cast<uint4*>(qw + r * (HD * 2) + ((c ^ (r & 7)) << 4)) = x;
         }
+        __syncwarp();
 #pragma unroll
         for (int k = 0; k < KS; k++)
+            ldsm4(smem_u32(qw) + (lane & 15) * (HD * 2) + (((2 * k + (lane >> 4)) ^ (lane & 7)) << 4), q[k]);
+        int to[2], from[2];
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                q[k][i] = qp[i] ? *reinterpret_cast<const uint32_t*>(qp[i] + 16 * k + 2 * tq) : 0u;
-                q[k][i + 2] = qp[i] ? *reinterpret_cast<const uint32_t*>(qp[i] + 16 * k + 8 + 2 * tq) : 0u;
-            }
+        for (int i = 0; i < 2; i++) {
+            const int r = g + 8 * i, pos = t.off + t.token(a, r);
+            to[i] = r >= t.rows ? 0 : a.causal ? min(t.s.len, pos + 1) : t.s.len;
+            from[i] = a.window ? max(0, pos - a.window + 1) : 0;
+        }
         // blocks that every row of the tile sees whole need no mask
-        const int sure_to = a.causal ? min(t.s.len, t.off + t.r0 / a.group + 1) : t.s.len;
-        const int sure_from = a.window ? t.off + (t.r0 + t.rows - 1) / a.group - a.window + 1 : 0;
+        const int sure_to = a.causal ? min(t.s.len, t.off + t.tok0 + 1) : t.s.len;
+        const int sure_from = a.window ? t.off + t.token(a, t.rows - 1) - a.window + 1 : 0;
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[HD / 8][4];
 #pragma unroll
         for (int n = 0; n < HD / 8; n++)
 #pragma unroll
             for (int i = 0; i < 4; i++) o[n][i] = 0.0f;
         const uint32_t skip = (warp - j) & (kDecWarps - 1);
+#pragma unroll 1
         for (int i = skip; i < w.n; i += kDecWarps) {
             const uint32_t jj = j + i, st = jj % C::kStages;
             const int p0 = (w.first + i) * KB;
@@ -384,6 +397,7 @@ __global__ void __launch_bounds__(kDecThreads, DecBf16<HD>::kCtas)
             }
             const bool tail = p0 + KB > t.hi;
             if (tail) {  // what lies behind the last position is not a number, perhaps: no weight of 0 hides that
+#pragma unroll 1
                 for (int e = lane; e < KB * (HD / 8); e += 32) {
                     const int r = e / (HD / 8), c = e - r * (HD / 8);
                     if (p0 + r >= t.hi)
@@ -432,6 +446,7 @@ __global__ void __launch_bounds__(kDecThreads, DecBf16<HD>::kCtas)
         named_sync(1, 32 * kDecWarps);
         finish<uint16_t, C::kRows, HD>(a, w, parts, set, &last);
     }
+    wait.report(a.status);
 }
 
 // ---------------------------------------------------------------- f32
@@ -444,25 +459,25 @@ struct DecF32 {
 };
 
 template <int HD, int R>
-__global__ void __launch_bounds__(kDecThreads, DecF32<HD, R>::kCtas) paged_decode_f32_kernel(const PagedAttnArgs a) {
+__global__ void __launch_bounds__(kDecThreads, DecF32<HD, R>::kCtas) paged_decode_f32_kernel(const __grid_constant__ PagedAttnArgs a) {
     using C = DecF32<HD, R>;
     constexpr int KB = C::kBlock, NI = KB / 4, NC = HD / 32, DL = HD / 32;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
     Parts<R, HD>* parts = reinterpret_cast<Parts<R, HD>*>(smem + C::kStages * kDecStage);
     float* weights = reinterpret_cast<float*>(parts + 1);  // [warp][KB][R]
-    int* starts = reinterpret_cast<int*>(weights + kDecWarps * KB * R);
+    const Plan plan(a, weights + kDecWarps * KB * R);
     __shared__ Ring<C::kStages> ring;
     __shared__ Share share;
     __shared__ int last;
     ring_init(&ring);
-    find_share<kDecThreads, R, KB, kDecMinUnits>(a, starts, &share);
+    find_share<kDecThreads, R, KB, kDecMinUnits>(a, plan, &share);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int page = 1 << a.page_shift, box = min(page, KB);
     if (warp >= kDecWarps) {
         const bool is_v = warp > kDecWarps;
         const float* src = static_cast<const float*>(is_v ? a.v : a.k);
-        produce<R, KB>(a, share, starts, &ring, smem + (is_v ? C::kHalf : 0), box, HD * 4,
+        produce<R, KB>(a, share, plan, &ring, smem + (is_v ? C::kHalf : 0), box, HD * 4,
                        [&](int id, int kvh, int off, int i, uint8_t* stage, uint64_t* bar) {
                            const size_t row = (((size_t)id * a.n_kv + kvh) << a.page_shift) + off;
                            const uint32_t bytes = box * HD * 4;
@@ -473,21 +488,21 @@ __global__ void __launch_bounds__(kDecThreads, DecF32<HD, R>::kCtas) paged_decod
     const int kg = lane >> 3, jj = lane & 7;
     const float k2 = a.scale * kLog2e;
     float* wp = weights + warp * KB * R;
-    Walk<R, KB> w(share, starts);
+    Walk<R, KB> w(share, plan);
     uint32_t j = 0;
     Waiter wait;  // (after one that ran out it waits no more: the results are void, the barriers are still met)
-    wait.status = a.status;
+#pragma unroll 1
     for (int set = 0; w.next(a); set ^= 1) {
         const Tile& t = w.t;
         float4 q[R][NC];
         int to[R], from[R];
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            const int tok = (t.r0 + r) / a.group, pos = t.off + tok;
+            const int tok = t.token(a, r), pos = t.off + tok;
             to[r] = r >= t.rows ? 0 : a.causal ? min(t.s.len, pos + 1) : t.s.len;
             from[r] = a.window ? max(0, pos - a.window + 1) : 0;
             const float* src = static_cast<const float*>(a.q) + (t.s.row0 + tok) * a.q_stride +
-                               (size_t)(t.kvh * a.group + (t.r0 + r) - tok * a.group) * HD;
+                               (size_t)t.head(a, r) * HD;
 #pragma unroll
             for (int c = 0; c < NC; c++)
                 q[r][c] = r < t.rows ? *reinterpret_cast<const float4*>(src + 4 * (jj + 8 * c))
@@ -502,6 +517,7 @@ __global__ void __launch_bounds__(kDecThreads, DecF32<HD, R>::kCtas) paged_decod
             for (int d = 0; d < DL; d++) o[r][d] = 0.0f;
         }
         const uint32_t skip = (warp - j) & (kDecWarps - 1);
+#pragma unroll 1
         for (int b = skip; b < w.n; b += kDecWarps) {
             const uint32_t jb = j + b, st = jb % C::kStages;
             const int p0 = (w.first + b) * KB, nv = min(KB, t.hi - p0);
@@ -608,23 +624,24 @@ __global__ void __launch_bounds__(kDecThreads, DecF32<HD, R>::kCtas) paged_decod
         named_sync(1, 32 * kDecWarps);
         finish<float, R, HD>(a, w, parts, set, &last);
     }
+    wait.report(a.status);
 }
 
 template <typename K>
 cudaError_t set_smem(K kernel, int bytes) {
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes + (kPagedMaxSeq + 1) * 4);
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes + Plan::bytes(kPagedMaxSeq));
 }
 
 template <int HD>
 cudaError_t bf16_case(const PagedMaps& maps, const PagedAttnArgs& a, int sms, cudaStream_t s) {
     paged_decode_bf16_kernel<HD>
-        <<<sms * DecBf16<HD>::kCtas, kDecThreads, DecBf16<HD>::kSmem + (a.n_seq + 1) * 4, s>>>(maps.k_dec, maps.v_dec, a);
+        <<<sms * DecBf16<HD>::kCtas, kDecThreads, DecBf16<HD>::kSmem + Plan::bytes(a.n_seq), s>>>(maps.k_dec, maps.v_dec, a);
     return cudaGetLastError();
 }
 
 template <int HD, int R>
 cudaError_t f32_case(const PagedAttnArgs& a, int sms, cudaStream_t s) {
-    paged_decode_f32_kernel<HD, R><<<sms * DecF32<HD, R>::kCtas, kDecThreads, DecF32<HD, R>::kSmem + (a.n_seq + 1) * 4, s>>>(a);
+    paged_decode_f32_kernel<HD, R><<<sms * DecF32<HD, R>::kCtas, kDecThreads, DecF32<HD, R>::kSmem + Plan::bytes(a.n_seq), s>>>(a);
     return cudaGetLastError();
 }
 

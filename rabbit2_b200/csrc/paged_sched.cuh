@@ -29,18 +29,18 @@ __device__ __forceinline__ float ex2(float x) {
 
 constexpr long long kWaitClocks = 4000000000ll;  // 2 s and more: far beyond any legitimate wait
 
-// A wait that gives up once, for good: the softmax then passes its other barriers at once.
+// A wait that gives up once, for good: what waits then passes its other barriers at once, and
+// says so at its end (report).
 struct Waiter {
     bool ok = true;
-    unsigned* status;
     __device__ __forceinline__ void operator()(uint64_t* bar, uint32_t parity) {
         if (!ok || tc::mbar_try_wait(bar, parity)) return;
         const long long t0 = clock64();
+#pragma unroll 1
         while (!tc::mbar_try_wait(bar, parity))
             if (clock64() - t0 > kWaitClocks) {
                 ok = false;
-                atomicCAS(status, 0u, (unsigned)kPagedWait);
-                return;
+                break;
             }
     }
     __device__ __forceinline__ bool one(uint64_t* bar, uint32_t parity) {
@@ -51,6 +51,9 @@ struct Waiter {
     __device__ __forceinline__ bool warp(uint64_t* bar, uint32_t parity) {
         (*this)(bar, parity);
         return ok = __all_sync(FULL_MASK, ok);
+    }
+    __device__ __forceinline__ void report(unsigned* status) const {
+        if (!ok) atomicCAS(status, 0u, (unsigned)kPagedWait);
     }
 };
 
@@ -67,23 +70,44 @@ __device__ __forceinline__ Seq load_seq(const PagedAttnArgs& a, int i) {
     s.count = end - s.row0;
     unsigned bad = 0;
     if (s.row0 < 0 || end < s.row0 || end > a.n_rows) bad = kPagedCu;
-    else if (s.len < 0 || (long long)s.len > ((long long)a.table_stride << a.page_shift)) bad = kPagedLen;
+    else if (s.len < 0 || s.len > a.most_len) bad = kPagedLen;
     if (bad) {
         atomicCAS(a.status, 0u, bad);
         s.count = 0;
     }
-    const long long rows = (long long)s.count * a.group;
+    const int rows = s.count * a.group;  // (the host bounds n_rows * group to 31 bits)
     if (rows <= a.rows_lo || rows > a.rows_hi) s.count = 0;
     return s;
 }
+
+// What the CTA keeps of the sequences, in dynamic shared memory: their first tiles and
+// themselves, read once.
+struct Plan {
+    int* starts;  // [n_seq + 1] first tile of each sequence, among one kv head's tiles
+    Seq* seqs;    // [n_seq]
+    __device__ __forceinline__ Plan(const PagedAttnArgs& a, void* smem)
+        : starts(static_cast<int*>(smem)), seqs(reinterpret_cast<Seq*>(starts + a.n_seq + 1)) {}
+    __host__ __device__ static constexpr int bytes(int n_seq) { return 4 + n_seq * (4 + (int)sizeof(Seq)); }
+};
 
 struct Tile {
     int seq, kvh;
     Seq s;
     int r0, rows;    // packed rows [r0, r0 + rows) of the sequence
+    int tok0, rem0;  // row r0 is head rem0 of token tok0
     int lo, hi;      // positions that some row of the tile sees
     int b0, nb;      // blocks b0 .. b0 + nb
     int off;         // position of a token minus its index: len - count
+
+    // Token of the sequence and head of the group of row r0 + r, 0 <= r < 512: rem0 + r < 1024 and the
+    // group is at most 512, for which the product with ceil(2^20 / group) gives the quotient exactly.
+    __device__ __forceinline__ int token(const PagedAttnArgs& a, int r) const {
+        return tok0 + (int)(((unsigned)(rem0 + r) * a.group_inv) >> 20);
+    }
+    __device__ __forceinline__ int head(const PagedAttnArgs& a, int r) const {
+        const unsigned x = rem0 + r, d = (x * a.group_inv) >> 20;
+        return kvh * a.group + (int)(x - d * a.group);
+    }
 };
 
 template <int kRows, int kBlock>
@@ -92,28 +116,52 @@ __device__ __forceinline__ void tile_range(const PagedAttnArgs& a, const Seq& s,
     t.r0 = r0;
     t.rows = min(kRows, s.count * a.group - r0);
     t.off = s.len - s.count;
+    t.tok0 = __umulhi((unsigned)r0, a.group_inv32);  // (off by one at most: r0 < 2^31)
+    t.rem0 = r0 - t.tok0 * a.group;
+    if (t.rem0 < 0) {
+        t.tok0--;
+        t.rem0 += a.group;
+    } else if (t.rem0 >= a.group) {
+        t.tok0++;
+        t.rem0 -= a.group;
+    }
     t.lo = 0;
     t.hi = s.len;
     if (a.causal) {
-        t.hi = max(0, min(s.len, t.off + (r0 + t.rows - 1) / a.group + 1));
-        if (a.window) t.lo = max(0, t.off + r0 / a.group - a.window + 1);
+        t.hi = max(0, min(s.len, t.off + t.token(a, t.rows - 1) + 1));
+        if (a.window) t.lo = max(0, t.off + t.tok0 - a.window + 1);
     }
     t.b0 = t.lo / kBlock;
     t.nb = max(1, (t.hi + kBlock - 1) / kBlock - t.b0);  // a tile that sees nothing is one unit, which writes its zeros
 }
 
+// How the units fall to the CTAs: CTA c begins at unit start(c) = units * c / ctas.
+struct Split {
+    long long units, per;  // of all kv heads; units / ctas
+    int rest, ctas;        // units % ctas; CTAs with any work
+    __device__ __forceinline__ long long start(int c) const { return per * c + (unsigned)(rest * c) / (unsigned)ctas; }
+    __device__ __forceinline__ int holder(long long u) const {  // the CTA that has unit u (an estimate, and the step or two it is off)
+        int c = min(ctas - 1, (int)((float)u / (float)units * (float)ctas));
+#pragma unroll 1
+        while (start(c) > u) c--;
+#pragma unroll 1
+        while (start(c + 1) <= u) c++;
+        return c;
+    }
+};
+
 // The share of this CTA: `left` units from block `skip` of tile `tile` of kv head `kvh`.
 struct Share {
+    Split split;
+    long long left;
     int tile, kvh, skip;  // index of the tile among one kv head's tiles
     int n_tiles;
-    int ctas;             // CTAs with any work
-    long long units;      // of all kv heads
-    long long left;
 };
 
 // largest i with start[i] <= x
 __device__ __forceinline__ int find(const int* start, int n, int x) {
     int lo = 0, hi = n;
+#pragma unroll 1
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (start[mid] <= x) lo = mid;
@@ -124,21 +172,20 @@ __device__ __forceinline__ int find(const int* start, int n, int x) {
 
 // Exclusive sum over the CTA's threads in order.  scratch: kThreads / 32 words.
 template <int kThreads>
-__device__ __forceinline__ long long scan(long long v, long long* scratch, long long* total) {
+__device__ __forceinline__ int scan(int v, int* scratch, int* total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    long long inc = v;
+    int inc = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long u = __shfl_up_sync(FULL_MASK, inc, o);
+        const int u = __shfl_up_sync(FULL_MASK, inc, o);
         if (lane >= o) inc += u;
     }
-    __syncthreads();  // scratch may still be read from an earlier scan
     if (lane == 31) scratch[warp] = inc;
     __syncthreads();
-    long long before = 0, all = 0;
+    int before = 0, all = 0;
 #pragma unroll
     for (int w = 0; w < kThreads / 32; w++) {
-        const long long s = scratch[w];
+        const int s = scratch[w];
         if (w < warp) before += s;
         all += s;
     }
@@ -146,75 +193,85 @@ __device__ __forceinline__ long long scan(long long v, long long* scratch, long 
     return before + inc - v;
 }
 
-// All threads of the CTA call it.  starts: n_seq + 1 ints of shared memory that stay (the
-// first tile of each sequence); share: one Share in shared memory, valid after the call.
+// All threads of the CTA call it; share, in shared memory, is valid after the call.  A CTA
+// takes at least kMinUnits units unless there are tiles for more CTAs than that: finer
+// parts of a tile cost more to add up than they save.  The lengths are read here, once;
+// what follows works on shared memory.
 template <int kThreads, int kRows, int kBlock, int kMinUnits>
-__device__ void find_share(const PagedAttnArgs& a, int* starts, Share* share) {
-    __shared__ long long scratch[kThreads / 32];
+__device__ __forceinline__ void find_share(const PagedAttnArgs& a, const Plan& plan, Share* share) {
+    __shared__ int scratch[2][kThreads / 32];
     const int tid = threadIdx.x, n = a.n_seq;
+    if (tid == 0) share->left = 0;
     const int per = (n + kThreads - 1) / kThreads, i0 = min(n, tid * per), i1 = min(n, i0 + per);
     int mine = 0;
+#pragma unroll 1
     for (int i = i0; i < i1; i++) {
-        const int tiles = (load_seq(a, i).count * a.group + kRows - 1) / kRows;
-        starts[i] = tiles;
+        const Seq s = load_seq(a, i);
+        plan.seqs[i] = s;
+        const int tiles = (s.count * a.group + kRows - 1) / kRows;
+        plan.starts[i] = tiles;
         mine += tiles;
     }
-    long long all_tiles;
-    int at = (int)scan<kThreads>(mine, scratch, &all_tiles);  // (the host bounds rows * group to 31 bits)
-    const int n_tiles = (int)all_tiles;
+    int n_tiles;
+    int at = scan<kThreads>(mine, scratch[0], &n_tiles);
+#pragma unroll 1
     for (int i = i0; i < i1; i++) {
-        const int tiles = starts[i];
-        starts[i] = at;
+        const int tiles = plan.starts[i];
+        plan.starts[i] = at;
         at += tiles;
     }
-    if (tid == 0) starts[n] = n_tiles;
+    if (tid == 0) plan.starts[n] = n_tiles;
     __syncthreads();
     // units of this thread's run of tiles
     const int pt = (n_tiles + kThreads - 1) / kThreads, g0 = min(n_tiles, tid * pt), g1 = min(n_tiles, g0 + pt);
-    long long units = 0;
+    int units = 0, first = 0;
     if (g0 < g1) {
-        int i = find(starts, n, g0);
-        Seq s = load_seq(a, i);
+        first = find(plan.starts, n, g0);
+        int i = first;
+#pragma unroll 1
         for (int g = g0; g < g1; g++) {
-            while (starts[i + 1] <= g) s = load_seq(a, ++i);
+#pragma unroll 1
+            while (plan.starts[i + 1] <= g) i++;
             Tile t;
-            tile_range<kRows, kBlock>(a, s, (g - starts[i]) * kRows, t);
+            tile_range<kRows, kBlock>(a, plan.seqs[i], (g - plan.starts[i]) * kRows, t);
             units += t.nb;
         }
     }
-    long long per_head;
-    const long long before = scan<kThreads>(units, scratch, &per_head);
-    const long long total = per_head * a.n_kv;
-    const int ctas = (int)min((long long)gridDim.x, (total + kMinUnits - 1) / kMinUnits);
+    int per_head;
+    const int before = scan<kThreads>(units, scratch[1], &per_head);  // (the host bounds it to 31 bits)
     const int c = blockIdx.x;
-    if (c >= ctas) {
-        if (tid == 0) {
-            share->left = 0;
-            share->ctas = ctas;
-        }
-    } else {
-        const long long u0 = total * c / ctas, u1 = total * (c + 1) / ctas;
-        const int kvh = (int)(u0 / per_head);
-        long long x = u0 - kvh * per_head;
+    Split sp;
+    sp.units = (long long)per_head * a.n_kv;
+    const long long most = max((sp.units + kMinUnits - 1) / kMinUnits, (long long)n_tiles * a.n_kv);
+    sp.ctas = (int)min((long long)gridDim.x, most);
+    if (c < sp.ctas) {
+        if (sp.units < (1ll << 31)) sp.per = (unsigned)sp.units / (unsigned)sp.ctas;
+        else sp.per = sp.units / sp.ctas;
+        sp.rest = (int)(sp.units - sp.per * sp.ctas);
+        const long long u0 = sp.start(c);
+        int kvh = (int)((float)u0 / (float)per_head);  // (an estimate, made exact)
+        long long x = u0 - (long long)kvh * per_head;
+#pragma unroll 1
+        for (; x < 0; x += per_head) kvh--;
+#pragma unroll 1
+        for (; x >= per_head; x -= per_head) kvh++;
         if (x >= before && x < before + units) {  // one thread: its run holds the first unit
-            int i = find(starts, n, g0), g = g0;
-            Seq s = load_seq(a, i);
-            x -= before;
-            for (;;) {
-                while (starts[i + 1] <= g) s = load_seq(a, ++i);
+            int i = first, g = g0, skip = (int)x - before;
+#pragma unroll 1
+            for (;; g++) {
+#pragma unroll 1
+                while (plan.starts[i + 1] <= g) i++;
                 Tile t;
-                tile_range<kRows, kBlock>(a, s, (g - starts[i]) * kRows, t);
-                if (x < t.nb) break;
-                x -= t.nb;
-                g++;
+                tile_range<kRows, kBlock>(a, plan.seqs[i], (g - plan.starts[i]) * kRows, t);
+                if (skip < t.nb) break;
+                skip -= t.nb;
             }
+            share->split = sp;
             share->tile = g;
             share->kvh = kvh;
-            share->skip = (int)x;
-            share->left = u1 - u0;
+            share->skip = skip;
+            share->left = sp.start(c + 1) - u0;
             share->n_tiles = n_tiles;
-            share->ctas = ctas;
-            share->units = total;
         }
     }
     __syncthreads();
@@ -223,42 +280,43 @@ __device__ void find_share(const PagedAttnArgs& a, int* starts, Share* share) {
 // Goes through a share segment by segment: blocks [first, first + n) of tile t.
 template <int kRows, int kBlock>
 struct Walk {
-    Share sh;
-    const int* starts;
-    int seq_hint = 0;
+    const Share& share;
+    const Plan plan;
+    long long left;
+    int tile, kvh, skip, n_tiles, seq = 0;
     Tile t;
     int first, n;     // blocks of this segment
     bool head, whole; // the segment begins its tile; it is the whole tile
 
-    __device__ __forceinline__ Walk(const Share& s, const int* st) : sh(s), starts(st) {}
+    __device__ __forceinline__ Walk(const Share& s, const Plan& p)
+        : share(s), plan(p), left(s.left), tile(s.tile), kvh(s.kvh), skip(s.skip), n_tiles(s.n_tiles) {}
     __device__ __forceinline__ bool next(const PagedAttnArgs& a) {
-        if (sh.left <= 0) return false;
-        if (sh.tile == sh.n_tiles) {
-            sh.tile = 0;
-            sh.kvh++;
+        if (left <= 0) return false;
+        if (tile == n_tiles) {
+            tile = 0;
+            kvh++;
+            seq = 0;
         }
-        const int i = starts[seq_hint] <= sh.tile && sh.tile < starts[seq_hint + 1] ? seq_hint
-                                                                                  : find(starts, a.n_seq, sh.tile);
-        seq_hint = i;
-        t.seq = i;
-        t.kvh = sh.kvh;
-        tile_range<kRows, kBlock>(a, load_seq(a, i), (sh.tile - starts[i]) * kRows, t);
-        first = t.b0 + sh.skip;
-        head = sh.skip == 0;
-        n = (int)min((long long)(t.nb - sh.skip), sh.left);
+        if (!(plan.starts[seq] <= tile && tile < plan.starts[seq + 1])) seq = find(plan.starts, a.n_seq, tile);
+        t.seq = seq;
+        t.kvh = kvh;
+        tile_range<kRows, kBlock>(a, plan.seqs[seq], (tile - plan.starts[seq]) * kRows, t);
+        first = t.b0 + skip;
+        head = skip == 0;
+        n = (int)min((long long)(t.nb - skip), left);
         whole = head && n == t.nb;
-        sh.left -= n;
-        sh.skip = 0;
-        sh.tile++;
+        left -= n;
+        skip = 0;
+        tile++;
         return true;
     }
     // The CTAs that share the tile of the present segment (a segment that is not the whole tile).
     __device__ __forceinline__ void sharers(int* c0, int* c1) const {
-        const long long share0 = sh.units * blockIdx.x / sh.ctas, share1 = sh.units * (blockIdx.x + 1) / sh.ctas;
+        const Split sp = share.split;
         // a segment that does not begin its tile is the share's first; one that does, but does not end it, its last
-        const long long u0 = head ? share1 - n : share0 - (first - t.b0), u1 = u0 + t.nb - 1;
-        *c0 = (int)(((u0 + 1) * sh.ctas - 1) / sh.units);
-        *c1 = (int)(((u1 + 1) * sh.ctas - 1) / sh.units);
+        const long long u0 = head ? sp.start(blockIdx.x + 1) - n : sp.start(blockIdx.x) - (first - t.b0);
+        *c0 = head ? blockIdx.x : sp.holder(u0);
+        *c1 = sp.holder(u0 + t.nb - 1);
     }
 };
 

@@ -187,7 +187,7 @@ struct Row {
 __device__ __forceinline__ int tile_steps(const PagedAttnArgs& a, const Tile& t, int i, int first, int n, int& rows) {
     rows = min(kTcTile, t.rows - i * kTcTile);
     if (rows <= 0) return 0;
-    const int hi = a.causal ? min(t.hi, t.off + (t.r0 + i * kTcTile + rows - 1) / a.group + 1) : t.hi;
+    const int hi = a.causal ? min(t.hi, t.off + t.token(a, i * kTcTile + rows - 1) + 1) : t.hi;
     return max(0, min(n * (kTcBlock / kTcStep), (hi - first * kTcBlock + kTcStep - 1) / kTcStep));
 }
 
@@ -257,8 +257,10 @@ struct Issuer {
         steps = tile_steps(a, w.t, I, w.first, w.n, rows);
         k_seen = v_seen = 0;
         if (steps && !wait.one(&bars.q_full[I], n_q++ & 1)) return false;
+#pragma unroll 1
         for (int s = 0; s < min(2, steps); s++)  // (the buffers are free: all products of the segment before were waited for)
             if (!scores(s)) return false;
+#pragma unroll 1
         for (int s = 0; s < steps; s++) {
             if (!product(s)) return false;
             // the scores after next take the place of the weights that this product reads
@@ -267,6 +269,7 @@ struct Issuer {
         }
         // Blocks that this tile has no step in are freed in turn, too: each when it has come, so that
         // an arrival never counts for the block that was in the stage before.
+#pragma unroll 1
         for (int b = (steps + 1) / 2; b < w.n; b++) {
             if (!need(b, k_seen, bars.k_full)) return false;
             mbar_arrive(&bars.k_empty[stage(b)]);
@@ -283,19 +286,21 @@ struct Issuer {
             if (!segment(w)) break;
         // every MMA has completed before TMEM is freed
         mma_commit(&bars.drain);
+        wait.report(a.status);
         wait.ok = true;
         wait(&bars.drain, 0);
+        wait.report(a.status);
     }
 };
 
 template <int HD>
 __global__ void __launch_bounds__(kTcThreads, 1)
     paged_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                    const PagedAttnArgs a) {
+                    const __grid_constant__ PagedAttnArgs a) {
     using C = TcCfg<HD>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    int* starts = reinterpret_cast<int*>(smem + C::oEnd);
+    const Plan plan(a, smem + C::oEnd);
     __shared__ TcBars bars;
     __shared__ Share share;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -326,12 +331,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tmem_relinquish();
     }
     tc_fence_before();
-    find_share<kTcThreads, kTcRows, kTcBlock, 1>(a, starts, &share);
+    find_share<kTcThreads, kTcRows, kTcBlock, 1>(a, plan, &share);
     tc_fence_after();
     const uint32_t tmem = bars.tmem;
-    Walk<kTcRows, kTcBlock> w(share, starts);
+    Walk<kTcRows, kTcBlock> w(share, plan);
     Waiter wait;
-    wait.status = a.status;
 
     if (warp == 10) {
         // ------------------------------------------------ copies
@@ -339,6 +343,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         uint32_t j = 0, n_tail = 0;
         while (w.next(a)) {
             const int32_t* table = a.table + (size_t)w.t.seq * a.table_stride;
+#pragma unroll 1
             for (int b = w.first; b < w.first + w.n; b++, j++) {
                 const uint32_t st = j % C::kStages, par = (j / C::kStages - 1) & 1;
                 const int p0 = b * kTcBlock, left = min(kTcBlock, w.t.hi - p0);
@@ -377,6 +382,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     // what lies behind the last position is not a number, perhaps, which a weight of 0 would not hide
                     const bool got = wait.warp(&bars.v_tail, n_tail++ & 1);
                     const int r0 = max(0, w.t.hi - p0);
+#pragma unroll 1
                     for (int e = lane; e < (kTcBlock - r0) * (HD / 8); e += 32) {
                         const int r = r0 + e / (HD / 8), c = e % (HD / 8);
                         *reinterpret_cast<uint4*>(smem + C::oV + st * C::kTileBytes + (c >> 3) * C::kHalf + sw128(r, c & 7)) =
@@ -394,7 +400,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (!wait.ok) break;
         }
         // every copy has landed before the CTA may exit
+        wait.report(a.status);
         wait.ok = true;
+#pragma unroll 1
         for (uint32_t i = j > C::kStages ? j - C::kStages : 0; i < j; i++) {
             wait(&bars.k_full[i % C::kStages], (i / C::kStages) & 1);
             wait(&bars.v_full[i % C::kStages], (i / C::kStages) & 1);
@@ -426,7 +434,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const int row = i * kTcTile + r;  // in the unit
             if (t.rows <= i * kTcTile) continue;
             const bool live = row < t.rows;
-            const int tok = (t.r0 + row) / a.group, head = t.kvh * a.group + (t.r0 + row) - tok * a.group;
+            const int tok = t.token(a, row), head = t.head(a, row);
             const int pos = t.off + tok;
             const int to = !live ? 0 : a.causal ? min(t.s.len, pos + 1) : t.s.len;
             const int from = a.window ? max(0, pos - a.window + 1) : 0;
@@ -450,6 +458,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 mbar_arrive(&bars.q_full[i]);
             }
             Row row_state(k2);
+#pragma unroll 1
             for (int n = 0; n < steps; n++, ns++) {
                 const int p0 = w.first * kTcBlock + n * kTcStep;
                 const uint32_t buf = tS + (ns & 1) * 64;
@@ -550,14 +559,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 template <int HD>
 cudaError_t tc_init() {
     return cudaFuncSetAttribute(paged_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                TcCfg<HD>::kSmem + (kPagedMaxSeq + 1) * 4);
+                                TcCfg<HD>::kSmem + Plan::bytes(kPagedMaxSeq));
 }
 
 template <int HD>
 cudaError_t tc_case(const PagedMaps& maps, const PagedAttnArgs& a, int ctas, cudaStream_t s) {
     using C = TcCfg<HD>;
-    static_assert(C::kSmem + (kPagedMaxSeq + 1) * 4 + 1024 <= 232448, "shared memory per CTA");
-    paged_tc_kernel<HD><<<ctas, kTcThreads, C::kSmem + (a.n_seq + 1) * 4, s>>>(maps.k_tc, maps.v_tc, a);
+    static_assert(C::kSmem + Plan::bytes(kPagedMaxSeq) + 1024 <= 232448, "shared memory per CTA");
+    paged_tc_kernel<HD><<<ctas, kTcThreads, C::kSmem + Plan::bytes(a.n_seq), s>>>(maps.k_tc, maps.v_tc, a);
     return cudaGetLastError();
 }
 
