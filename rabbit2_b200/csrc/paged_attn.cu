@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
         float M = -INFINITY, L = 0.0f, o[DL];
 #pragma unroll
         for (int d = 0; d < DL; d++) o[d] = 0.0f;
-#pragma unroll 1
+#pragma unroll 4
         for (int c = c0; c <= j.last; c++) {
             const float* p = a.part + ((size_t)c * 2 + (c == c0)) * part_floats;
             const float m = p[r], l = p[tile_rows + r];

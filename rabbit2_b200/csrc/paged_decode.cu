@@ -148,7 +148,7 @@ __device__ __forceinline__ void put_row(const PagedAttnArgs& a, const Tile& t, i
 // comes last adds up all parts, in CTA order, so the order of arrival changes nothing.
 // The tile's counter is that of its first CTA; the last to arrive leaves it at 0.
 template <typename T, int kRows, int HD, typename W>
-__device__ __forceinline__ void finish(const PagedAttnArgs& a, const W& w, const Parts<kRows, HD>* s, int set, int* last) {
+__device__ __forceinline__ void finish(const PagedAttnArgs& a, const W& w, Parts<kRows, HD>* s, int set, int* last) {
     constexpr int kThreads = 32 * kDecWarps, kFloats = paged_part_floats(kRows, HD), kO = paged_part_o(kRows);
     const Tile& t = w.t;
     float* part = a.part + ((size_t)blockIdx.x * 2 + (w.head ? 1 : 0)) * kFloats;
@@ -195,26 +195,64 @@ __device__ __forceinline__ void finish(const PagedAttnArgs& a, const W& w, const
     named_sync(1, kThreads);
     if (!*last) return;
     __threadfence();
+    // The rows' maxima and sums over the parts (a warp per row, a lane per part), then the outputs, a
+    // quarter of the parts per warp.  Short loops: this runs once a tile, from a cold instruction cache.
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = c1 - c0 + 1;
+    const float* first = a.part + ((size_t)c0 * 2 + 1) * kFloats;  // slot 1 of the first CTA, slot 0 of the others
+    const auto at = [&](int i) { return i ? a.part + (size_t)(c0 + i) * 2 * kFloats : first; };
+#pragma unroll 1
+    for (int r = warp; r < t.rows; r += kDecWarps) {
+        float M = -INFINITY, L = 0.0f;
+#pragma unroll 1
+        for (int i = lane; i < n; i += 32) {
+            const float m = __ldcg(at(i) + r), l = __ldcg(at(i) + kRows + r);
+            const float mn = fmaxf(M, m), base = mn == -INFINITY ? 0.0f : mn;
+            L = L * ex2(M - base) + l * ex2(m - base);
+            M = mn;
+        }
+#pragma unroll 1
+        for (int o = 16; o > 0; o >>= 1) {
+            const float m = __shfl_xor_sync(FULL_MASK, M, o), l = __shfl_xor_sync(FULL_MASK, L, o);
+            const float mn = fmaxf(M, m), base = mn == -INFINITY ? 0.0f : mn;
+            L = L * ex2(M - base) + l * ex2(m - base);
+            M = mn;
+        }
+        if (lane == 0) {
+            s->m[set][0][r] = M;
+            s->l[set][0][r] = L;
+        }
+    }
+    named_sync(1, kThreads);
+#pragma unroll 1
+    for (int e = lane; e < t.rows * (HD / 4); e += 32) {
+        const int r = e / (HD / 4), c = 4 * (e - r * (HD / 4));
+        const float M = s->m[set][0][r], base = M == -INFINITY ? 0.0f : M;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int i = warp; i < n; i += kDecWarps) {
+            const float y = ex2(__ldcg(at(i) + r) - base);
+            const float4 f = __ldcg(reinterpret_cast<const float4*>(at(i) + kO + (size_t)r * HD + c));
+            o.x = fmaf(f.x, y, o.x);
+            o.y = fmaf(f.y, y, o.y);
+            o.z = fmaf(f.z, y, o.z);
+            o.w = fmaf(f.w, y, o.w);
+        }
+        *reinterpret_cast<float4*>(&s->o[warp][r][c]) = o;
+    }
+    named_sync(1, kThreads);
 #pragma unroll 1
     for (int e = threadIdx.x; e < t.rows * (HD / 4); e += kThreads) {
         const int r = e / (HD / 4), c = 4 * (e - r * (HD / 4));
-        const float* p = a.part + ((size_t)c0 * 2 + 1) * kFloats;  // slot 1 of the first CTA, slot 0 of the others
-        float M = -INFINITY, L = 0.0f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-        for (int i = c0; i <= c1; i++, p = a.part + (size_t)i * 2 * kFloats) {
-            const float m = __ldcg(p + r), l = __ldcg(p + kRows + r);
-            const float4 f = __ldcg(reinterpret_cast<const float4*>(p + kO + (size_t)r * HD + c));
-            const float mn = fmaxf(M, m), base = mn == -INFINITY ? 0.0f : mn;
-            const float x = ex2(M - base), y = ex2(m - base);
-            L = L * x + l * y;
-            o.x = o.x * x + f.x * y;
-            o.y = o.y * x + f.y * y;
-            o.z = o.z * x + f.z * y;
-            o.w = o.w * x + f.w * y;
-            M = mn;
+#pragma unroll
+        for (int i = 0; i < kDecWarps; i++) {
+            const float4 f = *reinterpret_cast<const float4*>(&s->o[i][r][c]);
+            o.x += f.x;
+            o.y += f.y;
+            o.z += f.z;
+            o.w += f.w;
         }
-        put_row<T, HD>(a, t, r, c, o, M, L);
+        put_row<T, HD>(a, t, r, c, o, s->m[set][0][r], s->l[set][0][r]);
     }
 }
 
@@ -246,7 +284,8 @@ struct DecBf16 {
     static constexpr int kBlock = kDecStage / (4 * HD);  // positions of a stage: 32 (head_dim 128) or 64
     static constexpr int kHalf = kDecStage / 2;          // bytes of k
     static constexpr int kStages = DecShape<false>::kStages, kCtas = DecShape<false>::kCtas;
-    static constexpr int kSmem = kStages * kDecStage + (int)sizeof(Parts<kRows, HD>) + 1024;
+    static constexpr int kQBytes = kRows * HD * 2;
+    static constexpr int kSmem = kStages * kDecStage + (int)sizeof(Parts<kRows, HD>) + 2 * kQBytes + 1024;
 };
 
 template <int HD>
@@ -258,7 +297,8 @@ __global__ void __launch_bounds__(kDecThreads, DecBf16<HD>::kCtas)
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     Parts<C::kRows, HD>* parts = reinterpret_cast<Parts<C::kRows, HD>*>(smem + C::kStages * kDecStage);
-    const Plan plan(a, parts + 1);
+    uint8_t* q_buf = reinterpret_cast<uint8_t*>(parts + 1);
+    const Plan plan(a, q_buf + 2 * C::kQBytes);
     __shared__ Ring<C::kStages> ring;
     __shared__ Share share;
     __shared__ int last;
@@ -299,23 +339,23 @@ __global__ void __launch_bounds__(kDecThreads, DecBf16<HD>::kCtas)
 #pragma unroll 1
     for (int set = 0; w.next(a); set ^= 1) {
         const Tile& t = w.t;
-        // q as A fragments (rows g and g + 8), through shared memory: each warp its own copy, 16-byte
-        // chunk c of row r at chunk c ^ (r & 7) of the row
+        // q as A fragments (rows g and g + 8), through shared memory: 16-byte chunk c of row r at chunk
+        // c ^ (r & 7) of the row; two buffers, as a warp may still read the tile's before
         uint32_t q[KS][4];
-        uint8_t* qw = reinterpret_cast<uint8_t*>(&parts->o[warp][0][0]);  // (free between two segments' sums)
+        uint8_t* qs = q_buf + set * C::kQBytes;
 #pragma unroll 1
-        for (int e = lane; e < C::kRows * (HD / 8); e += 32) {
+        for (int e = threadIdx.x; e < C::kRows * (HD / 8); e += 32 * kDecWarps) {
             const int r = e / (HD / 8), c = e - r * (HD / 8);
             uint4 x = make_uint4(0, 0, 0, 0);
             if (r < t.rows)
                 x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
                                                     (t.s.row0 + t.token(a, r)) * a.q_stride + (size_t)t.head(a, r) * HD + 8 * c);
-            *reinterpret_cast<uint4*>(qw + r * (HD * 2) + ((c ^ (r & 7)) << 4)) = x;
+            *reinterpret_cast<uint4*>(qs + r * (HD * 2) + ((c ^ (r & 7)) << 4)) = x;
         }
-        __syncwarp();
+        named_sync(1, 32 * kDecWarps);
 #pragma unroll
         for (int k = 0; k < KS; k++)
-            ldsm4(smem_u32(qw) + (lane & 15) * (HD * 2) + (((2 * k + (lane >> 4)) ^ (lane & 7)) << 4), q[k]);
+            ldsm4(smem_u32(qs) + (lane & 15) * (HD * 2) + (((2 * k + (lane >> 4)) ^ (lane & 7)) << 4), q[k]);
         int to[2], from[2];
 #pragma unroll
         for (int i = 0; i < 2; i++) {
