@@ -191,10 +191,10 @@ __device__ __forceinline__ int tile_steps(const PagedAttnArgs& a, const Tile& t,
     return max(0, min(n * (kTcBlock / kTcStep), (hi - first * kTcBlock + kTcStep - 1) / kTcStep));
 }
 
-// The thread that issues tile I's MMAs.  One thread per tile: an issue waits until the
+// The thread that issues a tile's MMAs.  One thread per tile: an issue waits until the
 // tensor cores have room, and the waits and commits between two groups of MMAs of one tile
 // leave room for the other's.
-template <int HD, int I>
+template <int HD>
 struct Issuer {
     using C = TcCfg<HD>;
     static constexpr uint32_t kIdS = idesc_bf16_f32(kTcTile, kTcStep);
@@ -203,13 +203,14 @@ struct Issuer {
     const PagedAttnArgs& a;
     TcBars& bars;
     Waiter& wait;
-    uint32_t tmem, q, k, v;              // descriptors' lower halves (stage 0 of k and v)
+    const int tile;
+    uint32_t tS, tO, q, k, v;            // TMEM columns; descriptors' lower halves (stage 0 of k and v)
     uint32_t j0 = 0, n_q = 0, n_s = 0;   // blocks, phases of q_full and steps before this segment
     int steps, k_seen, v_seen;           // of this segment; blocks whose copies have been waited for
 
-    __device__ __forceinline__ Issuer(const PagedAttnArgs& a, TcBars& bars, uint8_t* smem, uint32_t tmem, Waiter& wait)
-        : a(a), bars(bars), wait(wait), tmem(tmem) {
-        q = (uint32_t)sw128_kmajor_desc(smem_u32(smem + C::oQ + I * C::kTileBytes));
+    __device__ __forceinline__ Issuer(const PagedAttnArgs& a, TcBars& bars, uint8_t* smem, uint32_t tmem, Waiter& wait, int tile)
+        : a(a), bars(bars), wait(wait), tile(tile), tS(tmem + C::cS + tile * 128), tO(tmem + C::cO + tile * 128) {
+        q = (uint32_t)sw128_kmajor_desc(smem_u32(smem + C::oQ + tile * C::kTileBytes));
         k = (uint32_t)sw128_kmajor_desc(smem_u32(smem + C::oK));
         v = (uint32_t)mn_desc(smem_u32(smem + C::oV), C::kHalf);
     }
@@ -225,7 +226,7 @@ struct Issuer {
     // Scores of step s into its buffer (steps so far) & 1.
     __device__ __forceinline__ bool scores(int s) {
         if (!need(s >> 1, k_seen, bars.k_full)) return false;
-        const uint32_t u = n_s + s, d = tmem + C::cS + I * 128 + (u & 1) * 64;
+        const uint32_t u = n_s + s, d = tS + (u & 1) * 64;
         const uint32_t kb = k + ((stage(s >> 1) * C::kTileBytes + (s & 1) * kHalfStep) >> 4);
         tc_fence_after();
 #pragma unroll
@@ -233,39 +234,36 @@ struct Issuer {
             const uint32_t o = ((kk >> 2) * C::kHalf + (kk & 3) * 32) >> 4;
             mma_bf16(d, desc(q + o), desc(kb + o), kIdS, kk != 0);
         }
-        mma_commit(&bars.s_full[I][u & 1]);
+        mma_commit(&bars.s_full[tile][u & 1]);
         if ((s & 1) || s + 1 == steps) mma_commit(&bars.k_empty[stage(s >> 1)]);
         return true;
     }
     // O += P v of step s.
     __device__ __forceinline__ bool product(int s) {
         if (!need(s >> 1, v_seen, bars.v_full)) return false;
-        const uint32_t u = n_s + s, p = tmem + C::cS + I * 128 + (u & 1) * 64;
+        const uint32_t u = n_s + s, p = tS + (u & 1) * 64;
         const uint32_t vb = v + ((stage(s >> 1) * C::kTileBytes + (s & 1) * kHalfStep) >> 4);
-        if (!wait.one(&bars.p_full[I][u & 1], (u >> 1) & 1)) return false;
+        if (!wait.one(&bars.p_full[tile][u & 1], (u >> 1) & 1)) return false;
         tc_fence_after();
 #pragma unroll
         for (int kk = 0; kk < kTcStep / 16; kk++)
-            mma_bf16_ts(tmem + C::cO + I * 128, p + kk * 8, desc(vb + (kk * 2048 >> 4)), kIdO, (s | kk) != 0);
-        mma_commit(&bars.pv_done[I]);
+            mma_bf16_ts(tO, p + kk * 8, desc(vb + (kk * 2048 >> 4)), kIdO, (s | kk) != 0);
+        mma_commit(&bars.pv_done[tile]);
         if ((s & 1) || s + 1 == steps) mma_commit(&bars.v_empty[stage(s >> 1)]);
         return true;
     }
     template <typename W>
     __device__ __forceinline__ bool segment(const W& w) {
         int rows;
-        steps = tile_steps(a, w.t, I, w.first, w.n, rows);
+        steps = tile_steps(a, w.t, tile, w.first, w.n, rows);
         k_seen = v_seen = 0;
-        if (steps && !wait.one(&bars.q_full[I], n_q++ & 1)) return false;
+        if (steps && !wait.one(&bars.q_full[tile], n_q++ & 1)) return false;
 #pragma unroll 1
-        for (int s = 0; s < min(2, steps); s++)  // (the buffers are free: all products of the segment before were waited for)
-            if (!scores(s)) return false;
-#pragma unroll 1
-        for (int s = 0; s < steps; s++) {
-            if (!product(s)) return false;
-            // the scores after next take the place of the weights that this product reads
-            if (!wait.one(&bars.pv_done[I], (n_s + s) & 1)) return false;
-            if (s + 2 < steps && !scores(s + 2)) return false;
+        for (int s = 0; s < steps + 2; s++) {
+            // The scores take the place of the weights that the product two steps before read.  (For the first
+            // two the buffers are free: all products of the segment before were waited for.)
+            if (s >= 2 && (!product(s - 2) || !wait.one(&bars.pv_done[tile], (n_s + s - 2) & 1))) return false;
+            if (s < steps && !scores(s)) return false;
         }
         // Blocks that this tile has no step in are freed in turn, too: each when it has come, so that
         // an arrival never counts for the block that was in the stage before.
@@ -407,18 +405,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             wait(&bars.k_full[i % C::kStages], (i / C::kStages) & 1);
             wait(&bars.v_full[i % C::kStages], (i / C::kStages) & 1);
         }
-    } else if (warp == 8) {
+    } else if (warp >= 8) {
         // ------------------------------------------------ MMAs: one thread per tile
-        if (lane == 0) {
-            Issuer<HD, 0> mma(a, bars, smem, tmem, wait);
-            mma.run(w);
-        }
-        __syncwarp();
-    } else if (warp == 9) {
-        if (lane == 0) {
-            Issuer<HD, 1> mma(a, bars, smem, tmem, wait);
-            mma.run(w);
-        }
+        if (lane == 0) Issuer<HD>(a, bars, smem, tmem, wait, warp - 8).run(w);
         __syncwarp();
     } else {
         // ------------------------------------------------ softmax: thread = row
@@ -444,7 +433,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
                                                                   (t.s.row0 + tok) * a.q_stride + (size_t)head * HD);
                 uint8_t* dst = smem + C::oQ + i * C::kTileBytes;
-#pragma unroll
+#pragma unroll 4
                 for (int c = 0; c < HD / 8; c++) {
                     uint4 x = live ? src[c] : make_uint4(0, 0, 0, 0);
                     x.x ^= flip;
@@ -513,7 +502,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             uint16_t* out = static_cast<uint16_t*>(a.out) + (t.s.row0 + tok) * a.out_stride + (size_t)head * HD;
             float* po = part + paged_part_o(kTcRows) + (size_t)row * HD;
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
                 uint32_t o[32];
                 __syncwarp();  // the rows of a warp part ways below, and tcgen05.ld is the whole warp's
