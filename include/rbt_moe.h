@@ -476,6 +476,30 @@ typedef struct RbtPagedAttention {
 } RbtPagedAttention;
 int rbt_paged_attention_device(RbtPaged *p, int layer, const RbtPagedAttention *a, void *stream);
 
+/* ---- A model over the paged cache: requests of different lengths, prompts in chunks
+ * beside decoding sequences, in one call per step.  These sequences are the model's
+ * own, apart from those of rbt_model_set_sequences.
+ *
+ * rbt_model_set_pages: caches of n_pages pages of page_size positions for every layer,
+ * in dtype (0 f32: the values the dense cache holds; 1 bf16: half the bytes, k, v, q and
+ * the attention's output rounded to bf16), for max_seqs sequences of up to ctx positions
+ * each, all empty.  n_pages == 0 frees them.  Needs head_dim 64 or 128.
+ *
+ * rbt_model_paged_step: counts[i] >= 0 new tokens for each of the first n sequences,
+ * behind what they hold (tokens: those of sequence 0, then of sequence 1, ...).  Pages
+ * are taken as needed; a step that does not fit fails before anything is changed.
+ * Outputs (host, each may be NULL): logits [n, vocab] and next [n], of each sequence's
+ * last new token (next as rbt_model_decode_batch; sequences without new tokens get -1
+ * and their logits rows are left as they were); routing_out [tokens, n_layers, top_k].
+ * After a step that failed while running the sequences are as before it.
+ *
+ * rbt_model_paged_release: the sequences with done[i] != 0 are emptied, their pages are
+ * free again. */
+int rbt_model_set_pages(RbtModel *m, int n_pages, int page_size, int dtype, int max_seqs);
+int rbt_model_paged_step(RbtModel *m, const int32_t *tokens, const int32_t *counts, int n, float *logits,
+                         int32_t *next, int32_t *routing_out);
+int rbt_model_paged_release(RbtModel *m, const int32_t *done, int n);
+
 /* Last error message of the calling thread ("" if none). */
 const char *rbt_moe_last_error(void);
 

@@ -1103,6 +1103,7 @@ void rbt_model_destroy(RbtModel* m) {
     cudaFreeHost(m->h_status);
     cudaFreeHost(m->h_steps);
     rbt::prefill_free(m);
+    rbt::paged_free(m);
     if (m->stream) cudaStreamDestroy(m->stream);
     rbt_moe_destroy(m->moe);
     delete m;

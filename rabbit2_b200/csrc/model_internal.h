@@ -34,8 +34,33 @@ struct PrefillBufs {
 
 }  // namespace rbt
 
+namespace rbt {
+// The model's paged sequences (rbt_model_set_pages).  Lengths and the free count exist
+// twice on the GPU, so that a step writes the other ones and a failed step is forgotten.
+struct PagedState {
+    RbtPaged* ctx = nullptr;
+    int max_seqs = 0, width = 0, n_pages = 0, page = 0, dtype = 0;
+    void *k = nullptr, *v = nullptr;     // [n_layers][n_pages][n_kv_heads][page][head_dim]
+    int32_t* table = nullptr;            // [max_seqs][width]
+    int32_t* free_list = nullptr;        // [n_pages]
+    int32_t* len[2] = {nullptr, nullptr};
+    int32_t* n_free[2] = {nullptr, nullptr};
+    int now = 0;                         // which of them hold
+    int32_t *counts = nullptr, *cu = nullptr;  // [max_seqs], [max_seqs + 1]
+    int cap = 0;                         // rows of the buffers below
+    int64_t* slot = nullptr;
+    int32_t *pos = nullptr, *last = nullptr;   // last: row of each sequence's last new token
+    void *q = nullptr, *ao = nullptr;    // [cap][nq] of dtype
+    float* rows = nullptr;               // [max_seqs][dim] those rows of the residual
+    int32_t* next = nullptr;             // [max_seqs]
+    std::vector<int> h_len;              // the lengths and the free count as the host knows them
+    int h_free = 0;
+};
+}  // namespace rbt
+
 struct RbtModel;
 namespace rbt {
+void paged_free(RbtModel* m);
 void prefill_free(RbtModel* m);  // model_prefill.cu: the batched prompt's buffers
 cudaError_t launch_attn_decode_rows(const RbtModel* m, int layer, const Step* steps, const float* qkv, int n,
                                     float* ao, float* part, unsigned* done, cudaStream_t s);
@@ -94,6 +119,7 @@ struct RbtModel {
     unsigned* ddone = nullptr;     // [dcap][n_heads] finished splits, zero between calls
     int32_t* dnext = nullptr;      // [dcap] greedy ids
     rbt::Step* h_steps = nullptr;  // [dcap] pinned staging of the steps
+    rbt::PagedState paged;  // model_prefill.cu
     // graphs: [0] without lm_head, [1] with
     cudaGraphExec_t graph[2] = {nullptr, nullptr};
     unsigned long long graph_gen = 0;  // the MoE workspace generation the graphs were captured with

@@ -665,6 +665,163 @@ int run_decode(RbtModel* m, int n, bool want_logits) {
     return 1;
 }
 
+// bf16 attention rows as the f32 rows that the output projection's split takes
+__global__ void __launch_bounds__(kRowThreads) widen_rows_kernel(const uint16_t* in, float* out, int64_t n) {
+    const int64_t i = ((int64_t)blockIdx.x * kRowThreads + threadIdx.x) * 8;
+    if (i >= n) return;
+    float f[8];
+    WeightTraits<uint16_t>::unpack(*reinterpret_cast<const uint4*>(in + i), f);
+    *reinterpret_cast<float4*>(out + i) = make_float4(f[0], f[1], f[2], f[3]);
+    *reinterpret_cast<float4*>(out + i + 4) = make_float4(f[4], f[5], f[6], f[7]);
+}
+
+// row last[i] of x [rows, D] as row i
+__global__ void __launch_bounds__(kRowThreads) pick_rows_kernel(const float* x, int D, const int32_t* last, float* out) {
+    const float4* src = reinterpret_cast<const float4*>(x + (size_t)last[blockIdx.x] * D);
+    float4* dst = reinterpret_cast<float4*>(out + (size_t)blockIdx.x * D);
+    for (int i = threadIdx.x; i < D / 4; i += kRowThreads) dst[i] = src[i];
+}
+
+// A step of the paged sequences: T new tokens, `ends` sequences with any (their last rows in p.last).  As
+// run_prefill, with the rows' k and v written to their slots and the attention over the pages.
+template <typename WT>
+int run_paged(RbtModel* m, int n, int T, int max_new, int ends, bool want_logits) {
+    const RbtModelConfig& c = m->cfg;
+    const int D = c.dim, nq = nq_of(c), nkv = nkv_of(c), nqkv = nq + 2 * nkv, L = c.n_layers, K = c.top_k;
+    const int wide = D > nq ? D : nq;
+    cudaStream_t s = m->stream;
+    PrefillBufs& b = m->pf;
+    PagedState& p = m->paged;
+    embed_rows_kernel<WT><<<T, 256, 0, s>>>(static_cast<const WT*>(m->tok_emb), D, b.tokens, b.x);
+    CU(cudaGetLastError());
+    if (!rbt_paged_plan_device(p.ctx, n, p.len[p.now], p.counts, p.table, p.width, p.free_list, p.n_free[p.now], T,
+                               p.len[p.now ^ 1], p.n_free[p.now ^ 1], p.cu, p.slot, p.pos, (void*)s))
+        return 0;
+    for (int l = 0; l < L; l++) {
+        const RbtModel::Layer& Ly = m->layers[l];
+        if (!split_rows(m, b.x, D, D, T, Ly.attn_norm, wide)) return 0;
+        if (!proj(m, Ly.wqkv, nqkv, D, T, wide, b.qkv, nqkv, false)) return 0;
+        RbtPagedAppend ap{};
+        ap.d_q = b.qkv;
+        ap.d_k = b.qkv + nq;
+        ap.d_v = b.qkv + nq + nkv;
+        ap.q_stride = ap.k_stride = ap.v_stride = nqkv;
+        ap.src_dtype = RBT_MOE_DT_F32;
+        ap.n_rows = T;
+        ap.d_slot = p.slot;
+        ap.d_pos = p.pos;
+        ap.d_q_norm = c.qk_norm ? Ly.q_norm : nullptr;
+        ap.d_k_norm = c.qk_norm ? Ly.k_norm : nullptr;
+        ap.eps = c.rms_eps;
+        ap.rope_len = m->ctx;
+        ap.d_cos = m->rope_cos;
+        ap.d_sin = m->rope_sin;
+        ap.d_q_out = p.q;
+        ap.q_out_stride = nq;
+        if (!rbt_paged_append_device(p.ctx, l, &ap, (void*)s)) return 0;
+        const bool bf = p.dtype == RBT_MOE_DT_BF16;
+        RbtPagedAttention at{};
+        at.d_q = p.q;
+        at.d_out = bf ? p.ao : (void*)b.ao;
+        at.q_stride = at.out_stride = nq;
+        at.n_rows = T;
+        at.n_seq = n;
+        at.max_new = max_new;
+        at.d_cu = p.cu;
+        at.d_len = p.len[p.now ^ 1];
+        at.d_table = p.table;
+        at.table_stride = p.width;
+        at.causal = 1;
+        at.scale = 1.0f / sqrtf((float)c.head_dim);
+        if (!rbt_paged_attention_device(p.ctx, l, &at, (void*)s)) return 0;
+        if (bf) {
+            const int64_t e = (int64_t)T * nq;
+            widen_rows_kernel<<<(unsigned)((e / 8 + kRowThreads - 1) / kRowThreads), kRowThreads, 0, s>>>(
+                static_cast<const uint16_t*>(p.ao), b.ao, e);
+            CU(cudaGetLastError());
+        }
+        if (!split_rows(m, b.ao, nq, nq, T, nullptr, wide)) return 0;
+        if (!proj(m, Ly.wo, D, nq, T, wide, b.x, D, true)) return 0;
+        if (!model_moe_block(m, l, b.x, T, b.routing + (size_t)l * K, L * K, s)) return 0;
+    }
+    if (want_logits) {
+        pick_rows_kernel<<<ends, kRowThreads, 0, s>>>(b.x, D, p.last, p.rows);
+        CU(cudaGetLastError());
+        if (!split_rows(m, p.rows, D, D, ends, m->final_norm, wide)) return 0;
+        if (!proj(m, m->lm_head, c.vocab, D, ends, wide, b.logits, c.vocab, false)) return 0;
+        argmax_rows_kernel<<<ends, kArgmaxThreads, 0, s>>>(b.logits, c.vocab, p.next);
+        CU(cudaGetLastError());
+    }
+    return 1;
+}
+
+// Row buffers of a paged step of T rows.
+int reserve_paged(RbtModel* m, int T) {
+    PagedState& p = m->paged;
+    if (T <= p.cap) return 1;
+    const size_t nq = nq_of(m->cfg), es = p.dtype == RBT_MOE_DT_BF16 ? 2 : 4;
+    void* old[] = {p.slot, p.pos, p.q, p.ao};
+    for (void* x : old) cudaFree(x);
+    p.slot = nullptr;
+    p.pos = nullptr;
+    p.q = p.ao = nullptr;
+    p.cap = 0;
+    CU(cudaMalloc((void**)&p.slot, (size_t)T * 8));
+    CU(cudaMalloc((void**)&p.pos, (size_t)T * 4));
+    CU(cudaMalloc(&p.q, (size_t)T * nq * es));
+    if (p.dtype == RBT_MOE_DT_BF16) CU(cudaMalloc(&p.ao, (size_t)T * nq * 2));
+    p.cap = T;
+    return 1;
+}
+
+int make_pages(RbtModel* m, int n_pages, int page, int dtype, int max_seqs) {
+    const RbtModelConfig& c = m->cfg;
+    PagedState& p = m->paged;
+    p.max_seqs = max_seqs;
+    p.width = (m->ctx + page - 1) / page;
+    p.n_pages = n_pages;
+    p.page = page;
+    p.dtype = dtype;
+    const size_t layer = (size_t)n_pages * page * nkv_of(c) * (dtype == RBT_MOE_DT_BF16 ? 2 : 4);
+    RbtPagedConfig pc{c.n_layers, c.n_heads, c.n_kv_heads, c.head_dim, page, n_pages, dtype};
+    if (!rbt_paged_create(&p.ctx, &pc, m->device)) return 0;
+    CU(cudaMalloc(&p.k, layer * c.n_layers));
+    CU(cudaMalloc(&p.v, layer * c.n_layers));
+    for (int l = 0; l < c.n_layers; l++)
+        if (!rbt_paged_bind_layer(p.ctx, l, static_cast<uint8_t*>(p.k) + l * layer, static_cast<uint8_t*>(p.v) + l * layer))
+            return 0;
+    const size_t n4 = (size_t)max_seqs * 4;
+    CU(cudaMalloc((void**)&p.table, n4 * p.width));
+    CU(cudaMalloc((void**)&p.free_list, (size_t)n_pages * 4));
+    for (int i = 0; i < 2; i++) {
+        CU(cudaMalloc((void**)&p.len[i], n4));
+        CU(cudaMalloc((void**)&p.n_free[i], 4));
+    }
+    CU(cudaMalloc((void**)&p.counts, n4));
+    CU(cudaMalloc((void**)&p.cu, n4 + 4));
+    CU(cudaMalloc((void**)&p.last, n4));
+    CU(cudaMalloc((void**)&p.next, n4));
+    CU(cudaMalloc((void**)&p.rows, (size_t)max_seqs * c.dim * 4));
+    std::vector<int32_t> ids(n_pages);
+    for (int i = 0; i < n_pages; i++) ids[i] = n_pages - 1 - i;  // page 0 is taken first
+    CU(cudaMemcpy(p.free_list, ids.data(), (size_t)n_pages * 4, cudaMemcpyHostToDevice));
+    CU(cudaMemcpy(p.n_free[0], &n_pages, 4, cudaMemcpyHostToDevice));
+    CU(cudaMemset(p.len[0], 0, n4));
+    CU(cudaMemset(p.table, 0, n4 * p.width));
+    CU(cudaStreamSynchronize(0));
+    p.h_len.assign(max_seqs, 0);
+    p.h_free = n_pages;
+    return 1;
+}
+
+int check_paged(RbtModel* m, int n) {
+    if (!m) return fail("null model");
+    if (!m->paged.ctx) return fail("the model has no pages (rbt_model_set_pages)");
+    if (n < 1 || n > m->paged.max_seqs) return fail("n %d outside [1, %d] (the sequences of rbt_model_set_pages)", n,
+                                                   m->paged.max_seqs);
+    return 1;
+}
+
 // the checks every whole-prompt or batched call makes before it runs
 int check_ready(RbtModel* m) {
     const RbtModelConfig& c = m->cfg;
@@ -686,7 +843,137 @@ void prefill_free(RbtModel* m) {
     m->proj_part = nullptr;
     m->proj_part_bytes = 0;
 }
+
+void paged_free(RbtModel* m) {
+    PagedState& p = m->paged;
+    rbt_paged_destroy(p.ctx);
+    void* bufs[] = {p.k, p.v, p.table, p.free_list, p.len[0], p.len[1], p.n_free[0], p.n_free[1], p.counts, p.cu, p.slot,
+                    p.pos, p.last, p.q, p.ao, p.rows, p.next};
+    for (void* x : bufs) cudaFree(x);
+    p = PagedState{};
+}
 }  // namespace rbt
+
+extern "C" int rbt_model_set_pages(RbtModel* m, int n_pages, int page_size, int dtype, int max_seqs) {
+    if (!m) return fail("null model");
+    if (n_pages < 0) return fail("n_pages must be >= 0 (got %d)", n_pages);
+    if (n_pages && (max_seqs < 1 || max_seqs > RBT_PAGED_MAX_SEQ))
+        return fail("max_seqs %d outside [1, %d]", max_seqs, RBT_PAGED_MAX_SEQ);
+    CU(cudaSetDevice(m->device));
+    CU(cudaStreamSynchronize(m->stream));
+    paged_free(m);
+    if (n_pages == 0) return 1;
+    int ok = 0;
+    try {
+        ok = make_pages(m, n_pages, page_size, dtype, max_seqs);
+    } catch (...) {
+        fail("out of host memory");
+    }
+    if (!ok) paged_free(m);
+    return ok;
+}
+
+extern "C" int rbt_model_paged_release(RbtModel* m, const int32_t* done, int n) {
+    if (!check_paged(m, n)) return 0;
+    if (!done) return fail("null done flags");
+    CU(cudaSetDevice(m->device));
+    PagedState& p = m->paged;
+    cudaStream_t s = m->stream;
+    const size_t n4 = (size_t)n * 4;
+    CU(cudaMemcpyAsync(p.counts, done, n4, cudaMemcpyHostToDevice, s));
+    CU(cudaMemcpyAsync(p.len[p.now ^ 1], p.len[p.now], (size_t)p.max_seqs * 4, cudaMemcpyDeviceToDevice, s));
+    if (!rbt_paged_release_device(p.ctx, n, p.len[p.now], p.counts, p.table, p.width, p.free_list, p.n_pages,
+                                  p.n_free[p.now], p.len[p.now ^ 1], p.n_free[p.now ^ 1], (void*)s))
+        return 0;
+    unsigned st = 0;
+    CU(cudaStreamSynchronize(s));
+    if (!rbt_paged_status(p.ctx, &st)) return 0;
+    if (st) return fail("release: code 0x%x", st);
+    p.now ^= 1;
+    for (int i = 0; i < n; i++)
+        if (done[i]) {
+            p.h_free += (p.h_len[i] + p.page - 1) / p.page;
+            p.h_len[i] = 0;
+        }
+    return 1;
+}
+
+extern "C" int rbt_model_paged_step(RbtModel* m, const int32_t* tokens, const int32_t* counts, int n, float* logits,
+                                    int32_t* next, int32_t* routing_out) {
+    if (!check_paged(m, n)) return 0;
+    if (!tokens || !counts) return fail("null tokens or counts");
+    const RbtModelConfig& c = m->cfg;
+    PagedState& p = m->paged;
+    int64_t total = 0, need = 0;
+    int max_new = 0, ends = 0;
+    for (int i = 0; i < n; i++) {
+        if (counts[i] < 0) return fail("sequence %d: %d new tokens", i, counts[i]);
+        if ((int64_t)p.h_len[i] + counts[i] > m->ctx)
+            return fail("sequence %d: positions %d..%lld outside the cache of %d", i, p.h_len[i],
+                        (long long)p.h_len[i] + counts[i] - 1, m->ctx);
+        need += (p.h_len[i] + counts[i] + p.page - 1) / p.page - (p.h_len[i] + p.page - 1) / p.page;
+        total += counts[i];
+        max_new = counts[i] > max_new ? counts[i] : max_new;
+        ends += counts[i] > 0;
+    }
+    if (total < 1) return fail("no tokens");
+    if (total > (1 << 24)) return fail("%lld tokens in one step: at most %d", (long long)total, 1 << 24);
+    if (need > p.h_free) return fail("%lld pages needed, %d are free", (long long)need, p.h_free);
+    const int T = (int)total;
+    for (int t = 0; t < T; t++)
+        if (tokens[t] < 0 || tokens[t] >= c.vocab) return fail("token %d out of range", tokens[t]);
+    if (!check_ready(m) || !model_moe_fits(m, T)) return 0;
+    CU(cudaSetDevice(m->device));
+    const bool want = logits || next;
+    std::vector<int32_t> last, ids, starts;
+    try {
+        for (int i = 0, at = 0; i < n; at += counts[i++])
+            if (counts[i] > 0) last.push_back(at + counts[i] - 1);
+        ids.resize(ends);
+    } catch (...) {
+        return fail("out of host memory");
+    }
+    if (!reserve(m, T, 0, want ? ends : 0) || !reserve_paged(m, T)) return 0;
+    cudaStream_t s = m->stream;
+    CU(cudaMemcpyAsync(m->pf.tokens, tokens, (size_t)T * 4, cudaMemcpyHostToDevice, s));
+    CU(cudaMemcpyAsync(p.counts, counts, (size_t)n * 4, cudaMemcpyHostToDevice, s));
+    CU(cudaMemcpyAsync(p.last, last.data(), (size_t)ends * 4, cudaMemcpyHostToDevice, s));
+    // the sequences behind the n of this step keep their lengths
+    CU(cudaMemcpyAsync(p.len[p.now ^ 1], p.len[p.now], (size_t)p.max_seqs * 4, cudaMemcpyDeviceToDevice, s));
+    const int ok = c.dtype == RBT_MOE_DT_BF16 ? run_paged<uint16_t>(m, n, T, max_new, ends, want)
+                                              : run_paged<float>(m, n, T, max_new, ends, want);
+    if (!ok) {
+        cudaStreamSynchronize(s);
+        return 0;
+    }
+    if (logits)
+        for (int i = 0, e = 0; i < n; i++)
+            if (counts[i] > 0)
+                CU(cudaMemcpyAsync(logits + (size_t)i * c.vocab, m->pf.logits + (size_t)e++ * c.vocab, (size_t)c.vocab * 4,
+                                   cudaMemcpyDeviceToHost, s));
+    if (next) CU(cudaMemcpyAsync(ids.data(), p.next, (size_t)ends * 4, cudaMemcpyDeviceToHost, s));
+    if (routing_out)
+        CU(cudaMemcpyAsync(routing_out, m->pf.routing, (size_t)T * c.n_layers * c.top_k * 4, cudaMemcpyDeviceToHost, s));
+    CU(cudaMemcpyAsync(m->h_status, m->status, sizeof(unsigned), cudaMemcpyDeviceToHost, s));
+    CU(cudaStreamSynchronize(s));
+    if (*m->h_status) {
+        const unsigned st = *m->h_status;
+        *m->h_status = 0;
+        CU(cudaMemset(m->status, 0, sizeof(unsigned)));
+        return fail("a bounded wait in the projection kernels ran out (code 0x%x)", st);
+    }
+    unsigned st = 0;
+    if (!rbt_paged_status(p.ctx, &st)) return 0;
+    if (st) return fail("the paged cache reports code 0x%x", st);
+    if (!moe_status_ok(m->moe)) return 0;
+    p.now ^= 1;
+    p.h_free -= (int)need;
+    for (int i = 0, e = 0; i < n; i++) {
+        p.h_len[i] += counts[i];
+        if (next) next[i] = counts[i] > 0 ? ids[e++] : -1;
+    }
+    return 1;
+}
 
 extern "C" int rbt_model_prefill(RbtModel* m, const int32_t* tokens, int n_tokens, int pos0, float* logits,
                                  int logit_rows, int32_t* routing_out) {

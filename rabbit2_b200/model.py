@@ -7,7 +7,9 @@ the offsets the engine's loader computes (rbt2fmt.layout, rabbit2.c:166-193);
 ``forward(token, pos)`` is forward(): the logits [vocab] and the routing rows
 [n_layers, top_k] of the token at position pos.  Several sequences:
 ``set_sequences(n)``, ``prefill(tokens, seq=i)`` and ``decode_batch(tokens, pos)``
-(one token of each of the first len(tokens) sequences per call).  Expert
+(one token of each of the first len(tokens) sequences per call).  Over a paged cache:
+``set_pages``, ``paged_step`` (chunks of prompts beside single tokens) and
+``paged_release``.  Expert
 parallelism: ``from_file(..., ep=(rank, n_ranks, max_tokens))`` loads this rank's
 experts only; ``moe()`` is the model's MoE context for the ep_* calls.
 """
@@ -18,6 +20,7 @@ import ctypes as C
 import numpy as np
 
 from rabbit2_b200 import moe
+from rabbit2_b200.moe import DT_BF16
 from rabbit2_b200.rbt2fmt import ModelConfig, layout, unpack_header
 
 
@@ -136,6 +139,29 @@ class ModelContext:
         self._call(self.lib.rbt_model_decode_batch, self.handle, toks.ctypes.data, ps.ctypes.data, n,
                    lg.ctypes.data if logits else None, nxt.ctypes.data, rt.ctypes.data if routing else None)
         return nxt, lg, rt
+
+    def set_pages(self, n_pages: int, page_size: int = 64, dtype: int = DT_BF16, max_seqs: int = 64):
+        """A paged KV cache for max_seqs sequences, all empty (rbt_model_set_pages)."""
+        self._call(self.lib.rbt_model_set_pages, self.handle, int(n_pages), int(page_size), int(dtype), int(max_seqs))
+
+    def paged_step(self, new, logits: bool = True, routing: bool = True):
+        """New tokens for the paged sequences: new[i] is the list of sequence i's (empty: none).
+        (greedy id after each sequence's last token [n] int32, -1 for sequences without new
+        tokens; logits [n, vocab] f32 or None; routing [tokens, n_layers, top_k] or None)."""
+        c, n = self.cfg, len(new)
+        counts = np.array([len(t) for t in new], np.int32)
+        toks = np.ascontiguousarray(np.concatenate([np.asarray(t, np.int32) for t in new]) if n else [], dtype=np.int32)
+        nxt = np.empty(n, np.int32)
+        lg = np.zeros((n, c.vocab), np.float32) if logits else None
+        rt = np.empty((len(toks), c.n_layers, c.top_k), np.int32) if routing else None
+        self._call(self.lib.rbt_model_paged_step, self.handle, toks.ctypes.data, counts.ctypes.data, n,
+                   lg.ctypes.data if logits else None, nxt.ctypes.data, rt.ctypes.data if routing else None)
+        return nxt, lg, rt
+
+    def paged_release(self, done):
+        """Empty the paged sequences with done[i] != 0 (rbt_model_paged_release)."""
+        d = np.ascontiguousarray(done, dtype=np.int32)
+        self._call(self.lib.rbt_model_paged_release, self.handle, d.ctypes.data, len(d))
 
     def close(self):
         if self.handle:

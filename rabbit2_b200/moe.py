@@ -84,6 +84,9 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
         "rbt_model_decode_batch": [vp, vp, vp, i32, vp, vp, vp],
         "rbt_model_set_router_bias": [vp, i32, vp],
         "rbt_moe_router_logits": [vp, vp, i32],
+        "rbt_model_set_pages": [vp, i32, i32, i32, i32],
+        "rbt_model_paged_step": [vp, vp, vp, i32, vp, vp, vp],
+        "rbt_model_paged_release": [vp, vp, i32],
         "rbt_paged_create": [C.POINTER(vp), vp, i32],
         "rbt_paged_bind_layer": [vp, i32, vp, vp],
         "rbt_paged_status": [vp, C.POINTER(C.c_uint)],

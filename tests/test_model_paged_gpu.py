@@ -1,0 +1,129 @@
+"""The model over the paged cache (rbt_model_set_pages / _paged_step / _paged_release): prompts in
+chunks beside decoding sequences, sequences that end and give their pages to others, against the
+same model's prompt call (rbt_model_prefill) on each sequence alone."""
+import dataclasses
+
+import numpy as np
+import pytest
+
+from rabbit2_b200 import moe, workload
+from rabbit2_b200.rbt2fmt import DT_BF16, DT_F32
+
+pytestmark = pytest.mark.gpu
+LOGIT_RTOL = 1e-3  # as the other paths of the model: f32 sums in another order, bf16 rows as hi + lo
+
+CONFIGS = {
+    "f32": {}, "bf16": dict(dtype=DT_BF16),
+    "gqa_bf16": dict(n_kv_heads=2, dtype=DT_BF16), "hd128": dict(n_heads=2, n_kv_heads=1, head_dim=128),
+}
+
+
+def _model(tmp_path, ctx=160, seed=3, **change):
+    from rabbit2_b200.model import ModelContext
+    cfg = dataclasses.replace(workload.tiny_olmoe_config(), **change)
+    path = str(tmp_path / "m.rbt2")
+    workload.write_model(path, cfg, seed=seed)
+    return cfg, ModelContext.from_file(path, ctx=ctx), ModelContext.from_file(path, ctx=ctx)
+
+
+def _serve(cfg, m, steps):
+    """Runs the steps ({sequence: tokens or None to end it}) and returns, per step and sequence,
+    (the sequence's tokens so far, its logits, its greedy id, the routing of its new tokens)."""
+    seen, out = {}, []
+    n = 1 + max(i for s in steps for i in s)
+    for s in steps:
+        ended = [i for i, t in s.items() if t is None]
+        if ended:
+            m.paged_release([int(i in ended) for i in range(n)])
+            for i in ended:
+                seen.pop(i, None)
+        new = [s.get(i) or [] for i in range(n)]
+        if not any(new):
+            continue
+        nxt, lg, rt = m.paged_step(new)
+        at = 0
+        for i, t in enumerate(new):
+            if t:
+                seen[i] = seen.get(i, []) + list(t)
+                out.append((list(seen[i]), lg[i], int(nxt[i]), rt[at:at + len(t)]))
+                at += len(t)
+            else:
+                assert nxt[i] == -1 and not lg[i].any()
+    return out
+
+
+def _steps(cfg, seed):
+    rng = np.random.default_rng(seed)
+    t = lambda n: rng.integers(0, cfg.vocab, size=n).tolist()  # noqa: E731
+    return [{0: t(40), 1: t(33)}, {0: t(1), 2: t(5)}, {0: t(57), 1: t(1), 2: t(1)}, {1: None, 0: t(1), 2: t(70)},
+            {1: t(90), 0: t(1)}, {0: None, 1: None}, {0: t(17), 3: t(2)}, {0: t(1), 1: t(1), 2: t(1), 3: t(1)}]
+
+
+@pytest.mark.parametrize("kind", list(CONFIGS))
+@pytest.mark.parametrize("page", [8, 64])
+def test_paged_steps_match_the_prompt_call(tmp_path, kind, page):
+    cfg, m, ref = _model(tmp_path, **CONFIGS[kind])
+    try:
+        m.set_pages(400 // page + 4, page, DT_F32, max_seqs=4)
+        same = []
+        for toks, lg, nxt, rt in _serve(cfg, m, _steps(cfg, 7)):
+            want, want_r = ref.prefill(toks, 0, logit_rows=1)
+            err = np.abs(lg.astype(np.float64) - want[0]).max() / np.abs(want[0]).max()
+            assert err < LOGIT_RTOL, (kind, len(toks), err)
+            assert nxt == int(np.argmax(lg))
+            same.append(np.all(rt == want_r[len(toks) - len(rt):], axis=(1, 2)))
+        assert np.mean(np.concatenate(same)) >= 0.99  # (near ties of two experts may fall the other way)
+    finally:
+        m.close()
+        ref.close()
+
+
+@pytest.mark.parametrize("dtype", [DT_F32, DT_BF16])
+def test_paged_steps_with_a_bf16_cache(tmp_path, dtype):
+    """q, k, v, the weights and the attention's output are rounded to bf16 (half a step 2^-8 each): a
+    layer's attention moves by some 5 x 2^-8 of itself, the logits of 4 layers by at most 4 x that
+    (to first order, and the MoE halves pass it on).  Every expert is chosen, so that no near tie of the
+    router turns a rounding into another expert."""
+    cfg, m, ref = _model(tmp_path, dtype=dtype, n_experts=2, top_k=2)
+    try:
+        m.set_pages(40, 16, DT_BF16, max_seqs=4)
+        for toks, lg, _, _ in _serve(cfg, m, _steps(cfg, 9)):
+            want, _ = ref.prefill(toks, 0, logit_rows=1)
+            err = np.abs(lg.astype(np.float64) - want[0]).max() / np.abs(want[0]).max()
+            assert err < cfg.n_layers * 5 * 2.0 ** -8, (len(toks), err)
+    finally:
+        m.close()
+        ref.close()
+
+
+def test_paged_steps_refuse_and_leave_the_sequences(tmp_path):
+    cfg, m, ref = _model(tmp_path)
+    try:
+        with pytest.raises(moe.RbtMoeError, match="no pages"):
+            m.paged_step([[1]])
+        with pytest.raises(moe.RbtMoeError, match="page_size"):
+            m.set_pages(10, 12, DT_F32, 2)
+        with pytest.raises(moe.RbtMoeError, match="max_seqs"):
+            m.set_pages(10, 16, DT_F32, 0)
+        m.set_pages(5, 16, DT_F32, 2)
+        a = list(range(1, 31))
+        m.paged_step([a, []])
+        for new, word in (([[], []], "no tokens"), ([[1] * 60, []], "pages needed"), ([[cfg.vocab], []], "token"),
+                          ([[1], [2], [3]], "n 3"), ([[], [1] * 161], "cache of 160")):
+            with pytest.raises(moe.RbtMoeError, match=word):
+                m.paged_step(new)
+        nxt, lg, _ = m.paged_step([[7], [8, 9]])
+        for lgi, toks in ((lg[0], a + [7]), (lg[1], [8, 9])):
+            want, _ = ref.prefill(toks, 0, logit_rows=1)
+            assert np.abs(lgi.astype(np.float64) - want[0]).max() / np.abs(want[0]).max() < LOGIT_RTOL
+        m.paged_release([1, 1])
+        m.paged_step([[1] * 70, []])  # all five pages again
+        with pytest.raises(moe.RbtMoeError, match="pages needed"):
+            m.paged_step([[1] * 11, []])
+        m.set_pages(0)
+        with pytest.raises(moe.RbtMoeError, match="no pages"):
+            m.paged_release([1])
+        ref.forward(1, 0)  # and the other paths are as before
+    finally:
+        m.close()
+        ref.close()
