@@ -389,7 +389,8 @@ RbtMoe *rbt_model_moe(RbtModel *m);
 
 typedef struct RbtPagedConfig {
     int32_t n_layers;    /* caches to bind (rbt_paged_bind_layer); 0: block tables only, the heads unused */
-    int32_t n_heads, n_kv_heads, head_dim; /* head_dim 64 or 128; n_heads a multiple of n_kv_heads */
+    int32_t n_heads, n_kv_heads, head_dim; /* head_dim 64 or 128; n_heads, up to 1024, a multiple of
+                                            n_kv_heads, up to 512 times it */
     int32_t page_size;   /* a power of two, 8 .. 256 */
     int32_t n_pages;     /* pages of the pool, the same for every layer */
     int32_t dtype;       /* of the caches, and of q and the output of the attention */
@@ -436,8 +437,8 @@ int rbt_paged_plan_device(RbtPaged *p, int n_seq, const int32_t *d_len, const in
  * at d_pos when d_cos/d_sin [rope_len][head_dim/2] are given (:481-482, pairs (i, i +
  * head_dim/2)), each result rounded once to the cache's type.  q, k, v are of
  * src_dtype; q_out, of the cache's type, may be the q rows themselves when the types
- * and strides are equal.  A row with a negative slot is padding: nothing is read or
- * written for it.  The slots of a call must be distinct.  All rows 16-byte aligned. */
+ * and strides are equal.  A row with a negative slot is padding: nothing is written for
+ * it.  The slots of a call must be distinct.  Rows, norms and angles 16-byte aligned. */
 typedef struct RbtPagedAppend {
     const void *d_q, *d_k, *d_v;
     int64_t q_stride, k_stride, v_stride; /* elements between rows */

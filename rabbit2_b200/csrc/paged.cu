@@ -293,6 +293,8 @@ int rbt_paged_append_device(RbtPaged* p, int layer, const RbtPagedAppend* args, 
     if (!x.d_slot) return fail("null slots");
     if (!x.d_q_norm != !x.d_k_norm) return fail("q_norm and k_norm must both be given or both be NULL");
     if (!x.d_cos != !x.d_sin) return fail("cos and sin must both be given or both be NULL");
+    if (!aligned16(x.d_cos) || !aligned16(x.d_sin) || !aligned16(x.d_q_norm) || !aligned16(x.d_k_norm))
+        return fail("cos, sin, q_norm and k_norm must be 16-byte aligned");
     if (x.d_cos && (!x.d_pos || x.rope_len <= 0)) return fail("RoPE needs positions and rope_len > 0");
     // in place only row by row, element by element; any other overlap would race
     const size_t es = esize(x.src_dtype), eo = esize(c.dtype);

@@ -24,7 +24,6 @@ enum PagedStatus : unsigned {
 };
 
 constexpr int kPagedMaxSeq = 2048;
-constexpr int kPagedMaxCtas = 1024;  // CTAs of one attention launch (an entry of PagedJoin each)
 
 // The tile that CTA c begins and others finish: its partial results are in slot 1 of CTA c
 // and slot 0 of CTAs c+1 .. last.  last == c: none.
@@ -60,7 +59,7 @@ struct PagedAttnArgs {
 // Rows of a tile of the kernels for few rows (f32: 1, 2, 4 or 8, chosen by the call).
 constexpr int kPagedDecRowsBf16 = 16, kPagedDecRowsF32 = 8;
 constexpr int kPagedTcRows = 256;  // rows of a unit of the tensor-core kernel (two MMA tiles)
-constexpr int kPagedF32Rows = 64;     // rows of a tile of the f32 kernel for chunks
+constexpr int kPagedF32Rows = 64;  // rows of a tile of the f32 kernel for chunks
 
 // Tensor maps of one layer's bf16 caches as rows [page][kv head][position] of head_dim.
 struct PagedMaps {

@@ -223,12 +223,17 @@ __global__ void __launch_bounds__(kTabThreads) release_kernel(const PagedTablesA
 }
 
 // ---------------------------------------------------------------- append
-// One CTA per token.  With the QK-norm the CTA first sums the squares of the whole q and
-// k rows (f32, a fixed order), then a thread takes kVec adjacent dims i and their partners
-// i + hd/2 (16-byte loads of the source): norm, rotation, one rounding to the cache's
-// type.  v is copied (and rounded).  Bound by bytes: each row is read once from HBM (the
-// second read of q and k with the norm hits L1) and written once.
-constexpr int kAppThreads = 256;
+// One CTA per token.  A thread's item is kVec adjacent dims i of a head and their partners
+// i + hd/2 (16-byte loads of the source): norm, rotation, one rounding to the cache's type;
+// v is copied (and rounded).  The loads of a thread's first items and of the token's slot
+// and position are in flight together, and with the QK-norm those items are kept between
+// the sum of the squares (f32, a fixed order) and their use; later items are read again.
+// Bound by bytes: each row is read once from HBM and written once.  4096 bf16 rows of 32 + 8
+// + 8 heads of 128 (101 MB) take 18.5 us, 5.4 TB/s; in CTAs of 256 threads 29.1, with 5 items
+// kept 22.1 (registers), with loads that wait for the slot 20.5.  64 rows of 16 heads take
+// 6.2 us, the time of a launch, its loads' latency and its stores; CTAs of 64 threads 8.2 to 10.3.
+constexpr int kAppThreads = 128;
+constexpr int kAppHeld = 3;  // items that a thread keeps
 
 template <typename S>
 struct Source;
@@ -240,11 +245,6 @@ template <>
 struct Source<uint16_t> {
     static constexpr int kVec = 8;
 };
-
-template <typename S>
-__device__ __forceinline__ void load_vec(const S* p, float (&f)[Source<S>::kVec]) {
-    WeightTraits<S>::unpack(*reinterpret_cast<const uint4*>(p), f);
-}
 
 template <int N>
 __device__ __forceinline__ void store_vec(float* p, const float (&f)[N]) {
@@ -262,43 +262,60 @@ __device__ __forceinline__ void store_vec(uint16_t* p, const float (&f)[N]) {
     if constexpr (N == 8) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
     else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
 }
+template <int N>
+__device__ __forceinline__ void load_vec(const float* p, float (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(f + i) = __ldg(reinterpret_cast<const float4*>(p + i));
+}
 
 template <typename S, typename T>
-__global__ void __launch_bounds__(kAppThreads) append_kernel(const PagedAppendArgs a) {
+__global__ void __launch_bounds__(kAppThreads) append_kernel(const __grid_constant__ PagedAppendArgs a) {
     constexpr int V = Source<S>::kVec;
     __shared__ float red[2][kAppThreads / 32];
     const int r = blockIdx.x, tid = threadIdx.x, hd = a.hd, half = hd / 2;
-    const int64_t slot = a.slot[r];
-    if (slot < 0) return;
-    if (slot >= a.n_slots) {
-        if (tid == 0) record(a.status, kPagedSlot);
-        return;
-    }
-    const float *cs = nullptr, *sn = nullptr;
-    if (a.cos) {
-        const int pos = a.pos[r];
-        if (pos < 0 || pos >= a.rope_len) {
-            if (tid == 0) record(a.status, kPagedPos);
-            return;
-        }
-        cs = a.cos + (size_t)pos * half;
-        sn = a.sin + (size_t)pos * half;
-    }
+    const int hv = half / V, hv_shift = __ffs(hv) - 1;  // items of a head (a power of two)
+    const int64_t slot = __ldg(a.slot + r);
+    const int pos = a.cos ? __ldg(a.pos + r) : 0;
     const S* q = static_cast<const S*>(a.q) + r * a.q_stride;
     const S* k = static_cast<const S*>(a.k) + r * a.k_stride;
     const S* v = static_cast<const S*>(a.v) + r * a.v_stride;
-    const int nq = a.n_heads * hd, nkv = a.n_kv * hd;
+    const int n_pairs = (a.n_heads + a.n_kv) * hv;
+    const auto load = [&](int it, uint4& x, uint4& y) {
+        const int hh = it >> hv_shift, i = (it & (hv - 1)) * V;
+        const S* src = (hh < a.n_heads ? q + (size_t)hh * hd : k + (size_t)(hh - a.n_heads) * hd) + i;
+        x = *reinterpret_cast<const uint4*>(src);
+        y = *reinterpret_cast<const uint4*>(src + half);
+    };
+    uint4 hx[kAppHeld], hy[kAppHeld];
+#pragma unroll
+    for (int j = 0; j < kAppHeld; j++)
+        if (tid + j * kAppThreads < n_pairs) load(tid + j * kAppThreads, hx[j], hy[j]);
+    if (slot < 0) return;
+    if (slot >= a.n_slots || (a.cos && (pos < 0 || pos >= a.rope_len))) {
+        if (tid == 0) record(a.status, slot >= a.n_slots ? kPagedSlot : kPagedPos);
+        return;
+    }
     float inv_q = 1.0f, inv_k = 1.0f;
     if (a.q_norm) {
+        const int n_q = a.n_heads * hv;
         float sq = 0.0f, sk = 0.0f;
-        for (int i = tid; i < (nq + nkv) / V; i += kAppThreads) {
-            const bool is_q = i < nq / V;
-            float f[V], t = 0.0f;
-            load_vec<S>(is_q ? q + (size_t)i * V : k + (size_t)(i - nq / V) * V, f);
+        const auto add = [&](int it, const uint4& x, const uint4& y) {
+            float f[V], g[V], t = 0.0f;
+            WeightTraits<S>::unpack(x, f);
+            WeightTraits<S>::unpack(y, g);
 #pragma unroll
-            for (int e = 0; e < V; e++) t = fmaf(f[e], f[e], t);
-            if (is_q) sq += t;
+            for (int e = 0; e < V; e++) t = fmaf(g[e], g[e], fmaf(f[e], f[e], t));
+            if (it < n_q) sq += t;
             else sk += t;
+        };
+#pragma unroll
+        for (int j = 0; j < kAppHeld; j++)
+            if (tid + j * kAppThreads < n_pairs) add(tid + j * kAppThreads, hx[j], hy[j]);
+#pragma unroll 1
+        for (int it = tid + kAppHeld * kAppThreads; it < n_pairs; it += kAppThreads) {
+            uint4 x, y;
+            load(it, x, y);
+            add(it, x, y);
         }
         sq = warp_sum(sq);
         sk = warp_sum(sk);
@@ -313,51 +330,66 @@ __global__ void __launch_bounds__(kAppThreads) append_kernel(const PagedAppendAr
             sq += red[0][w];
             sk += red[1][w];
         }
-        inv_q = 1.0f / sqrtf(sq / (float)nq + a.eps);
-        inv_k = 1.0f / sqrtf(sk / (float)nkv + a.eps);
+        inv_q = 1.0f / sqrtf(sq / (float)(a.n_heads * hd) + a.eps);
+        inv_k = 1.0f / sqrtf(sk / (float)(a.n_kv * hd) + a.eps);
     }
     const int64_t page = slot >> a.page_shift;
     const int off = (int)(slot & ((1 << a.page_shift) - 1));
     // element 0 of kv head 0 at this slot; kv heads are page_size * hd apart
     const size_t base = (((size_t)page * a.n_kv << a.page_shift) + off) * hd;
     const size_t head_step = (size_t)hd << a.page_shift;
-    const int hv = half / V, n_pairs = (a.n_heads + a.n_kv) * hv, n_v = nkv / V;
-    for (int it = tid; it < n_pairs + n_v; it += kAppThreads) {
-        if (it >= n_pairs) {  // v
-            const int e = (it - n_pairs) * V, h = e / hd;
-            float f[V];
-            load_vec<S>(v + e, f);
-            store_vec<V>(static_cast<T*>(a.vc) + base + h * head_step + (e - h * hd), f);
-            continue;
-        }
-        const int hh = it / hv, i = (it - hh * hv) * V;
+    const float *cs = a.cos + (size_t)pos * half, *sn = a.sin + (size_t)pos * half;
+    const auto put = [&](int it, const uint4& px, const uint4& py) {
+        const int hh = it >> hv_shift, i = (it & (hv - 1)) * V;
         const bool is_q = hh < a.n_heads;
         const int h = is_q ? hh : hh - a.n_heads;
-        const S* src = (is_q ? q : k) + (size_t)h * hd + i;
         float x[V], y[V];
-        load_vec<S>(src, x);
-        load_vec<S>(src + half, y);
+        WeightTraits<S>::unpack(px, x);
+        WeightTraits<S>::unpack(py, y);
         if (a.q_norm) {
             const float* w = (is_q ? a.q_norm : a.k_norm) + (size_t)h * hd + i;
             const float inv = is_q ? inv_q : inv_k;
+            float wx[V], wy[V];
+            load_vec(w, wx);
+            load_vec(w + half, wy);
 #pragma unroll
             for (int e = 0; e < V; e++) {
-                x[e] = x[e] * inv * w[e];
-                y[e] = y[e] * inv * w[e + half];
+                x[e] = x[e] * inv * wx[e];
+                y[e] = y[e] * inv * wy[e];
             }
         }
-        if (cs) {
+        if (a.cos) {
+            float c[V], s[V];
+            load_vec(cs + i, c);
+            load_vec(sn + i, s);
 #pragma unroll
             for (int e = 0; e < V; e++) {
-                const float c = cs[i + e], s = sn[i + e], u = x[e], t = y[e];
-                x[e] = u * c - t * s;
-                y[e] = t * c + u * s;
+                const float u = x[e], t = y[e];
+                x[e] = u * c[e] - t * s[e];
+                y[e] = t * c[e] + u * s[e];
             }
         }
         T* dst = is_q ? static_cast<T*>(a.q_out) + r * a.q_out_stride + (size_t)h * hd + i
                       : static_cast<T*>(a.kc) + base + h * head_step + i;
         store_vec<V>(dst, x);
         store_vec<V>(dst + half, y);
+    };
+    const int n_v = a.n_kv * 2 * hv;
+#pragma unroll 2
+    for (int it = tid; it < n_v; it += kAppThreads) {
+        const int h = it >> (hv_shift + 1), e = (it & (2 * hv - 1)) * V;
+        float f[V];
+        WeightTraits<S>::unpack(*reinterpret_cast<const uint4*>(v + (size_t)it * V), f);
+        store_vec<V>(static_cast<T*>(a.vc) + base + h * head_step + e, f);
+    }
+#pragma unroll
+    for (int j = 0; j < kAppHeld; j++)
+        if (tid + j * kAppThreads < n_pairs) put(tid + j * kAppThreads, hx[j], hy[j]);
+#pragma unroll 1
+    for (int it = tid + kAppHeld * kAppThreads; it < n_pairs; it += kAppThreads) {
+        uint4 x, y;
+        load(it, x, y);
+        put(it, x, y);
     }
 }
 

@@ -105,11 +105,10 @@ class PagedTables:
 
     def _vector(self, t, n, name, dtype=_I32):
         """Address of a contiguous vector of n values on the pool's GPU (n None: of any length)."""
-        shape = t.shape
-        if t.dtype is not dtype or t.get_device() != self.index or len(shape) != 1 or (n is not None and shape[0] != n) \
-                or not t.is_contiguous():
+        if t.dtype is not dtype or t.get_device() != self.index or t.dim() != 1 or \
+                (n is not None and t.numel() != n) or not t.is_contiguous():
             raise ValueError(f"{name}: a contiguous {dtype} vector{'' if n is None else f' of {n}'} on {self.device} is "
-                             f"wanted (got {t.dtype} {tuple(shape)} on {t.device})")
+                             f"wanted (got {t.dtype} {tuple(t.shape)} on {t.device})")
         return t.data_ptr()
 
     def _table(self, t, n):

@@ -19,6 +19,7 @@ def _error():
     (dict(n_pages=0), "n_pages"), (dict(head_dim=96), "head_dim"), (dict(n_kv_heads=3), "n_kv_heads"),
     (dict(n_kv_heads=0), "n_kv_heads"), (dict(dtype=2), "dtype"), (dict(n_layers=-1), "n_layers"),
     (dict(n_pages=1 << 26), "rows"), (dict(n_heads=2048, n_kv_heads=2048), "n_heads"),
+    (dict(n_heads=513, n_kv_heads=1), "heads per kv head"),
 ])
 def test_create_refuses(change, word):
     cfg = dict(n_layers=1, n_heads=8, n_kv_heads=4, head_dim=64, page_size=16, n_pages=10, dtype=1)

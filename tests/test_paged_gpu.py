@@ -292,6 +292,11 @@ def test_append_refuses():
     with pytest.raises(moe.RbtMoeError, match="aligned"):
         wide = torch.zeros(5, 4 * 64 + 2, device="cuda")
         kv.append(wide[:, 2:].unflatten(1, (4, 64)), k, v, slot, pos, out)
+    with pytest.raises(moe.RbtMoeError, match="aligned"):
+        kv.append(q, k, v, slot, pos, out, q_norm=torch.ones(257, device="cuda")[1:], k_norm=torch.ones(128, device="cuda"))
+    with pytest.raises(moe.RbtMoeError, match="aligned"):
+        off = torch.zeros(10 * 32 + 1, device="cuda")[1:].view(10, 32)
+        kv.append(q, k, v, slot, pos, out, cos=off, sin=sin)
     with pytest.raises(moe.RbtMoeError, match="overlaps"):
         both = torch.zeros(9, 4, 64, device="cuda")
         kv.append(both[:5], k, v, slot, pos, both[4:])
