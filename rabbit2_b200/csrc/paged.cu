@@ -94,6 +94,12 @@ int check_layer(const RbtPaged* p, int layer) {
 
 size_t esize(int dtype) { return dtype == RBT_MOE_DT_BF16 ? 2 : 4; }
 
+bool in_caches(const RbtPaged* p, int layer, const void* a, size_t n) {
+    const RbtPagedConfig& c = p->cfg;
+    const size_t bytes = (size_t)c.n_pages * c.n_kv_heads * c.page_size * c.head_dim * esize(c.dtype);
+    return overlap(a, n, p->layers[layer].k, bytes) || overlap(a, n, p->layers[layer].v, bytes);
+}
+
 // rows of `width` elements, stride elements apart, 16-byte aligned
 int check_rows(const char* name, const void* ptr, int64_t stride, int width, int dtype) {
     if (!ptr) return fail("null %s", name);
@@ -110,7 +116,7 @@ int rbt_paged_create(RbtPaged** out, const RbtPagedConfig* cfg, int device) {
     if (!out || !cfg) return fail("null argument");
     *out = nullptr;
     const RbtPagedConfig& c = *cfg;
-    if (c.n_layers < 0) return fail("n_layers must be >= 0 (got %d)", c.n_layers);
+    if (c.n_layers < 0 || c.n_layers > 65536) return fail("n_layers %d outside [0, 65536]", c.n_layers);
     if (c.page_size < 8 || c.page_size > 256 || (c.page_size & (c.page_size - 1)))
         return fail("page_size %d must be a power of two in [8, 256]", c.page_size);
     if (c.n_pages <= 0) return fail("n_pages must be positive (got %d)", c.n_pages);
@@ -312,6 +318,7 @@ int rbt_paged_append_device(RbtPaged* p, int layer, const RbtPagedAppend* args, 
     if ((overlap(x.d_q_out, n_out, x.d_k, span(x.k_stride, nkv, es)) && !rows_apart(x.d_k, x.k_stride)) ||
         (overlap(x.d_q_out, n_out, x.d_v, span(x.v_stride, nkv, es)) && !rows_apart(x.d_v, x.v_stride)))
         return fail("q_out overlaps k or v");
+    if (in_caches(p, layer, x.d_q_out, n_out)) return fail("q_out overlaps the caches");
     ON_DEVICE(p);
     PagedAppendArgs a{};
     a.q = x.d_q;
@@ -364,6 +371,7 @@ int rbt_paged_attention_device(RbtPaged* p, int layer, const RbtPagedAttention* 
     if (overlap(x.d_q, ((size_t)(x.n_rows - 1) * x.q_stride + nq) * e, x.d_out,
                 ((size_t)(x.n_rows - 1) * x.out_stride + nq) * e))
         return fail("out overlaps q");
+    if (in_caches(p, layer, x.d_out, ((size_t)(x.n_rows - 1) * x.out_stride + nq) * e)) return fail("out overlaps the caches");
     ON_DEVICE(p);
     PagedAttnArgs a{};
     a.q = x.d_q;
@@ -389,7 +397,7 @@ int rbt_paged_attention_device(RbtPaged* p, int layer, const RbtPagedAttention* 
     a.page_shift = p->page_shift;
     a.n_pages = c.n_pages;
     a.causal = x.causal;
-    a.window = x.window;
+    a.window = x.window < a.most_len ? x.window : 0;  // (a wider one hides nothing)
     a.scale = x.scale;
     a.part = p->part;
     a.join = p->join;

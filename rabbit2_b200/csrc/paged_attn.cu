@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const __grid_c
             for (int e = tid; e < KB * CH; e += kRowsThreads) {
                 const int r = e / CH, c = (e - r * CH) * V, p = p0 + r;
                 float4 k4 = make_float4(0.f, 0.f, 0.f, 0.f), v4 = k4;
-                if (p < t.hi) {
+                if (p >= t.lo && p < t.hi) {
                     const int id = table[p >> a.page_shift];
                     if ((unsigned)id < (unsigned)a.n_pages) {
                         const size_t at = ((((size_t)id * a.n_kv + t.kvh) << a.page_shift) + (p & (page - 1))) * HD + c;
@@ -221,7 +221,7 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedAttnArgs a, int tile_rows) {
     const PagedJoin j = a.join[blockIdx.x];
     const int c0 = blockIdx.x;
-    if (j.last <= c0) return;
+    if (j.last <= c0 || j.last >= (int)gridDim.x) return;
     constexpr int DL = HD / 32;
     const int lane = threadIdx.x & 31, part_floats = paged_part_floats(tile_rows, HD);
     for (int r = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5); r < j.n_rows;

@@ -435,12 +435,12 @@ __global__ void __launch_bounds__(kDecThreads, DecBf16<HD>::kCtas)
                 pa[n >> 1][(n & 1) * 2] = pack2(x0, x1);
                 pa[n >> 1][(n & 1) * 2 + 1] = pack2(y0, y1);
             }
-            const bool tail = p0 + KB > t.hi;
-            if (tail) {  // what lies behind the last position is not a number, perhaps: no weight of 0 hides that
+            const bool tail = p0 + KB > t.hi || p0 < t.lo;
+            if (tail) {  // what no row sees is not a number, perhaps: no weight of 0 hides that
 #pragma unroll 1
                 for (int e = lane; e < KB * (HD / 8); e += 32) {
                     const int r = e / (HD / 8), c = e - r * (HD / 8);
-                    if (p0 + r >= t.hi)
+                    if (p0 + r >= t.hi || p0 + r < t.lo)
                         *reinterpret_cast<uint4*>(smem + st * kDecStage + C::kHalf + row_at(r) + (c >> 3) * half_bytes +
                                                   (((c ^ r) & 7) << 4)) = make_uint4(0, 0, 0, 0);
                 }
@@ -560,7 +560,7 @@ __global__ void __launch_bounds__(kDecThreads, DecF32<HD, R>::kCtas) paged_decod
 #pragma unroll 1
         for (int b = skip; b < w.n; b += kDecWarps) {
             const uint32_t jb = j + b, st = jb % C::kStages;
-            const int p0 = (w.first + b) * KB, nv = min(KB, t.hi - p0);
+            const int p0 = (w.first + b) * KB, v0 = max(0, t.lo - p0), nv = min(KB, t.hi - p0);  // seen by some row
             wait.warp(&ring.full[st], (jb / C::kStages) & 1);
             const float* Ks = reinterpret_cast<const float*>(smem + st * kDecStage);
             const float* Vs = reinterpret_cast<const float*>(smem + st * kDecStage + C::kHalf);
@@ -625,7 +625,7 @@ __global__ void __launch_bounds__(kDecThreads, DecF32<HD, R>::kCtas) paged_decod
 #pragma unroll
                 for (int d = 0; d < DL; d++) o[r][d] *= alpha[r];
 #pragma unroll 4
-            for (int p = 0; p < nv; p++) {
+            for (int p = v0; p < nv; p++) {
                 float v[DL], x[R];
 #pragma unroll
                 for (int d = 0; d < DL; d += 2)

@@ -371,18 +371,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     wait.ok = false;
                     break;
                 }
-                const bool tail = p0 + kTcBlock > w.t.hi;
+                const bool tail = p0 + kTcBlock > w.t.hi || p0 < w.t.lo;
                 uint64_t* bar = tail ? &bars.v_tail : &bars.v_full[st];
                 if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
                 __syncwarp();
                 if (on) tma_load_3d(smem + C::oV + st * C::kTileBytes + at, &tm_v, bar, 0, y, half);
                 if (tail) {
-                    // what lies behind the last position is not a number, perhaps, which a weight of 0 would not hide
+                    // what no row sees is not a number, perhaps, which a weight of 0 would not hide: rows
+                    // [0, r1) before the window and [r0, 128) behind the last position
                     const bool got = wait.warp(&bars.v_tail, n_tail++ & 1);
-                    const int r0 = max(0, w.t.hi - p0);
+                    const int r1 = min(kTcBlock, max(0, w.t.lo - p0)), r0 = max(r1, min(kTcBlock, w.t.hi - p0));
+                    const int hidden = r1 + kTcBlock - r0;
 #pragma unroll 1
-                    for (int e = lane; e < (kTcBlock - r0) * (HD / 8); e += 32) {
-                        const int r = r0 + e / (HD / 8), c = e % (HD / 8);
+                    for (int e = lane; e < hidden * (HD / 8); e += 32) {
+                        const int z = e / (HD / 8), c = e % (HD / 8), r = z < r1 ? z : z - r1 + r0;
                         *reinterpret_cast<uint4*>(smem + C::oV + st * C::kTileBytes + (c >> 3) * C::kHalf + sw128(r, c & 7)) =
                             make_uint4(0, 0, 0, 0);
                     }

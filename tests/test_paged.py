@@ -17,7 +17,7 @@ def _error():
 @pytest.mark.parametrize("change, word", [
     (dict(page_size=24), "page_size"), (dict(page_size=4), "page_size"), (dict(page_size=512), "page_size"),
     (dict(n_pages=0), "n_pages"), (dict(head_dim=96), "head_dim"), (dict(n_kv_heads=3), "n_kv_heads"),
-    (dict(n_kv_heads=0), "n_kv_heads"), (dict(dtype=2), "dtype"), (dict(n_layers=-1), "n_layers"),
+    (dict(n_kv_heads=0), "n_kv_heads"), (dict(dtype=2), "dtype"), (dict(n_layers=-1), "n_layers"), (dict(n_layers=1 << 30), "n_layers"),
     (dict(n_pages=1 << 26), "rows"), (dict(n_heads=2048, n_kv_heads=2048), "n_heads"),
     (dict(n_heads=513, n_kv_heads=1), "heads per kv head"),
 ])

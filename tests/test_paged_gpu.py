@@ -547,11 +547,48 @@ def test_attention_is_repeatable_and_captured(dtype, seqs):
     assert kv.status() == 0
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads, kvh, hd, page", [(16, 16, 128, 64), (8, 2, 64, 16), (12, 1, 128, 256), (4, 4, 64, 8)])
+@pytest.mark.parametrize("seqs, window", [([(c, 1) for c in (0, 5, 40, 77, 300, 1000)], 21), ([(300, 70), (50, 1), (0, 90)], 33)])
+def test_what_lies_before_every_window_may_hold_anything(dtype, heads, kvh, hd, page, seqs, window):
+    b = Batch(seqs, heads, kvh, hd, page, dtype, seed=5)
+    for i, (c, n) in enumerate(seqs):
+        p = torch.arange(max(0, c - window + 1), device="cuda")  # the first new token sees c - window + 1 ..
+        pg = b.table[i].long()[p // page]
+        b.k[pg, :, p % page] = math.inf
+        b.v[pg, :, p % page] = math.nan
+    b.check(window=window)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_window_beyond_the_table_is_none(dtype):
+    b = Batch([(70, 1), (0, 0), (10, 40)], 8, 2, 64, 16, dtype)
+    b.length[1] = 0
+    want = b.run()[1:]
+    for window in (112, 4096, (1 << 31) - 1):
+        for got, w in zip(b.run(window=window)[1:], want):
+            assert torch.equal(got, w)
+    # new tokens that a length does not hold stand before position 0 and see nothing, under any window
+    b = Batch([(0, 40)], 8, 2, 64, 16, dtype)
+    b.length[0] = 3
+    for window in (0, 2, (1 << 31) - 1):
+        kv, out, lse = b.run(window=window)
+        assert kv.status() == 0 and (out[:37] == 0).all() and (lse[:37] == -math.inf).all()
+        assert torch.isfinite(lse[37:]).all()
+
+
 def test_attention_refuses():
     from rabbit2_b200.paged import PagedKv
     b = Batch([(20, 3)], 4, 2, 64, 16, "bf16")
     kv = PagedKv(b.k, b.v, 4)
     out = torch.zeros_like(b.q)
+    with pytest.raises(moe.RbtMoeError, match="overlaps the caches"):
+        kv.attention(b.q, b.k.view(-1)[:b.q.numel()].view(b.q.shape), b.cu, b.length, b.table, 3)
+    with pytest.raises(moe.RbtMoeError, match="too many for one call"):
+        # 2^15 rows of two heads each (tiles of 16) over 2^23 positions (an arithmetic refusal: nothing is read)
+        wide = torch.zeros(1, 1 << 19, dtype=torch.int32, device="cuda")
+        q = torch.zeros(1 << 15, 4, 64, dtype=torch.bfloat16, device="cuda")
+        kv.attention(q, torch.zeros_like(q), b.cu, b.length, wide, 1 << 15)
     with pytest.raises(moe.RbtMoeError, match="window"):
         kv.attention(b.q, out, b.cu, b.length, b.table, 3, causal=False, window=4)
     with pytest.raises(moe.RbtMoeError, match="window"):
