@@ -213,55 +213,42 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const __grid_c
 }
 
 // ---------------------------------------------------------------- join
-// CTA c adds up the parts of the tile that attention CTA c began and others finished: a
-// warp per row, M = max m_i, o = sum o_i 2^(m_i - M) / sum l_i 2^(m_i - M), in CTA order.
-constexpr int kJoinThreads = 128, kJoinSplit = 8;
+// CTA (c, y) adds up the parts of rows 8 y .. 8 y + 8 of the tile that attention CTA c began
+// and others finished: a thread per row and four dims, M = max m_i, o = sum o_i 2^(m_i - M) /
+// sum l_i 2^(m_i - M), in CTA order.
+constexpr int kJoinRows = 8;
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedAttnArgs a, int tile_rows) {
+__global__ void __launch_bounds__(kJoinRows * HD / 4) paged_join_kernel(const __grid_constant__ PagedAttnArgs a, int tile_rows) {
     const PagedJoin j = a.join[blockIdx.x];
-    const int c0 = blockIdx.x;
-    if (j.last <= c0 || j.last >= (int)gridDim.x) return;
-    constexpr int DL = HD / 32;
-    const int lane = threadIdx.x & 31, part_floats = paged_part_floats(tile_rows, HD);
-    for (int r = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5); r < j.n_rows;
-         r += kJoinSplit * (kJoinThreads / 32)) {
-        float M = -INFINITY, L = 0.0f, o[DL];
-#pragma unroll
-        for (int d = 0; d < DL; d++) o[d] = 0.0f;
+    const int c0 = blockIdx.x, r = blockIdx.y * kJoinRows + threadIdx.x / (HD / 4), d = threadIdx.x % (HD / 4) * 4;
+    if (j.last <= c0 || j.last >= (int)gridDim.x || r >= j.n_rows) return;
+    const int part_floats = paged_part_floats(tile_rows, HD);
+    float M = -INFINITY, L = 0.0f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-        for (int c = c0; c <= j.last; c++) {
-            const float* p = a.part + ((size_t)c * 2 + (c == c0)) * part_floats;
-            const float m = p[r], l = p[tile_rows + r];
-            const float* po = p + paged_part_o(tile_rows) + (size_t)r * HD + lane * DL;
-            const float mn = fmaxf(M, m), base = mn == -INFINITY ? 0.0f : mn;
-            const float x = ex2(M - base), y = ex2(m - base);
-            L = L * x + l * y;
-            float f[DL];
-            if constexpr (DL == 4) *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(po);
-            else *reinterpret_cast<float2*>(f) = *reinterpret_cast<const float2*>(po);
-#pragma unroll
-            for (int d = 0; d < DL; d++) o[d] = o[d] * x + f[d] * y;
-            M = mn;
-        }
-        const int pr = j.row0 + r, tok = pr / a.group, h = j.kvh * a.group + pr - tok * a.group;
-        const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;
-        T* dst = static_cast<T*>(a.out) + (j.tok0 + tok) * a.out_stride + (size_t)h * HD + lane * DL;
-#pragma unroll
-        for (int d = 0; d < DL; d++) o[d] *= inv;
-        if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int d = 0; d < DL; d++) dst[d] = o[d];
-        } else {
-#pragma unroll
-            for (int d = 0; d < DL; d += 2) {
-                const __nv_bfloat162 b = __floats2bfloat162_rn(o[d], o[d + 1]);
-                *reinterpret_cast<uint32_t*>(dst + d) = *reinterpret_cast<const uint32_t*>(&b);
-            }
-        }
-        if (a.lse && lane == 0)
-            a.lse[(size_t)(j.tok0 + tok) * a.n_heads + h] = L == 0.0f ? -INFINITY : M * kLn2 + logf(L);
+    for (int c = c0; c <= j.last; c++) {
+        const float* p = a.part + ((size_t)c * 2 + (c == c0)) * part_floats;
+        const float m = p[r], l = p[tile_rows + r];
+        const float4 f = *reinterpret_cast<const float4*>(p + paged_part_o(tile_rows) + (size_t)r * HD + d);
+        const float mn = fmaxf(M, m), base = mn == -INFINITY ? 0.0f : mn;
+        const float x = ex2(M - base), y = ex2(m - base);
+        L = L * x + l * y;
+        o = make_float4(o.x * x + f.x * y, o.y * x + f.y * y, o.z * x + f.z * y, o.w * x + f.w * y);
+        M = mn;
     }
+    const int pr = j.row0 + r, tok = pr / a.group, h = j.kvh * a.group + pr - tok * a.group;
+    const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;
+    T* dst = static_cast<T*>(a.out) + (j.tok0 + tok) * a.out_stride + (size_t)h * HD + d;
+    o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(dst) = o;
+    } else {
+        const __nv_bfloat162 x = __floats2bfloat162_rn(o.x, o.y), y = __floats2bfloat162_rn(o.z, o.w);
+        *reinterpret_cast<uint2*>(dst) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+    }
+    if (a.lse && d == 0) a.lse[(size_t)(j.tok0 + tok) * a.n_heads + h] = L == 0.0f ? -INFINITY : M * kLn2 + logf(L);
 }
 
 template <int HD>
@@ -290,13 +277,13 @@ cudaError_t launch_paged_rows(int hd, const PagedAttnArgs& a, int ctas, cudaStre
 }
 
 cudaError_t launch_paged_join(int dtype, int hd, int tile_rows, const PagedAttnArgs& a, int ctas, cudaStream_t s) {
-    const dim3 grid(ctas, kJoinSplit);
+    const dim3 grid(ctas, tile_rows / kJoinRows);
     if (dtype == RBT_MOE_DT_BF16) {
-        if (hd == 64) paged_join_kernel<uint16_t, 64><<<grid, kJoinThreads, 0, s>>>(a, tile_rows);
-        else paged_join_kernel<uint16_t, 128><<<grid, kJoinThreads, 0, s>>>(a, tile_rows);
+        if (hd == 64) paged_join_kernel<uint16_t, 64><<<grid, kJoinRows * 64 / 4, 0, s>>>(a, tile_rows);
+        else paged_join_kernel<uint16_t, 128><<<grid, kJoinRows * 128 / 4, 0, s>>>(a, tile_rows);
     } else {
-        if (hd == 64) paged_join_kernel<float, 64><<<grid, kJoinThreads, 0, s>>>(a, tile_rows);
-        else paged_join_kernel<float, 128><<<grid, kJoinThreads, 0, s>>>(a, tile_rows);
+        if (hd == 64) paged_join_kernel<float, 64><<<grid, kJoinRows * 64 / 4, 0, s>>>(a, tile_rows);
+        else paged_join_kernel<float, 128><<<grid, kJoinRows * 128 / 4, 0, s>>>(a, tile_rows);
     }
     return cudaGetLastError();
 }

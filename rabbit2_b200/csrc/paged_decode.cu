@@ -560,10 +560,10 @@ __global__ void __launch_bounds__(kDecThreads, DecF32<HD, R>::kCtas) paged_decod
 #pragma unroll 1
         for (int b = skip; b < w.n; b += kDecWarps) {
             const uint32_t jb = j + b, st = jb % C::kStages;
-            const int p0 = (w.first + b) * KB, v0 = max(0, t.lo - p0), nv = min(KB, t.hi - p0);  // seen by some row
+            const int p0 = (w.first + b) * KB, v0 = max(0, t.lo - p0), nv = min(KB, t.hi - p0) - v0;  // seen by some row: v0 .. v0 + nv
             wait.warp(&ring.full[st], (jb / C::kStages) & 1);
             const float* Ks = reinterpret_cast<const float*>(smem + st * kDecStage);
-            const float* Vs = reinterpret_cast<const float*>(smem + st * kDecStage + C::kHalf);
+            const float* Vs = reinterpret_cast<const float*>(smem + st * kDecStage + C::kHalf) + v0 * HD;
             float s[NI][R];
 #pragma unroll
             for (int i = 0; i < NI; i++) {
@@ -624,14 +624,15 @@ __global__ void __launch_bounds__(kDecThreads, DecF32<HD, R>::kCtas) paged_decod
             for (int r = 0; r < R; r++)
 #pragma unroll
                 for (int d = 0; d < DL; d++) o[r][d] *= alpha[r];
+            const float* wv = wp + v0 * R;
 #pragma unroll 4
-            for (int p = v0; p < nv; p++) {
+            for (int p = 0; p < nv; p++) {
                 float v[DL], x[R];
 #pragma unroll
                 for (int d = 0; d < DL; d += 2)
                     *reinterpret_cast<float2*>(v + d) = *reinterpret_cast<const float2*>(Vs + p * HD + lane * DL + d);
 #pragma unroll
-                for (int r = 0; r < R; r++) x[r] = wp[p * R + r];
+                for (int r = 0; r < R; r++) x[r] = wv[p * R + r];
 #pragma unroll
                 for (int r = 0; r < R; r++)
 #pragma unroll

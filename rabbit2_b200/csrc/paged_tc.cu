@@ -538,6 +538,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (!w.whole && w.head && threadIdx.x == 0)
                 join_later(a, w);
         }
+        wait.report(a.status);
     }
     tc_fence_before();
     __syncthreads();
