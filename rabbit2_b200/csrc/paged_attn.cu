@@ -22,7 +22,13 @@ using namespace paged;
 
 // ---------------------------------------------------------------- rows kernel
 // 16 x 16 threads: thread (ty, tx) owns rows ty kRM .. + kRM, score columns tx + 16 j and
-// output dims 4 tx + 64 k.
+// output dims 4 tx + 64 k.  Bound by the f32 FMAs (74 TFLOP/s nominal) and the shared-memory
+// reads that feed them, three quarters as long: products and sums stay in f32, so that a
+// cache of f32 loses nothing.  Two CTAs per SM of 8 warps; k and v of the next block are
+// copied while one is computed (109 -> 102 us for 5 chunks of up to 333 tokens on up to
+// 1500 cached, 12 heads over 6 of 64; 154 -> 144 us for a chunk of 1024, 16 heads of 128,
+// of that 4 us by the packed FMAs); four warps of 8 rows a thread take as long, blocks
+// of 32 positions at head_dim 64 109 us.
 constexpr int kRowsThreads = 256;
 
 template <int HD>
@@ -30,20 +36,26 @@ struct RowsCfg {
     static constexpr int kRM = kPagedF32Rows / 16, kRows = kPagedF32Rows;
     static constexpr int kKN = HD == 64 ? 4 : 2, kBlock = 16 * kKN;
     static constexpr int kLd = HD + 4, kLdP = kBlock + 4;
-    static constexpr int kFloats = kRows * kLd + 2 * kBlock * kLd + kRows * kLdP;
+    static constexpr int kKv = 2 * kBlock * kLd;  // k and v of a block; two blocks are kept
+    static constexpr int kFloats = kRows * kLd + 2 * kKv + kRows * kLdP;
     static constexpr int kPart = paged_part_floats(kRows, HD);
 };
 
+// 16 bytes to shared memory, asynchronously; zeros if not `on` (nothing is read then)
+__device__ __forceinline__ void copy16(float* dst, const float* src, bool on) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::smem_u32(dst)), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 template <int HD>
-__global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const __grid_constant__ PagedAttnArgs a) {
+__global__ void __launch_bounds__(kRowsThreads, 2) paged_rows_kernel(const __grid_constant__ PagedAttnArgs a) {
     using C = RowsCfg<HD>;
     constexpr int RM = C::kRM, KN = C::kKN, KB = C::kBlock, LD = C::kLd, LDP = C::kLdP, DV = HD / 64;
     constexpr int V = 4, CH = HD / V;
     extern __shared__ __align__(16) float sm[];
     float* Qs = sm;
-    float* Ks = Qs + C::kRows * LD;
-    float* Vs = Ks + KB * LD;
-    float* Ps = Vs + KB * LD;
+    float* Kv = Qs + C::kRows * LD;
+    float* Ps = Kv + 2 * C::kKv;
     const Plan plan(a, sm + C::kFloats);
     __shared__ Share share;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
@@ -67,7 +79,7 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const __grid_c
         }
         int from[RM], to[RM];  // positions [from, to) that the thread's rows see
         float m[RM], l[RM];
-        float4 o[RM][DV];
+        ulonglong2 o[RM][DV];  // of four dims
 #pragma unroll
         for (int i = 0; i < RM; i++) {
             const int r = ty * RM + i, pos = t.off + t.token(a, r);
@@ -76,60 +88,61 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const __grid_c
             m[i] = -INFINITY;
             l[i] = 0.0f;
 #pragma unroll
-            for (int k = 0; k < DV; k++) o[i][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int k = 0; k < DV; k++) o[i][k] = make_ulonglong2(0, 0);
         }
         const int32_t* table = a.table + (size_t)t.seq * a.table_stride;
+        // positions of block b into one of the two buffers; what no row sees becomes zeros
+        const auto fetch = [&](int b) {
+            float* dst = Kv + (b & 1) * C::kKv;
+            const int p0 = b * KB;
+#pragma unroll
+            for (int e = tid; e < KB * CH; e += kRowsThreads) {
+                const int r = e / CH, c = (e - r * CH) * V, p = p0 + r;
+                size_t at = 0;
+                bool on = p >= t.lo && p < t.hi;
+                if (on) {
+                    const int id = table[p >> a.page_shift];
+                    on = (unsigned)id < (unsigned)a.n_pages;
+                    if (on) at = ((((size_t)id * a.n_kv + t.kvh) << a.page_shift) + (p & (page - 1))) * HD + c;
+                    else atomicCAS(a.status, 0u, (unsigned)kPagedTable);
+                }
+                copy16(dst + r * LD + c, static_cast<const float*>(a.k) + at, on);
+                copy16(dst + (KB + r) * LD + c, static_cast<const float*>(a.v) + at, on);
+            }
+        };
+        fetch(w.first);
 #pragma unroll 1
         for (int b = w.first; b < w.first + w.n; b++) {
             const int p0 = b * KB;
-            __syncthreads();  // the block before is consumed (and Qs written, on the first pass)
-            for (int e = tid; e < KB * CH; e += kRowsThreads) {
-                const int r = e / CH, c = (e - r * CH) * V, p = p0 + r;
-                float4 k4 = make_float4(0.f, 0.f, 0.f, 0.f), v4 = k4;
-                if (p >= t.lo && p < t.hi) {
-                    const int id = table[p >> a.page_shift];
-                    if ((unsigned)id < (unsigned)a.n_pages) {
-                        const size_t at = ((((size_t)id * a.n_kv + t.kvh) << a.page_shift) + (p & (page - 1))) * HD + c;
-                        k4 = *reinterpret_cast<const float4*>(static_cast<const float*>(a.k) + at);
-                        v4 = *reinterpret_cast<const float4*>(static_cast<const float*>(a.v) + at);
-                    } else {
-                        atomicCAS(a.status, 0u, (unsigned)kPagedTable);
-                    }
-                }
-                *reinterpret_cast<float4*>(Ks + r * LD + c) = k4;
-                *reinterpret_cast<float4*>(Vs + r * LD + c) = v4;
-            }
-            __syncthreads();
-            float s[RM][KN];
+            const float *Ks = Kv + (b & 1) * C::kKv, *Vs = Ks + KB * LD;
+            copies_done();
+            __syncthreads();  // block b has come (and Qs is written), the block before is consumed
+            if (b + 1 < w.first + w.n) fetch(b + 1);
+            uint64_t s2[RM][KN];  // even and odd dims
 #pragma unroll
             for (int i = 0; i < RM; i++)
 #pragma unroll
-                for (int j = 0; j < KN; j++) s[i][j] = 0.0f;
+                for (int j = 0; j < KN; j++) s2[i][j] = 0;
 #pragma unroll 4
             for (int c = 0; c < HD; c += 4) {
-                float4 q4[RM], k4[KN];
+                ulonglong2 q4[RM], k4[KN];
 #pragma unroll
-                for (int i = 0; i < RM; i++) q4[i] = *reinterpret_cast<const float4*>(Qs + (ty * RM + i) * LD + c);
+                for (int i = 0; i < RM; i++) q4[i] = *reinterpret_cast<const ulonglong2*>(Qs + (ty * RM + i) * LD + c);
 #pragma unroll
-                for (int j = 0; j < KN; j++) k4[j] = *reinterpret_cast<const float4*>(Ks + (tx + 16 * j) * LD + c);
+                for (int j = 0; j < KN; j++) k4[j] = *reinterpret_cast<const ulonglong2*>(Ks + (tx + 16 * j) * LD + c);
 #pragma unroll
                 for (int i = 0; i < RM; i++)
 #pragma unroll
-                    for (int j = 0; j < KN; j++) {
-                        s[i][j] = fmaf(q4[i].x, k4[j].x, s[i][j]);
-                        s[i][j] = fmaf(q4[i].y, k4[j].y, s[i][j]);
-                        s[i][j] = fmaf(q4[i].z, k4[j].z, s[i][j]);
-                        s[i][j] = fmaf(q4[i].w, k4[j].w, s[i][j]);
-                    }
+                    for (int j = 0; j < KN; j++) s2[i][j] = fma2(q4[i].y, k4[j].y, fma2(q4[i].x, k4[j].x, s2[i][j]));
             }
 #pragma unroll
             for (int i = 0; i < RM; i++) {
-                float top = -INFINITY;
+                float top = -INFINITY, s[KN];
 #pragma unroll
                 for (int j = 0; j < KN; j++) {
                     const int p = p0 + tx + 16 * j;
-                    s[i][j] = p >= from[i] && p < to[i] ? s[i][j] * k2 : -INFINITY;
-                    top = fmaxf(top, s[i][j]);
+                    s[j] = p >= from[i] && p < to[i] ? (low(s2[i][j]) + high(s2[i][j])) * k2 : -INFINITY;
+                    top = fmaxf(top, s[j]);
                 }
 #pragma unroll
                 for (int d = 1; d < 16; d <<= 1) top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, d));
@@ -138,7 +151,7 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const __grid_c
                 float sum = 0.0f;
 #pragma unroll
                 for (int j = 0; j < KN; j++) {
-                    const float p = ex2(s[i][j] - base);
+                    const float p = ex2(s[j] - base);
                     Ps[(ty * RM + i) * LDP + tx + 16 * j] = p;
                     sum += p;
                 }
@@ -148,10 +161,8 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const __grid_c
                 m[i] = mn;
 #pragma unroll
                 for (int k = 0; k < DV; k++) {
-                    o[i][k].x *= alpha;
-                    o[i][k].y *= alpha;
-                    o[i][k].z *= alpha;
-                    o[i][k].w *= alpha;
+                    o[i][k].x = mul2(o[i][k].x, pair2(alpha, alpha));
+                    o[i][k].y = mul2(o[i][k].y, pair2(alpha, alpha));
                 }
             }
             __syncwarp();  // the 16 threads of a row are lanes of one warp
@@ -164,14 +175,12 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const __grid_c
                 for (int e = 0; e < 4; e++)
 #pragma unroll
                     for (int k = 0; k < DV; k++) {
-                        const float4 v4 = *reinterpret_cast<const float4*>(Vs + (c + e) * LD + 4 * tx + 64 * k);
+                        const ulonglong2 v4 = *reinterpret_cast<const ulonglong2*>(Vs + (c + e) * LD + 4 * tx + 64 * k);
 #pragma unroll
                         for (int i = 0; i < RM; i++) {
                             const float p = e == 0 ? p4[i].x : e == 1 ? p4[i].y : e == 2 ? p4[i].z : p4[i].w;
-                            o[i][k].x = fmaf(p, v4.x, o[i][k].x);
-                            o[i][k].y = fmaf(p, v4.y, o[i][k].y);
-                            o[i][k].z = fmaf(p, v4.z, o[i][k].z);
-                            o[i][k].w = fmaf(p, v4.w, o[i][k].w);
+                            o[i][k].x = fma2(pair2(p, p), v4.x, o[i][k].x);
+                            o[i][k].y = fma2(pair2(p, p), v4.y, o[i][k].y);
                         }
                     }
             }
@@ -188,7 +197,7 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const __grid_c
 #pragma unroll
                 for (int k = 0; k < DV; k++)
                     *reinterpret_cast<float4*>(dst + 4 * tx + 64 * k) =
-                        make_float4(o[i][k].x * inv, o[i][k].y * inv, o[i][k].z * inv, o[i][k].w * inv);
+                        make_float4(low(o[i][k].x) * inv, high(o[i][k].x) * inv, low(o[i][k].y) * inv, high(o[i][k].y) * inv);
                 if (a.lse && tx == 0)
                     a.lse[(size_t)(t.s.row0 + tok) * a.n_heads + h] = l[i] == 0.0f ? -INFINITY : m[i] * kLn2 + logf(l[i]);
             }
@@ -204,7 +213,7 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const __grid_c
                 }
 #pragma unroll
                 for (int k = 0; k < DV; k++)
-                    *reinterpret_cast<float4*>(part + paged_part_o(C::kRows) + (size_t)r * HD + 4 * tx + 64 * k) = o[i][k];
+                    *reinterpret_cast<ulonglong2*>(part + paged_part_o(C::kRows) + (size_t)r * HD + 4 * tx + 64 * k) = o[i][k];
             }
             if (w.head && tid == 0) join_later(a, w);
         }

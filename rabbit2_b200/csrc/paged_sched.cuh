@@ -27,6 +27,28 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// Two f32 values as one operand of the packed instructions.
+__device__ __forceinline__ uint64_t pair2(float x, float y) {
+    return (uint64_t)__float_as_uint(x) | (uint64_t)__float_as_uint(y) << 32;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(x), "l"(y), "l"(z));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t x, uint64_t y) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
+    return d;
+}
+__device__ __forceinline__ float low(uint64_t x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float high(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
+    return d;
+}
+
 constexpr long long kWaitClocks = 4000000000ll;  // 2 s and more: far beyond any legitimate wait
 
 // A wait that gives up once, for good: what waits then passes its other barriers at once, and

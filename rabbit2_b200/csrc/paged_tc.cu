@@ -87,21 +87,6 @@ __device__ __forceinline__ uint32_t sw128(int r, int c) {  // 16-byte chunk c of
     return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4));
 }
 
-// Two f32 values as one operand of the packed instructions.
-__device__ __forceinline__ uint64_t pair2(float x, float y) {
-    return (uint64_t)__float_as_uint(x) | (uint64_t)__float_as_uint(y) << 32;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(x), "l"(y), "l"(z));
-    return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
-    return d;
-}
-
 // Two weights (0 .. 2^8) as bf16, to nearest with ties upwards: two integer adds and a byte
 // permute.  The conversion instruction shares the special-function pipe with ex2, which
 // bounds the softmax.  (NaN may become a number here; the row's sum keeps it.)
