@@ -21,20 +21,22 @@ namespace {
 using namespace paged;
 
 // ---------------------------------------------------------------- rows kernel
-// 16 x 16 threads: thread (ty, tx) owns rows ty kRM .. + kRM, score columns tx + 16 j and
-// output dims 4 tx + 64 k.  Bound by the f32 FMAs (74 TFLOP/s nominal) and the shared-memory
-// reads that feed them, three quarters as long: products and sums stay in f32, so that a
-// cache of f32 loses nothing.  Two CTAs per SM of 8 warps; k and v of the next block are
-// copied while one is computed (109 -> 102 us for 5 chunks of up to 333 tokens on up to
-// 1500 cached, 12 heads over 6 of 64; 154 -> 144 us for a chunk of 1024, 16 heads of 128,
-// of that 4 us by the packed FMAs); four warps of 8 rows a thread take as long, blocks
-// of 32 positions at head_dim 64 109 us.
-constexpr int kRowsThreads = 256;
+// 16 x 8 threads: thread (ty, tx) owns rows ty + 16 i, score columns tx + 8 j and output dims
+// 4 tx + 32 k .. + 4; the rows of a warp's threads and the positions of its columns lie in
+// different banks.  Products and sums stay in f32, so that a cache of f32 loses nothing; with
+// 4 rows a thread the FMA pipe is busy for half the time (50 % of its cycles, measured) and
+// bound by the shared-memory reads that feed it (70 % of theirs) and by their latency.  Two CTAs
+// per SM of 4 warps; k and v of the next block are copied while one is computed.  A chunk of
+// 1024, 16 heads of 128: 139 us (0.42 of the f32 FMA rate, 74 TFLOP/s nominal); 5 chunks of
+// up to 333 tokens on up to 1500 cached, 12 heads over 6 of 64: 101 us with its other two
+// launches.  Measured in that order: scalar FMAs 154 and 104; packed 150 and 104; with the
+// next block's copies 144 and 102; with 8 threads to a row instead of 16, 139 and 101.
+constexpr int kRowsThreads = 128;
 
 template <int HD>
 struct RowsCfg {
-    static constexpr int kRM = kPagedF32Rows / 16, kRows = kPagedF32Rows;
-    static constexpr int kKN = HD == 64 ? 4 : 2, kBlock = 16 * kKN;
+    static constexpr int kRM = 4, kRows = kPagedF32Rows;
+    static constexpr int kKN = HD == 64 ? 8 : 4, kBlock = 8 * kKN;
     static constexpr int kLd = HD + 4, kLdP = kBlock + 4;
     static constexpr int kKv = 2 * kBlock * kLd;  // k and v of a block; two blocks are kept
     static constexpr int kFloats = kRows * kLd + 2 * kKv + kRows * kLdP;
@@ -50,7 +52,7 @@ __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;
 template <int HD>
 __global__ void __launch_bounds__(kRowsThreads, 2) paged_rows_kernel(const __grid_constant__ PagedAttnArgs a) {
     using C = RowsCfg<HD>;
-    constexpr int RM = C::kRM, KN = C::kKN, KB = C::kBlock, LD = C::kLd, LDP = C::kLdP, DV = HD / 64;
+    constexpr int RM = C::kRM, KN = C::kKN, KB = C::kBlock, LD = C::kLd, LDP = C::kLdP, DV = HD / 32;
     constexpr int V = 4, CH = HD / V;
     extern __shared__ __align__(16) float sm[];
     float* Qs = sm;
@@ -58,7 +60,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_rows_kernel(const __gri
     float* Ps = Kv + 2 * C::kKv;
     const Plan plan(a, sm + C::kFloats);
     __shared__ Share share;
-    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    const int tid = threadIdx.x, tx = tid & 7, ty = tid >> 3;
     find_share<kRowsThreads, C::kRows, KB, 4>(a, plan, &share);
     Walk<C::kRows, KB> w(share, plan);
     if (tid == 0) a.join[blockIdx.x].last = blockIdx.x;
@@ -82,7 +84,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_rows_kernel(const __gri
         ulonglong2 o[RM][DV];  // of four dims
 #pragma unroll
         for (int i = 0; i < RM; i++) {
-            const int r = ty * RM + i, pos = t.off + t.token(a, r);
+            const int r = ty + 16 * i, pos = t.off + t.token(a, r);
             to[i] = r >= t.rows ? 0 : a.causal ? min(t.s.len, pos + 1) : t.s.len;
             from[i] = a.window ? max(0, pos - a.window + 1) : 0;
             m[i] = -INFINITY;
@@ -127,9 +129,9 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_rows_kernel(const __gri
             for (int c = 0; c < HD; c += 4) {
                 ulonglong2 q4[RM], k4[KN];
 #pragma unroll
-                for (int i = 0; i < RM; i++) q4[i] = *reinterpret_cast<const ulonglong2*>(Qs + (ty * RM + i) * LD + c);
+                for (int i = 0; i < RM; i++) q4[i] = *reinterpret_cast<const ulonglong2*>(Qs + (ty + 16 * i) * LD + c);
 #pragma unroll
-                for (int j = 0; j < KN; j++) k4[j] = *reinterpret_cast<const ulonglong2*>(Ks + (tx + 16 * j) * LD + c);
+                for (int j = 0; j < KN; j++) k4[j] = *reinterpret_cast<const ulonglong2*>(Ks + (tx + 8 * j) * LD + c);
 #pragma unroll
                 for (int i = 0; i < RM; i++)
 #pragma unroll
@@ -140,23 +142,23 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_rows_kernel(const __gri
                 float top = -INFINITY, s[KN];
 #pragma unroll
                 for (int j = 0; j < KN; j++) {
-                    const int p = p0 + tx + 16 * j;
+                    const int p = p0 + tx + 8 * j;
                     s[j] = p >= from[i] && p < to[i] ? (low(s2[i][j]) + high(s2[i][j])) * k2 : -INFINITY;
                     top = fmaxf(top, s[j]);
                 }
 #pragma unroll
-                for (int d = 1; d < 16; d <<= 1) top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, d));
+                for (int d = 1; d < 8; d <<= 1) top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, d));
                 const float mn = fmaxf(m[i], top), base = mn == -INFINITY ? 0.0f : mn;  // (nothing seen yet)
                 const float alpha = ex2(m[i] - base);
                 float sum = 0.0f;
 #pragma unroll
                 for (int j = 0; j < KN; j++) {
                     const float p = ex2(s[j] - base);
-                    Ps[(ty * RM + i) * LDP + tx + 16 * j] = p;
+                    Ps[(ty + 16 * i) * LDP + tx + 8 * j] = p;
                     sum += p;
                 }
 #pragma unroll
-                for (int d = 1; d < 16; d <<= 1) sum += __shfl_xor_sync(FULL_MASK, sum, d);
+                for (int d = 1; d < 8; d <<= 1) sum += __shfl_xor_sync(FULL_MASK, sum, d);
                 l[i] = l[i] * alpha + sum;
                 m[i] = mn;
 #pragma unroll
@@ -165,17 +167,17 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_rows_kernel(const __gri
                     o[i][k].y = mul2(o[i][k].y, pair2(alpha, alpha));
                 }
             }
-            __syncwarp();  // the 16 threads of a row are lanes of one warp
+            __syncwarp();  // the 8 threads of a row are lanes of one warp
 #pragma unroll 2
             for (int c = 0; c < KB; c += 4) {
                 float4 p4[RM];
 #pragma unroll
-                for (int i = 0; i < RM; i++) p4[i] = *reinterpret_cast<const float4*>(Ps + (ty * RM + i) * LDP + c);
+                for (int i = 0; i < RM; i++) p4[i] = *reinterpret_cast<const float4*>(Ps + (ty + 16 * i) * LDP + c);
 #pragma unroll
                 for (int e = 0; e < 4; e++)
 #pragma unroll
                     for (int k = 0; k < DV; k++) {
-                        const ulonglong2 v4 = *reinterpret_cast<const ulonglong2*>(Vs + (c + e) * LD + 4 * tx + 64 * k);
+                        const ulonglong2 v4 = *reinterpret_cast<const ulonglong2*>(Vs + (c + e) * LD + 4 * tx + 32 * k);
 #pragma unroll
                         for (int i = 0; i < RM; i++) {
                             const float p = e == 0 ? p4[i].x : e == 1 ? p4[i].y : e == 2 ? p4[i].z : p4[i].w;
@@ -189,14 +191,14 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_rows_kernel(const __gri
         if (w.whole) {
 #pragma unroll
             for (int i = 0; i < RM; i++) {
-                const int r = ty * RM + i;
+                const int r = ty + 16 * i;
                 if (r >= t.rows) continue;
                 const int tok = t.token(a, r), h = t.head(a, r);
                 const float inv = l[i] > 0.0f || l[i] != l[i] ? 1.0f / l[i] : 0.0f;
                 float* dst = static_cast<float*>(a.out) + (t.s.row0 + tok) * a.out_stride + (size_t)h * HD;
 #pragma unroll
                 for (int k = 0; k < DV; k++)
-                    *reinterpret_cast<float4*>(dst + 4 * tx + 64 * k) =
+                    *reinterpret_cast<float4*>(dst + 4 * tx + 32 * k) =
                         make_float4(low(o[i][k].x) * inv, high(o[i][k].x) * inv, low(o[i][k].y) * inv, high(o[i][k].y) * inv);
                 if (a.lse && tx == 0)
                     a.lse[(size_t)(t.s.row0 + tok) * a.n_heads + h] = l[i] == 0.0f ? -INFINITY : m[i] * kLn2 + logf(l[i]);
@@ -205,7 +207,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_rows_kernel(const __gri
             float* part = a.part + ((size_t)blockIdx.x * 2 + (w.head ? 1 : 0)) * C::kPart;
 #pragma unroll
             for (int i = 0; i < RM; i++) {
-                const int r = ty * RM + i;
+                const int r = ty + 16 * i;
                 if (r >= t.rows) continue;
                 if (tx == 0) {
                     part[r] = m[i];
@@ -213,7 +215,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_rows_kernel(const __gri
                 }
 #pragma unroll
                 for (int k = 0; k < DV; k++)
-                    *reinterpret_cast<ulonglong2*>(part + paged_part_o(C::kRows) + (size_t)r * HD + 4 * tx + 64 * k) = o[i][k];
+                    *reinterpret_cast<ulonglong2*>(part + paged_part_o(C::kRows) + (size_t)r * HD + 4 * tx + 32 * k) = o[i][k];
             }
             if (w.head && tid == 0) join_later(a, w);
         }
