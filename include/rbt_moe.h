@@ -413,14 +413,16 @@ int rbt_paged_status(RbtPaged *p, unsigned *status_out);
  * entries of the free list d_free [free_cap], sequence by sequence, block by block;
  * d_n_free_out[0] is the new count, d_len_out[i] is 0 for those sequences and
  * d_len[i] for the others.  On an error (0x804, 0x805) no page moves and the outputs
- * repeat the inputs.  The outputs must not overlap the inputs. */
+ * repeat the inputs.  The outputs must not overlap the inputs.  Pages that several
+ * sequences share are not counted: they would be in the free list once for each. */
 int rbt_paged_release_device(RbtPaged *p, int n_seq, const int32_t *d_len, const int32_t *d_done,
                              const int32_t *d_table, int table_stride, int32_t *d_free, int free_cap,
                              const int32_t *d_n_free, int32_t *d_len_out, int32_t *d_n_free_out, void *stream);
 
 /* d_new[i] >= 0 new tokens for each sequence of d_len[i] positions: the pages they
  * need beyond those the sequence holds are taken from the end of the free list
- * (d_free[d_n_free[0] - 1] first), sequence by sequence, and written into d_table.
+ * (d_free[d_n_free[0] - 1] first; the list holds as many entries as the count says),
+ * sequence by sequence, and written into d_table.
  * d_len_out[i] = d_len[i] + d_new[i]; d_n_free_out[0] the pages left; d_cu [n_seq+1]
  * the rows of each sequence; for every row of the new tokens its slot and position.
  * Rows n_tokens .. n_rows (the padding of a step of fixed size) get slot -1 and

@@ -393,7 +393,7 @@ int rbt_paged_attention_device(RbtPaged* p, int layer, const RbtPagedAttention* 
     a.group_inv = ((1u << 20) + a.group - 1) / a.group;
     a.group_inv32 = a.group == 1 ? 0xffffffffu : (unsigned)(((1ull << 32) + a.group - 1) / a.group);
     const int64_t most_len = (int64_t)x.table_stride << p->page_shift;
-    a.most_len = most_len > INT32_MAX ? INT32_MAX : (int)most_len;
+    a.most_len = most_len > kPagedMaxLen ? kPagedMaxLen : (int)most_len;
     a.page_shift = p->page_shift;
     a.n_pages = c.n_pages;
     a.causal = x.causal;

@@ -24,6 +24,7 @@ enum PagedStatus : unsigned {
 };
 
 constexpr int kPagedMaxSeq = 2048;
+constexpr int kPagedMaxLen = INT32_MAX - 255;  // the end of a length's last block is an int, too
 
 // The tile that CTA c begins and others finish: its partial results are in slot 1 of CTA c
 // and slot 0 of CTAs c+1 .. last.  last == c: none.

@@ -13,7 +13,7 @@ more layers with ``append`` and ``attention``.  A serving step:
 
 Lengths, tables, counts, offsets and positions are int32 tensors and slots int64, all on the
 pool's GPU.  The calls run on the current stream of that GPU unless ``stream`` names another,
-and return without waiting.  A tensor of another type, shape or device raises ValueError; what
+and return without waiting; they are for serving and record nothing for autograd.  A tensor of another type, shape or device raises ValueError; what
 only the GPU can see leaves a code that ``status()`` returns.
 """
 from __future__ import annotations
@@ -72,7 +72,9 @@ class PagedTables:
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         self.page_size, self.n_pages = page_size, n_pages
         cfg = _cfg or RbtPagedConfig(0, 0, 0, 0, page_size, n_pages, 0)
-        self.index = self.device.index or 0
+        if self.device.index is None:
+            self.device = torch.device(self.device.type, torch.cuda.current_device())
+        self.index = self.device.index
         h = C.c_void_p()
         self._call(self.lib.rbt_paged_create(C.byref(h), C.byref(cfg), self.index))
         self.handle = h.value

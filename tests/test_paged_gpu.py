@@ -577,6 +577,16 @@ def test_a_window_beyond_the_table_is_none(dtype):
         assert torch.isfinite(lse[37:]).all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_the_last_lengths_of_31_bits_are_refused(dtype):
+    from rabbit2_b200.paged import PagedKv
+    k = torch.zeros(1, 1, 256, 64, device="cuda", dtype=DT[dtype])
+    kv, q = PagedKv(k, k.clone(), 1), torch.ones(1, 1, 64, device="cuda", dtype=DT[dtype])
+    out, table = torch.full_like(q, 5), torch.zeros(1, 1 << 23, dtype=torch.int32, device="cuda")  # 2^31 positions
+    kv.attention(q, out, dev([0, 1]), dev([(1 << 31) - 1]), table, 1)
+    assert kv.status() == 0x822 and (out == 5).all()
+
+
 def test_attention_refuses():
     from rabbit2_b200.paged import PagedKv
     b = Batch([(20, 3)], 4, 2, 64, 16, "bf16")
