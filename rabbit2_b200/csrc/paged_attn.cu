@@ -226,7 +226,8 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_rows_kernel(const __gri
 // ---------------------------------------------------------------- join
 // CTA (c, y) adds up the parts of rows 8 y .. 8 y + 8 of the tile that attention CTA c began
 // and others finished: a thread per row and four dims, M = max m_i, o = sum o_i 2^(m_i - M) /
-// sum l_i 2^(m_i - M), in CTA order.
+// sum l_i 2^(m_i - M), in CTA order.  Bound by the latency of its loads: 10 us for 148 shared
+// tiles of 256 rows of 64 (17 MB); a warp to a row, several rows in turn, took 16 us.
 constexpr int kJoinRows = 8;
 
 template <typename T, int HD>

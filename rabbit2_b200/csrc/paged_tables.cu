@@ -5,7 +5,8 @@
 // few per thread: two 64-bit sums by warp shuffles), so one launch needs no exchange
 // between CTAs, and then writes its share of the pages, slots and positions.  Both are
 // bound by latency (a launch, one round of loads, the scan, one or two dependent
-// loads), not by bytes.  The outputs must not overlap the inputs because CTAs read and
+// loads), not by bytes: a release and a plan take 6.2 us together for 7 sequences, 8.2 us
+// for 1000 with 100 KB of slots.  The outputs must not overlap the inputs because CTAs read and
 // write at different times; the table (plan) and the free list (release) are only
 // written where no CTA of the call reads them.
 #include <cuda_bf16.h>
