@@ -16,10 +16,10 @@
 //
 // Four prompts of 4096 in pages of 64, 16 heads of 128 (275 GFLOP): 365 us, 753 TFLOP/s, 0.45
 // of a large bf16 GEMM's rate.  Neither the tensor pipe (38 % of its cycles) nor the
-// special-function unit (38 %) nor the copies bound it: without the exponentials it takes as
-// long, without the MMAs 0.9 and without the copies 0.98 of the time.  What it waits for is the
-// chain of a step of 64 positions (scores, weights, product) through TMEM and barriers: 1500 to
-// 1800 clocks for both tiles, of which the MMAs need 1024.  Also measured: steps of 128 positions
+// special-function unit (38 %) bounds it: without the exponentials it takes as long, without the
+// MMAs 0.88 and without MMAs and softmax 0.64 of the time.  What it waits for is the chain of a
+// step of 64 positions (scores, weights, product) through TMEM and barriers: 1.5 us for both
+// tiles, of which the MMAs need 0.55 at their nominal rate.  Also measured: steps of 128 positions
 // with one score buffer 380-420 us, four issuing threads 377-382, 16 softmax warps 407, the next
 // scores issued when the weights arrive instead of when the product before them ends 454.
 //
