@@ -1,0 +1,286 @@
+// paged_bind.cpp -- the checks and calls of rabbit2_b200/paged.py for torch tensors, as an
+// extension module (_paged_bind.so): a step's calls come once per layer and take 4 to 8 us on
+// the GPU when it decodes.  The host takes 4 to 5 us a call, of which the launch is half; the
+// same checks through tensor attributes and ctypes took 7 to 11 us.  The module calls the functions of librbt_moe.so that use() is given.
+#include <Python.h>
+
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <cstdint>
+#include <stdexcept>
+#include <string>
+
+#include "../../include/rbt_moe.h"
+
+namespace {
+
+decltype(&rbt_paged_release_device) g_release = nullptr;
+decltype(&rbt_paged_plan_device) g_plan = nullptr;
+decltype(&rbt_paged_append_device) g_append = nullptr;
+decltype(&rbt_paged_attention_device) g_attention = nullptr;
+
+struct Wrong : std::runtime_error {  // becomes a ValueError
+    using std::runtime_error::runtime_error;
+};
+struct Raised {};  // a Python error is set
+
+const char* name_of(at::ScalarType t) {
+    switch (t) {
+        case at::kFloat: return "float32";
+        case at::kBFloat16: return "bfloat16";
+        case at::kInt: return "int32";
+        case at::kLong: return "int64";
+        case at::kDouble: return "float64";
+        case at::kHalf: return "float16";
+        default: return c10::toString(t);
+    }
+}
+
+std::string got(const at::Tensor& t) {
+    const auto list = [](at::IntArrayRef v) {
+        std::string s = "[";
+        for (size_t i = 0; i < v.size(); i++) s += (i ? ", " : "") + std::to_string(v[i]);
+        return s + "]";
+    };
+    return std::string(" (got ") + name_of(t.scalar_type()) + " " + list(t.sizes()) +
+           (t.layout() == at::kStrided ? ", strides " + list(t.strides()) : ", not strided") + ", on " + t.device().str() + ")";
+}
+
+const at::Tensor& tensor(PyObject* o, const char* name) {
+    if (!THPVariable_Check(o)) throw Wrong(std::string(name) + ": a tensor is wanted");
+    return THPVariable_Unpack(o);
+}
+
+int64_t integer(PyObject* o) {
+    const int64_t v = PyLong_AsLongLong(o);
+    if (v == -1 && PyErr_Occurred()) throw Raised();
+    return v;
+}
+
+int32_t int32(int64_t v, const char* name) {
+    if (v < INT32_MIN || v > INT32_MAX) throw Wrong(std::string(name) + ": " + std::to_string(v) + " does not fit in 32 bits");
+    return (int32_t)v;
+}
+
+RbtPaged* context(PyObject* o) {  // None: a closed one, which the library refuses
+    if (o == Py_None) return nullptr;
+    void* p = PyLong_AsVoidPtr(o);
+    if (!p && PyErr_Occurred()) throw Raised();
+    return static_cast<RbtPaged*>(p);
+}
+
+float real(PyObject* o) {
+    const double v = PyFloat_AsDouble(o);
+    if (v == -1.0 && PyErr_Occurred()) throw Raised();
+    return (float)v;
+}
+
+// The calls' device; tensors on it.
+struct Call {
+    int index;
+
+    bool here(const at::Tensor& t, at::ScalarType type) const {
+        return t.layout() == at::kStrided && t.is_cuda() && t.get_device() == index && t.scalar_type() == type;
+    }
+    std::string device() const { return "cuda:" + std::to_string(index); }
+
+    // A contiguous vector of n values (n < 0: of any length).
+    template <typename T>
+    T* vector(PyObject* o, int64_t n, const char* name, at::ScalarType type = at::kInt) const {
+        const at::Tensor& t = tensor(o, name);
+        if (!here(t, type) || t.dim() != 1 || (n >= 0 && t.numel() != n) || !t.is_contiguous())
+            throw Wrong(std::string(name) + ": a contiguous " + name_of(type) + " vector" +
+                        (n < 0 ? "" : " of " + std::to_string(n)) + " on " + device() + " is wanted" + got(t));
+        return static_cast<T*>(t.data_ptr());
+    }
+    int32_t length(PyObject* o, const char* name) const {
+        const at::Tensor& t = tensor(o, name);
+        if (t.dim() < 1) throw Wrong(std::string(name) + ": a vector is wanted" + got(t));
+        return int32(t.size(0), name);
+    }
+    int32_t* table(PyObject* o, int64_t n, int32_t* stride) const {
+        const at::Tensor& t = tensor(o, "table");
+        if (!here(t, at::kInt) || t.dim() != 2 || t.size(0) != n || !t.is_contiguous())
+            throw Wrong("table: contiguous int32 rows for " + std::to_string(n) + " sequences on " + device() + " are wanted" + got(t));
+        *stride = int32(t.size(1), "table");
+        return static_cast<int32_t*>(t.data_ptr());
+    }
+    // Rows [n, heads, head dim], the heads of a row contiguous; *stride: elements between rows.
+    void* rows(PyObject* o, int64_t n, int64_t heads, int64_t hd, const char* name, at::ScalarType type, int64_t* stride) const {
+        const at::Tensor& t = tensor(o, name);
+        if (!here(t, type) || t.dim() != 3 || t.size(0) != n || t.size(1) != heads || t.size(2) != hd || t.stride(2) != 1 ||
+            (heads > 1 && t.stride(1) != hd))
+            throw Wrong(std::string(name) + ": " + name_of(type) + " rows [" + std::to_string(n) + ", " + std::to_string(heads) +
+                        ", " + std::to_string(hd) + "] on " + device() + ", contiguous within a row, are wanted" + got(t));
+        *stride = n > 1 ? t.stride(0) : heads * hd;
+        return t.data_ptr();
+    }
+    // A contiguous f32 matrix; its rows in *n if that is negative, else *n of them.
+    float* matrix(PyObject* o, int64_t* n, int64_t width, const char* name) const {
+        const at::Tensor& t = tensor(o, name);
+        if (!here(t, at::kFloat) || t.dim() != 2 || (*n >= 0 && t.size(0) != *n) || t.size(1) != width || !t.is_contiguous())
+            throw Wrong(std::string(name) + ": contiguous float32 [" + (*n < 0 ? "positions" : std::to_string(*n)) + ", " +
+                        std::to_string(width) + "] on " + device() + " is wanted" + got(t));
+        *n = t.size(0);
+        return static_cast<float*>(t.data_ptr());
+    }
+    void* stream(PyObject* o) const {  // None: the device's current one
+        if (o == Py_None) return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)index).stream();
+        void* s = PyLong_AsVoidPtr(o);
+        if (!s && PyErr_Occurred()) throw Raised();
+        return s;
+    }
+};
+
+at::ScalarType type_of(int64_t dtype) { return dtype == RBT_MOE_DT_BF16 ? at::kBFloat16 : at::kFloat; }
+
+template <typename F>
+PyObject* call(F f) {
+    int ok;
+    Py_BEGIN_ALLOW_THREADS;
+    ok = f();
+    Py_END_ALLOW_THREADS;
+    return PyBool_FromLong(ok);
+}
+
+// handle, device, length, done, table, free, n_free, length_out, n_free_out, stream
+PyObject* release(PyObject* const* x) {
+    RbtPaged* p = context(x[0]);
+    const Call c{(int)integer(x[1])};
+    const int32_t n = c.length(x[2], "length"), cap = c.length(x[5], "free");
+    const int32_t* len = c.vector<int32_t>(x[2], n, "length");
+    const int32_t* done = c.vector<int32_t>(x[3], n, "done");
+    int32_t width;
+    const int32_t* table = c.table(x[4], n, &width);
+    int32_t* free_list = c.vector<int32_t>(x[5], -1, "free");
+    const int32_t* n_free = c.vector<int32_t>(x[6], 1, "n_free");
+    int32_t* len_out = c.vector<int32_t>(x[7], n, "length_out");
+    int32_t* n_free_out = c.vector<int32_t>(x[8], 1, "n_free_out");
+    void* s = c.stream(x[9]);
+    return call([&] { return g_release(p, n, len, done, table, width, free_list, cap, n_free, len_out, n_free_out, s); });
+}
+
+// handle, device, length, new, table, free, n_free, length_out, n_free_out, cu, slot, pos, stream
+PyObject* plan(PyObject* const* x) {
+    RbtPaged* p = context(x[0]);
+    const Call c{(int)integer(x[1])};
+    const int32_t n = c.length(x[2], "length"), rows = c.length(x[10], "slot");
+    const int32_t* len = c.vector<int32_t>(x[2], n, "length");
+    const int32_t* count = c.vector<int32_t>(x[3], n, "new");
+    int32_t width;
+    int32_t* table = c.table(x[4], n, &width);
+    const int32_t* free_list = c.vector<int32_t>(x[5], -1, "free");
+    const int32_t* n_free = c.vector<int32_t>(x[6], 1, "n_free");
+    int32_t* len_out = c.vector<int32_t>(x[7], n, "length_out");
+    int32_t* n_free_out = c.vector<int32_t>(x[8], 1, "n_free_out");
+    int32_t* cu = c.vector<int32_t>(x[9], (int64_t)n + 1, "cu");
+    int64_t* slot = c.vector<int64_t>(x[10], rows, "slot", at::kLong);
+    int32_t* pos = c.vector<int32_t>(x[11], rows, "pos");
+    void* s = c.stream(x[12]);
+    return call([&] { return g_plan(p, n, len, count, table, width, free_list, n_free, rows, len_out, n_free_out, cu, slot, pos, s); });
+}
+
+// handle, device, heads, kv heads, head dim, dtype, layer, q, k, v, slot, pos, q_out, cos, sin, q_norm, k_norm, eps, stream
+PyObject* append(PyObject* const* x) {
+    RbtPaged* p = context(x[0]);
+    const Call c{(int)integer(x[1])};
+    const int64_t heads = integer(x[2]), kvh = integer(x[3]), hd = integer(x[4]);
+    const int layer = int32(integer(x[6]), "layer");
+    const at::Tensor& q = tensor(x[7], "q");
+    const at::ScalarType src = q.scalar_type();
+    if (src != at::kFloat && src != at::kBFloat16) throw Wrong(std::string("q of ") + name_of(src) + ": float32 or bfloat16 are wanted");
+    RbtPagedAppend a{};
+    a.n_rows = c.length(x[7], "q");
+    a.src_dtype = src == at::kBFloat16 ? RBT_MOE_DT_BF16 : RBT_MOE_DT_F32;
+    a.d_q = c.rows(x[7], a.n_rows, heads, hd, "q", src, &a.q_stride);
+    a.d_k = c.rows(x[8], a.n_rows, kvh, hd, "k", src, &a.k_stride);
+    a.d_v = c.rows(x[9], a.n_rows, kvh, hd, "v", src, &a.v_stride);
+    a.d_slot = c.vector<int64_t>(x[10], a.n_rows, "slot", at::kLong);
+    if (x[11] != Py_None) a.d_pos = c.vector<int32_t>(x[11], a.n_rows, "pos");
+    a.d_q_out = c.rows(x[12], a.n_rows, heads, hd, "q_out", type_of(integer(x[5])), &a.q_out_stride);
+    if ((x[13] == Py_None) != (x[14] == Py_None)) throw Wrong("cos and sin must both be given or both be None");
+    if (x[13] != Py_None) {
+        int64_t n = -1;
+        a.d_cos = c.matrix(x[13], &n, hd / 2, "cos");
+        a.d_sin = c.matrix(x[14], &n, hd / 2, "sin");
+        a.rope_len = int32(n, "cos");
+    }
+    if (x[15] != Py_None) a.d_q_norm = c.vector<float>(x[15], heads * hd, "q_norm", at::kFloat);
+    if (x[16] != Py_None) a.d_k_norm = c.vector<float>(x[16], kvh * hd, "k_norm", at::kFloat);
+    a.eps = real(x[17]);
+    void* s = c.stream(x[18]);
+    return call([&] { return g_append(p, layer, &a, s); });
+}
+
+// handle, device, heads, kv heads, head dim, dtype, layer, q, out, cu, length, table, max_new, lse, causal, window, scale, stream
+PyObject* attention(PyObject* const* x) {
+    RbtPaged* p = context(x[0]);
+    const Call c{(int)integer(x[1])};
+    const int64_t heads = integer(x[2]), hd = integer(x[4]);
+    const at::ScalarType type = type_of(integer(x[5]));
+    const int layer = int32(integer(x[6]), "layer");
+    RbtPagedAttention a{};
+    a.n_rows = c.length(x[7], "q");
+    a.n_seq = c.length(x[10], "length");
+    a.d_q = c.rows(x[7], a.n_rows, heads, hd, "q", type, &a.q_stride);
+    a.d_out = c.rows(x[8], a.n_rows, heads, hd, "out", type, &a.out_stride);
+    a.d_cu = c.vector<int32_t>(x[9], (int64_t)a.n_seq + 1, "cu");
+    a.d_len = c.vector<int32_t>(x[10], a.n_seq, "length");
+    a.d_table = c.table(x[11], a.n_seq, &a.table_stride);
+    a.max_new = int32(integer(x[12]), "max_new");
+    if (x[13] != Py_None) {
+        int64_t n = a.n_rows;
+        a.d_lse = c.matrix(x[13], &n, heads, "lse");
+    }
+    a.causal = PyObject_IsTrue(x[14]);
+    a.window = int32(integer(x[15]), "window");
+    a.scale = real(x[16]);
+    void* s = c.stream(x[17]);
+    return call([&] { return g_attention(p, layer, &a, s); });
+}
+
+// addresses of the four functions, in the order of these
+PyObject* use(PyObject* const* x) {
+    void* f[4];
+    for (int i = 0; i < 4; i++) {
+        f[i] = PyLong_AsVoidPtr(x[i]);
+        if (!f[i]) throw Wrong("an address is wanted");
+    }
+    g_release = reinterpret_cast<decltype(g_release)>(f[0]);
+    g_plan = reinterpret_cast<decltype(g_plan)>(f[1]);
+    g_append = reinterpret_cast<decltype(g_append)>(f[2]);
+    g_attention = reinterpret_cast<decltype(g_attention)>(f[3]);
+    Py_RETURN_NONE;
+}
+
+template <PyObject* (*kCall)(PyObject* const*), int kArgs>
+PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n != kArgs) {
+        PyErr_Format(PyExc_TypeError, "%d arguments are wanted (got %zd)", kArgs, n);
+        return nullptr;
+    }
+    try {
+        return kCall(args);
+    } catch (const Wrong& e) {
+        PyErr_SetString(PyExc_ValueError, e.what());
+    } catch (const Raised&) {
+    } catch (const std::exception& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+    }
+    return nullptr;
+}
+
+template <PyObject* (*kCall)(PyObject* const*), int kArgs>
+PyMethodDef method(const char* name) {
+    return PyMethodDef{name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&entry<kCall, kArgs>)), METH_FASTCALL, nullptr};
+}
+
+PyMethodDef methods[] = {method<use, 4>("use"),           method<release, 10>("release"),     method<plan, 13>("plan"),
+                         method<append, 19>("append"), method<attention, 18>("attention"), {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_paged_bind", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__paged_bind() { return PyModule_Create(&module); }

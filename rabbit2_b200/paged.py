@@ -1,6 +1,7 @@
 """Python binding of the paged KV cache of librbt_moe.so (rbt_paged_*, include/rbt_moe.h).
 
-Plumbing over the C ABI for torch tensors, like moe.py and model.py.  ``PagedTables`` holds a
+Plumbing over the C ABI for torch tensors, like moe.py and model.py; the checks of a step's
+calls are in C++ (csrc/paged_bind.cpp), as these come once per layer.  ``PagedTables`` holds a
 page pool's bookkeeping calls (``release``, ``plan``); ``PagedKv`` adds the caches of one or
 more layers with ``append`` and ``attention``.  A serving step:
 
@@ -20,7 +21,6 @@ from __future__ import annotations
 
 import ctypes as C
 import math
-import struct
 
 import torch
 
@@ -51,12 +51,22 @@ class RbtPagedAttention(C.Structure):
 
 
 _DTYPES = {torch.float32: moe.DT_F32, torch.bfloat16: moe.DT_BF16}
-_I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
-# the argument structs, packed in one call (a ctypes Structure costs a call per field)
-_APPEND = struct.Struct("@QQQqqqiiQQQQfiQQQq")
-_ATTENTION = struct.Struct("@QQQqqiiiQQQiiif")
-assert _APPEND.size == C.sizeof(RbtPagedAppend) and _ATTENTION.size == C.sizeof(RbtPagedAttention)
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_calls = None  # the module of csrc/paged_bind.cpp, once it has been loaded
+
+
+def _bind(lib):
+    """The checks and calls of csrc/paged_bind.cpp, over the given library."""
+    global _calls
+    if _calls is None:
+        try:
+            from rabbit2_b200 import _paged_bind
+        except ImportError as e:
+            raise ImportError(f"rabbit2_b200/_paged_bind.so: {e}; run `make -C rabbit2_b200/csrc bind` "
+                              "(or __graft_entry__.build())") from e
+        _paged_bind.use(*(C.cast(getattr(lib, f"rbt_paged_{f}_device"), C.c_void_p).value
+                          for f in ("release", "plan", "append", "attention")))
+        _calls = _paged_bind
+    return _calls
 
 
 def _want(ok, what):
@@ -64,11 +74,17 @@ def _want(ok, what):
         raise ValueError(what)
 
 
+def _handle(stream):
+    """A stream's address; None stays None, the device's current one."""
+    return stream if stream is None or isinstance(stream, int) else stream.cuda_stream
+
+
 class PagedTables:
     """Block tables of a pool of ``n_pages`` pages of ``page_size`` positions."""
 
     def __init__(self, page_size, n_pages, device=None, *, _cfg=None):
         self.lib = moe.load_library()
+        self.calls = _bind(self.lib)
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         self.page_size, self.n_pages = page_size, n_pages
         cfg = _cfg or RbtPagedConfig(0, 0, 0, 0, page_size, n_pages, 0)
@@ -100,50 +116,18 @@ class PagedTables:
         self._call(self.lib.rbt_paged_status(self.handle, C.byref(v)))
         return v.value
 
-    def _stream(self, stream):
-        if stream is None:
-            return _raw_stream(self.index)
-        return stream if isinstance(stream, int) else stream.cuda_stream
-
-    def _vector(self, t, n, name, dtype=_I32):
-        """Address of a contiguous vector of n values on the pool's GPU (n None: of any length)."""
-        if t.dtype is not dtype or t.get_device() != self.index or t.dim() != 1 or \
-                (n is not None and t.numel() != n) or not t.is_contiguous():
-            raise ValueError(f"{name}: a contiguous {dtype} vector{'' if n is None else f' of {n}'} on {self.device} is "
-                             f"wanted (got {t.dtype} {tuple(t.shape)} on {t.device})")
-        return t.data_ptr()
-
-    def _table(self, t, n):
-        shape = t.shape
-        if t.dtype is not _I32 or t.get_device() != self.index or len(shape) != 2 or shape[0] != n or \
-                not t.is_contiguous():
-            raise ValueError(f"table: contiguous int32 rows for {n} sequences on {self.device} are wanted "
-                             f"(got {t.dtype} {tuple(shape)} on {t.device})")
-        return t.data_ptr(), shape[1]
-
     def release(self, length, done, table, free, n_free, length_out, n_free_out, stream=None):
         """Pages of the sequences with done != 0 back to the end of the free list
         (rbt_paged_release_device)."""
-        n = length.shape[0]
-        tp, ts = self._table(table, n)
-        v = self._vector
-        self._call(self.lib.rbt_paged_release_device(
-            self.handle, n, v(length, n, "length"), v(done, n, "done"), tp, ts, v(free, None, "free"), free.shape[0],
-            v(n_free, 1, "n_free"), v(length_out, n, "length_out"), v(n_free_out, 1, "n_free_out"),
-            self._stream(stream)))
+        self._call(self.calls.release(self.handle, self.index, length, done, table, free, n_free, length_out, n_free_out,
+                                      _handle(stream)))
 
     def plan(self, length, new, table, free, n_free, length_out, n_free_out, cu, slot, pos, stream=None):
         """Pages from the end of the free list for ``new`` tokens of each sequence; their row
         offsets, slots and positions (rbt_paged_plan_device).  Rows of slot/pos past the new
         tokens get slot -1."""
-        n = length.shape[0]
-        tp, ts = self._table(table, n)
-        v = self._vector
-        rows = slot.shape[0]
-        self._call(self.lib.rbt_paged_plan_device(
-            self.handle, n, v(length, n, "length"), v(new, n, "new"), tp, ts, v(free, None, "free"),
-            v(n_free, 1, "n_free"), rows, v(length_out, n, "length_out"), v(n_free_out, 1, "n_free_out"),
-            v(cu, n + 1, "cu"), v(slot, rows, "slot", torch.int64), v(pos, rows, "pos"), self._stream(stream)))
+        self._call(self.calls.plan(self.handle, self.index, length, new, table, free, n_free, length_out, n_free_out, cu,
+                                   slot, pos, _handle(stream)))
 
 
 class PagedKv(PagedTables):
@@ -161,67 +145,25 @@ class PagedKv(PagedTables):
         _want(ks[0].dtype in _DTYPES, f"caches of {ks[0].dtype}: float32 or bfloat16 are wanted")
         self.k, self.v, self.dtype = ks, vs, ks[0].dtype
         self.n_heads, self.n_kv_heads, self.head_dim = n_heads, kvh, hd
-        self.scale = 1.0 / math.sqrt(hd)
+        self.scale, self.code = 1.0 / math.sqrt(hd), _DTYPES[self.dtype]
         super().__init__(page, n_pages, ks[0].device, _cfg=RbtPagedConfig(len(ks), n_heads, kvh, hd, page, n_pages,
-                                                                        _DTYPES[self.dtype]))
+                                                                        self.code))
         for i, (a, b) in enumerate(zip(ks, vs)):
             self._call(self.lib.rbt_paged_bind_layer(self.handle, i, a.data_ptr(), b.data_ptr()))
-
-    def _rows(self, t, heads, n, name, dtype):
-        """Address and row stride of rows [n, heads, head dim] (heads of a row contiguous)."""
-        hd = self.head_dim
-        if t.dtype is not dtype or t.get_device() != self.index or t.shape != (n, heads, hd):
-            raise ValueError(self._rows_wanted(t, heads, n, name, dtype))
-        row, head, one = t.stride()
-        if one != 1 or (head != hd and heads > 1):
-            raise ValueError(self._rows_wanted(t, heads, n, name, dtype))
-        return t.data_ptr(), row if n > 1 else heads * hd
-
-    def _rows_wanted(self, t, heads, n, name, dtype):
-        return (f"{name}: {dtype} rows [{n}, {heads}, {self.head_dim}] on {self.device}, contiguous within a row, are "
-                f"wanted (got {t.dtype} {tuple(t.shape)}, strides {t.stride()}, on {t.device})")
 
     def append(self, q, k, v, slot, pos, q_out, *, cos=None, sin=None, q_norm=None, k_norm=None, eps=1e-5, layer=0,
                stream=None):
         """k and v rows [n, kv heads, head dim] into their slots and q rows into q_out, after the
         whole-projection QK-norm (q_norm, k_norm) and RoPE (cos, sin [positions, head dim / 2])
         where given (rbt_paged_append_device)."""
-        n, dt, v32 = q.shape[0], q.dtype, self._vector
-        src = _DTYPES.get(dt)
-        _want(src is not None, f"q of {dt}: float32 or bfloat16 are wanted")
-        qp, qs = self._rows(q, self.n_heads, n, "q", dt)
-        kp, ks = self._rows(k, self.n_kv_heads, n, "k", dt)
-        vp, vs = self._rows(v, self.n_kv_heads, n, "v", dt)
-        op, os = self._rows(q_out, self.n_heads, n, "q_out", self.dtype)
-        qn = 0 if q_norm is None else v32(q_norm, self.n_heads * self.head_dim, "q_norm", _F32)
-        kn = 0 if k_norm is None else v32(k_norm, self.n_kv_heads * self.head_dim, "k_norm", _F32)
-        cp = sp = angles = 0
-        if cos is not None or sin is not None:
-            _want(cos is not None and sin is not None, "cos and sin must both be given or both be None")
-            for t, name in ((cos, "cos"), (sin, "sin")):
-                _want(t.dtype is _F32 and t.get_device() == self.index and t.shape == cos.shape and t.dim() == 2 and
-                      t.shape[1] * 2 == self.head_dim and t.is_contiguous(),
-                      f"{name}: contiguous float32 [positions, {self.head_dim // 2}] on {self.device} is wanted")
-            cp, sp, angles = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
-        a = _APPEND.pack(qp, kp, vp, qs, ks, vs, src, n, v32(slot, n, "slot", _I64),
-                         0 if pos is None else v32(pos, n, "pos"), qn, kn, eps, angles, cp, sp, op, os)
-        self._call(self.lib.rbt_paged_append_device(self.handle, layer, a, self._stream(stream)))
+        self._call(self.calls.append(self.handle, self.index, self.n_heads, self.n_kv_heads, self.head_dim, self.code,
+                                     layer, q, k, v, slot, pos, q_out, cos, sin, q_norm, k_norm, eps, _handle(stream)))
 
     def attention(self, q, out, cu, length, table, max_new, *, lse=None, causal=True, window=0, scale=None, layer=0,
                   stream=None):
         """out rows [n, heads, head dim] of the q rows' attention over their sequences' pages, and
         the rows' ln sum exp into lse [n, heads] where given (rbt_paged_attention_device).
         max_new: an upper bound of the sequences' new tokens; scale: 1/sqrt(head dim) if None."""
-        n, n_seq = q.shape[0], length.shape[0]
-        qp, qs = self._rows(q, self.n_heads, n, "q", self.dtype)
-        op, os = self._rows(out, self.n_heads, n, "out", self.dtype)
-        lp = 0
-        if lse is not None:
-            _want(lse.dtype is _F32 and lse.get_device() == self.index and lse.shape == (n, self.n_heads) and
-                  lse.is_contiguous(), f"lse: contiguous float32 [{n}, {self.n_heads}] on {self.device} is wanted")
-            lp = lse.data_ptr()
-        tp, ts = self._table(table, n_seq)
-        a = _ATTENTION.pack(qp, op, lp, qs, os, n, n_seq, max_new, self._vector(cu, n_seq + 1, "cu"),
-                            self._vector(length, n_seq, "length"), tp, ts, 1 if causal else 0, window,
-                            self.scale if scale is None else scale)
-        self._call(self.lib.rbt_paged_attention_device(self.handle, layer, a, self._stream(stream)))
+        self._call(self.calls.attention(self.handle, self.index, self.n_heads, self.n_kv_heads, self.head_dim, self.code,
+                                        layer, q, out, cu, length, table, max_new, lse, causal, window,
+                                        self.scale if scale is None else scale, _handle(stream)))

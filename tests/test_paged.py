@@ -52,3 +52,30 @@ def test_structs_match_the_header():
         names = re.findall(r"(\w+)\s*(?=[,;])", body)
         assert names == [f[0] for f in cls._fields_], name
     assert int(re.search(r"RBT_PAGED_MAX_SEQ (\d+)", text).group(1)) == paged.MAX_SEQ
+
+
+def test_the_binding_refuses_tensors_before_it_calls():
+    """The C++ checks on CPU tensors: every one is refused with its name, type, shape and device."""
+    import torch
+    calls = paged._bind(_lib())
+    i = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match=r"length: a contiguous int32 vector of 2 on cuda:0 is wanted \(got int32 \[2\], "
+                                         r"strides \[1\], on cpu\)"):
+        calls.release(None, 0, i, i, i.view(2, 1), i, i, i, i, None)
+    with pytest.raises(ValueError, match="length: a tensor is wanted"):
+        calls.release(None, 0, 3, i, i.view(2, 1), i, i, i, i, None)
+    with pytest.raises(ValueError, match="slot: a vector is wanted"):
+        calls.plan(None, 0, i, i, i.view(2, 1), i, i, i, i, i, torch.tensor(3), i, None)
+    with pytest.raises(TypeError, match="integer"):
+        calls.release(None, "x", i, i, i.view(2, 1), i, i, i, i, None)
+    with pytest.raises(TypeError, match="10 arguments"):
+        calls.release(None)
+    q = torch.zeros(2, 4, 64)
+    with pytest.raises(ValueError, match="q of float64"):
+        calls.append(None, 0, 4, 4, 64, 0, 0, q.double(), q, q, i, i, q, None, None, None, None, 1e-5, None)
+    with pytest.raises(ValueError, match=r"q: float32 rows \[2, 4, 64\] on cuda:0"):
+        calls.append(None, 0, 4, 4, 64, 0, 0, q, q, q, i, i, q, None, None, None, None, 1e-5, None)
+    with pytest.raises(ValueError, match=r"q: bfloat16 rows \[2, 4, 64\] on cuda:0"):
+        calls.attention(None, 0, 4, 4, 64, 1, 0, q, q, i, i, i.view(2, 1), 1, None, True, 0, 1.0, None)
+    with pytest.raises(ValueError, match="q: float32 rows.*not strided"):
+        calls.attention(None, 0, 4, 4, 64, 0, 0, q.to_sparse(), q, i, i, i.view(2, 1), 1, None, True, 0, 1.0, None)
