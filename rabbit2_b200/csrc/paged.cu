@@ -404,8 +404,11 @@ int rbt_paged_attention_device(RbtPaged* p, int layer, const RbtPagedAttention* 
     a.arrived = p->arrived;
     a.status = p->status;
     cudaStream_t s = (cudaStream_t)stream;
-    // Few query rows per kv head: the kernel that streams the cache; more: the tile kernel.
-    // A batch of both kinds takes both, each its own sequences.
+    // Few query rows per kv head: the kernel that streams the cache; more: the tile kernel.  A batch of
+    // both kinds takes both, each its own sequences, unless the tile kernel has few blocks per CTA even
+    // if every sequence fills its table row: then it takes all, and a launch is saved.  One chunk of 40
+    // and the rest single tokens, 3 to 4 kv heads: bf16 31 -> 18.5 us at 0.8 blocks a CTA, 47 -> 37 at
+    // 7.8, 39 to 42 either way at 10.4; f32 51 -> 41 at 1.4, 60 -> 52 at 4.1, but 68 -> 79 at 6.9.
     const bool bf = c.dtype == RBT_MOE_DT_BF16;
     const int few = bf ? kPagedDecRowsBf16 : kPagedDecRowsF32;
     const int64_t most = (int64_t)x.max_new * a.group;
@@ -417,17 +420,21 @@ int rbt_paged_attention_device(RbtPaged* p, int layer, const RbtPagedAttention* 
     if (((int64_t)x.n_rows * a.group / tile + x.n_seq) * (a.most_len / 16 + 1) > INT32_MAX)
         return fail("%d rows over tables of %d positions are too many for one call", x.n_rows, a.most_len);
     const PagedMaps& maps = p->layers[layer].maps;
-    if (most <= few || x.n_seq > 1) {
+    const int ctas = bf ? p->sm_count : 2 * p->sm_count;  // of the tile kernel
+    const int64_t blocks = (a.most_len + paged_tile_block(bf, c.head_dim) - 1) / paged_tile_block(bf, c.head_dim);
+    const bool alone = x.n_seq == 1 || x.n_seq * c.n_kv_heads * blocks <= (int64_t)ctas * (bf ? 8 : 4);
+    if (most <= few || !alone) {
         a.rows_lo = 0;
         a.rows_hi = most <= few ? INT32_MAX : few;
         CU(launch_paged_decode(c.dtype, c.head_dim, dec_rows, maps, a, p->sm_count, s));
     }
     if (most > few) {
-        a.rows_lo = x.n_seq > 1 ? few : 0;
+        a.rows_lo = alone ? 0 : few;
         a.rows_hi = INT32_MAX;
-        if (bf) CU(launch_paged_tc(c.head_dim, maps, a, p->sm_count, s));
-        else CU(launch_paged_rows(c.head_dim, a, 2 * p->sm_count, s));
-        CU(launch_paged_join(c.dtype, c.head_dim, bf ? kPagedTcRows : kPagedF32Rows, a, bf ? p->sm_count : 2 * p->sm_count, s));
+        if (bf) CU(launch_paged_tc(c.head_dim, maps, a, ctas, s));
+        else CU(launch_paged_rows(c.head_dim, a, ctas, s));
+        if (blocks > 1)  // (a tile of one block is never shared)
+            CU(launch_paged_join(c.dtype, c.head_dim, bf ? kPagedTcRows : kPagedF32Rows, a, ctas, s));
     }
     return 1;
 }

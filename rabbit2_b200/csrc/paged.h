@@ -61,6 +61,9 @@ struct PagedAttnArgs {
 constexpr int kPagedDecRowsBf16 = 16, kPagedDecRowsF32 = 8;
 constexpr int kPagedTcRows = 256;  // rows of a unit of the tensor-core kernel (two MMA tiles)
 constexpr int kPagedF32Rows = 64;  // rows of a tile of the f32 kernel for chunks
+constexpr int kPagedTcBlock = 128;  // positions of a block of the tensor-core kernel
+constexpr int paged_rows_block(int hd) { return hd == 64 ? 64 : 32; }  // of the f32 kernel for chunks
+constexpr int paged_tile_block(bool bf16, int hd) { return bf16 ? kPagedTcBlock : paged_rows_block(hd); }
 
 // Tensor maps of one layer's bf16 caches as rows [page][kv head][position] of head_dim.
 struct PagedMaps {

@@ -28,15 +28,16 @@ using namespace paged;
 // bound by the shared-memory reads that feed it (70 % of theirs) and by their latency.  Two CTAs
 // per SM of 4 warps; k and v of the next block are copied while one is computed.  A chunk of
 // 1024, 16 heads of 128: 139 us (0.42 of the f32 FMA rate, 74 TFLOP/s nominal); 5 chunks of
-// up to 333 tokens on up to 1500 cached, 12 heads over 6 of 64: 101 us with its other two
-// launches.  Measured in that order: scalar FMAs 154 and 104; packed 150 and 104; with the
-// next block's copies 144 and 102; with 8 threads to a row instead of 16, 139 and 101.
+// up to 333 tokens on up to 1500 cached, 12 heads over 6 of 64: 84 us with the join.
+// Measured in that order (the second with a launch for few rows, too): scalar FMAs 154 and 104;
+// packed 150 and 104; with the next block's copies 144 and 102; with 8 threads to a row instead
+// of 16, 139 and 101; without that launch 139 and 84.
 constexpr int kRowsThreads = 128;
 
 template <int HD>
 struct RowsCfg {
     static constexpr int kRM = 4, kRows = kPagedF32Rows;
-    static constexpr int kKN = HD == 64 ? 8 : 4, kBlock = 8 * kKN;
+    static constexpr int kBlock = paged_rows_block(HD), kKN = kBlock / 8;
     static constexpr int kLd = HD + 4, kLdP = kBlock + 4;
     static constexpr int kKv = 2 * kBlock * kLd;  // k and v of a block; two blocks are kept
     static constexpr int kFloats = kRows * kLd + 2 * kKv + kRows * kLdP;

@@ -47,7 +47,7 @@ using namespace tc;
 
 constexpr int kTcTile = 128;               // rows of one MMA tile
 constexpr int kTcRows = kPagedTcRows;      // two tiles
-constexpr int kTcBlock = 128;              // positions of a block: one stage of k and v
+constexpr int kTcBlock = kPagedTcBlock;              // positions of a block: one stage of k and v
 constexpr int kTcStep = 64;                // positions of a softmax step
 constexpr int kTcThreads = 352;
 constexpr float kTcRescale = 8.0f;         // log2 of the largest weight before the maximum moves

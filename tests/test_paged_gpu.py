@@ -578,6 +578,24 @@ def test_a_window_beyond_the_table_is_none(dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads, kvh, hd", [(16, 4, 128), (8, 4, 64)])
+@pytest.mark.parametrize("window", [0, 50])
+def test_tables_of_any_width_give_the_same_rows(dtype, heads, kvh, hd, window):
+    """A mixed batch under its own table (one launch for all rows), one wide enough that single
+    tokens and chunks are launched apart, and one of a single block."""
+    seqs = [(0, 1), (300, 1), (37, 90), (0, 0), (513, 2), (90, 300), (20, 5)]
+    b = Batch(seqs, heads, kvh, hd, 16, dtype, seed=8)
+    narrow = b.table
+    for width in (narrow.shape[1], 1000):
+        b.table = torch.full((len(seqs), width), -1, dtype=torch.int32, device="cuda")
+        b.table[:, :narrow.shape[1]] = narrow
+        b.check(window=window)
+    b = Batch([(0, 1), (3, 20), (0, 31), (9, 0)], heads, kvh, hd, 32, dtype, seed=9)
+    b.table = b.table[:, :1].contiguous()
+    b.check(window=window)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_the_last_lengths_of_31_bits_are_refused(dtype):
     from rabbit2_b200.paged import PagedKv
     k = torch.zeros(1, 1, 256, 64, device="cuda", dtype=DT[dtype])
