@@ -16,9 +16,9 @@
 // k and v come by tensor copies in the 128-byte swizzle, so that ldmatrix reads them
 // without bank conflicts, v transposed on the way.
 // 96 single tokens at ragged lengths to 16384, pages of 16, 32 heads over 8 of 128 (3.5 GB):
-// 530 us, 6.6 TB/s, the rate of a plain copy; 64 f32 tokens at 2048 (2.1 GB): 312 us, 6.9 TB/s.
+// 541 us, 6.5 TB/s, the rate of a plain copy; 64 f32 tokens at 2048 (2.1 GB): 312 us, 6.9 TB/s.
 // Short sequences are bound by latency instead, about 5 us a tile (128 sequences to 200
-// positions: 41 us; 16 rows of q, two rounds of blocks, the sums of four warps), a lone token at
+// positions: 37 to 41 us; 16 rows of q, two rounds of blocks, the sums of four warps), a lone token at
 // 4095 with 16 heads by launch, split and join (16.4 us, 2.0 TB/s).
 // f32: products and sums in f32 on the CUDA cores.  Eight lanes share a position (dims
 // jj, jj + 8, ... in 16-byte groups), four positions at a time; the weights go through
@@ -53,6 +53,11 @@ struct DecShape {
 };
 constexpr int kDecStage = 16384;        // bytes: k | v
 constexpr int kDecMinUnits = kDecWarps; // a CTA with less would leave warps idle
+// Tiles of up to as many blocks are not shared (three turns of the four warps; two in f32, whose blocks
+// hold fewer positions): a part given away and added up costs about two turns.  Measured on 60
+// batches of 1 to 500 sequences of 50 to 700 positions, 0.90 of the time (0.56 for one sequence of
+// 300 at head_dim 64, 1.12 at worst); 1 to 2 % is lost where all tiles are long.
+constexpr int kDecKeepBf16 = 12, kDecKeepF32 = 8;
 
 // ---------------------------------------------------------------- both kernels
 template <int kStages>
@@ -74,11 +79,11 @@ __device__ __forceinline__ void ring_init(Ring<kStages>* r) {
 // A producer warp, of k or of v.  copy(id, kvh, off, box, stage, bar) starts the copy of
 // positions [off, off + box rows) of page id into box `box` of its half of the stage (one
 // lane per box).
-template <int kRows, int kBlock, int kStages, typename Copy>
+template <int kRows, int kBlock, int kKeep, int kStages, typename Copy>
 __device__ __forceinline__ void produce(const PagedAttnArgs& a, const Share& share, const Plan& plan, Ring<kStages>* ring,
                                         uint8_t* stages, int box_rows, uint32_t row_bytes, Copy copy) {
     const int lane = threadIdx.x & 31;
-    Walk<kRows, kBlock> w(share, plan);
+    Walk<kRows, kBlock, kKeep> w(share, plan);
     uint32_t j = 0;
     Waiter wait;
 #pragma unroll 1
@@ -312,12 +317,12 @@ __global__ void __launch_bounds__(kDecThreads, DecBf16<HD>::kCtas)
         prefetch_tmap(&tm_k);
         prefetch_tmap(&tm_v);
     }
-    find_share<kDecThreads, C::kRows, KB, kDecMinUnits>(a, plan, &share);  // (its barriers publish the ring's too)
+    find_share<kDecThreads, C::kRows, KB, kDecMinUnits, kDecKeepBf16>(a, plan, &share);  // (its barriers publish the ring's too)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int page = 1 << a.page_shift, box = min(page, KB);
     if (warp >= kDecWarps) {
         const bool is_v = warp > kDecWarps;
-        produce<C::kRows, KB>(a, share, plan, &ring, smem + (is_v ? C::kHalf : 0), box, HD * 2,
+        produce<C::kRows, KB, kDecKeepBf16>(a, share, plan, &ring, smem + (is_v ? C::kHalf : 0), box, HD * 2,
                               [&](int id, int kvh, int off, int i, uint8_t* stage, uint64_t* bar) {
                                   const int y = ((id * a.n_kv + kvh) << a.page_shift) + off;
                                   tma_load_3d(stage + i * box * HD * 2, is_v ? &tm_v : &tm_k, bar, 0, y, 0);
@@ -338,7 +343,7 @@ __global__ void __launch_bounds__(kDecThreads, DecBf16<HD>::kCtas)
 #pragma unroll
     for (int k = 0; k < NT / 2; k++) v_row[k] = C::kHalf + row_at(16 * k + (lane & 15));
     const uint32_t k_swz = ((lane >> 3) ^ (lane & 7)) << 4, v_swz = ((lane >> 4) ^ (lane & 7)) << 4;
-    Walk<C::kRows, KB> w(share, plan);
+    Walk<C::kRows, KB, kDecKeepBf16> w(share, plan);
     uint32_t j = 0;
     Waiter wait;  // (after one that ran out it waits no more: the results are void, the barriers are still met)
 #pragma unroll 1
@@ -516,13 +521,13 @@ __global__ void __launch_bounds__(kDecThreads, DecF32<HD, R>::kCtas) paged_decod
     __shared__ Share share;
     __shared__ int last;
     ring_init(&ring);
-    find_share<kDecThreads, R, KB, kDecMinUnits>(a, plan, &share);
+    find_share<kDecThreads, R, KB, kDecMinUnits, kDecKeepF32>(a, plan, &share);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int page = 1 << a.page_shift, box = min(page, KB);
     if (warp >= kDecWarps) {
         const bool is_v = warp > kDecWarps;
         const float* src = static_cast<const float*>(is_v ? a.v : a.k);
-        produce<R, KB>(a, share, plan, &ring, smem + (is_v ? C::kHalf : 0), box, HD * 4,
+        produce<R, KB, kDecKeepF32>(a, share, plan, &ring, smem + (is_v ? C::kHalf : 0), box, HD * 4,
                        [&](int id, int kvh, int off, int i, uint8_t* stage, uint64_t* bar) {
                            const size_t row = (((size_t)id * a.n_kv + kvh) << a.page_shift) + off;
                            const uint32_t bytes = box * HD * 4;
@@ -533,7 +538,7 @@ __global__ void __launch_bounds__(kDecThreads, DecF32<HD, R>::kCtas) paged_decod
     const int kg = lane >> 3, jj = lane & 7;
     const float k2 = a.scale * kLog2e;
     float* wp = weights + warp * KB * R;
-    Walk<R, KB> w(share, plan);
+    Walk<R, KB, kDecKeepF32> w(share, plan);
     uint32_t j = 0;
     Waiter wait;  // (after one that ran out it waits no more: the results are void, the barriers are still met)
 #pragma unroll 1

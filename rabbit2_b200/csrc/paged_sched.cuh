@@ -217,9 +217,11 @@ __device__ __forceinline__ int scan(int v, int* scratch, int* total) {
 
 // All threads of the CTA call it; share, in shared memory, is valid after the call.  A CTA
 // takes at least kMinUnits units unless there are tiles for more CTAs than that: finer
-// parts of a tile cost more to add up than they save.  The lengths are read here, once;
-// what follows works on shared memory.
-template <int kThreads, int kRows, int kBlock, int kMinUnits>
+// parts of a tile cost more to add up than they save.  For the same reason a tile of up to
+// kKeep units is not shared: the CTA that would have its last unit takes all of it (Walk leaves
+// out a tile that goes on in the next share).  The lengths are read here, once; what follows
+// works on shared memory.
+template <int kThreads, int kRows, int kBlock, int kMinUnits, int kKeep>
 __device__ __forceinline__ void find_share(const PagedAttnArgs& a, const Plan& plan, Share* share) {
     __shared__ int scratch[2][kThreads / 32];
     const int tid = threadIdx.x, n = a.n_seq;
@@ -285,14 +287,20 @@ __device__ __forceinline__ void find_share(const PagedAttnArgs& a, const Plan& p
                 while (plan.starts[i + 1] <= g) i++;
                 Tile t;
                 tile_range<kRows, kBlock>(a, plan.seqs[i], (g - plan.starts[i]) * kRows, t);
-                if (skip < t.nb) break;
+                if (skip < t.nb) {
+                    share->left = sp.start(c + 1) - u0;
+                    if (t.nb <= kKeep) {
+                        share->left += skip;
+                        skip = 0;
+                    }
+                    break;
+                }
                 skip -= t.nb;
             }
             share->split = sp;
             share->tile = g;
             share->kvh = kvh;
             share->skip = skip;
-            share->left = sp.start(c + 1) - u0;
             share->n_tiles = n_tiles;
         }
     }
@@ -300,7 +308,7 @@ __device__ __forceinline__ void find_share(const PagedAttnArgs& a, const Plan& p
 }
 
 // Goes through a share segment by segment: blocks [first, first + n) of tile t.
-template <int kRows, int kBlock>
+template <int kRows, int kBlock, int kKeep>
 struct Walk {
     const Share& share;
     const Plan plan;
@@ -330,7 +338,7 @@ struct Walk {
         left -= n;
         skip = 0;
         tile++;
-        return true;
+        return whole || t.nb > kKeep;  // (a small tile that goes on: the next share begins with it)
     }
     // The CTAs that share the tile of the present segment (a segment that is not the whole tile).
     __device__ __forceinline__ void sharers(int* c0, int* c1) const {
