@@ -374,8 +374,9 @@ RbtMoe *rbt_model_moe(RbtModel *m);
  * graph; the calling thread's current device is left as it was.  Pointers are device
  * pointers on the context's device.  The attention keeps partial results in the
  * context: two attention calls of one context whose kernels overlap on the GPU
- * (unordered streams, two graphs in flight) race on them; create a second context
- * over the same caches for that.  The other calls keep nothing.
+ * (unordered streams, two graphs in flight) race on them, and their results and those
+ * of later calls are void; create a second context over the same caches for that.  The
+ * other calls keep nothing.
  *
  * What only the kernels can see (lengths, pages, slots) is checked there, never
  * followed out of bounds, and leaves a code in the context's status word, which

@@ -251,6 +251,7 @@ __global__ void __launch_bounds__(kJoinRows * HD / 4) paged_join_kernel(const __
         M = mn;
     }
     const int pr = j.row0 + r, tok = pr / a.group, h = j.kvh * a.group + pr - tok * a.group;
+    if (j.tok0 + tok >= a.n_rows) return;  // (only after a call that overlapped this one on the GPU)
     const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;
     T* dst = static_cast<T*>(a.out) + (j.tok0 + tok) * a.out_stride + (size_t)h * HD + d;
     o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);

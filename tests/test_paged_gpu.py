@@ -596,6 +596,75 @@ def test_tables_of_any_width_give_the_same_rows(dtype, heads, kvh, hd, window):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads, kvh", [(512, 1), (100, 2)])
+def test_many_heads_share_a_kv_head(dtype, heads, kvh):
+    Batch([(40, 1), (0, 0), (130, 1)], heads, kvh, 64, 16, dtype, seed=11).check()
+    Batch([(40, 3), (0, 9), (77, 1)], heads, kvh, 64, 16, dtype, seed=12).check(window=20)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_two_contexts_at_once_and_two_graphs_of_one(dtype):
+    from rabbit2_b200.paged import PagedKv
+    b = [Batch([(700, 1), (90, 200), (3, 5)], 8, 2, 64, 16, dtype, seed=21),
+         Batch([(0, 300), (1500, 1)], 8, 2, 64, 16, dtype, seed=22)]
+    want = [x.run()[1:] for x in b]
+    kv = [PagedKv(x.k, x.v, x.heads) for x in b]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in b]
+    outs = [(torch.zeros_like(x.q), torch.zeros(x.n, x.heads, device="cuda")) for x in b]
+    torch.cuda.synchronize()
+    for _ in range(20):  # one by the stream argument, one by the current stream
+        b[0].run(kv[0], *outs[0], stream=streams[0])
+        with torch.cuda.stream(streams[1]):
+            b[1].run(kv[1], *outs[1])
+    torch.cuda.synchronize()
+    for (o, l), (wo, wl), k in zip(outs, want, kv):
+        assert torch.equal(o, wo) and torch.equal(l, wl) and k.status() == 0
+    # two graphs that share a context's partial results, replayed in turn
+    two = Batch([(700, 1), (90, 200), (3, 5)], 8, 2, 64, 16, dtype, seed=21)
+    two.q = two.q.flip(0).contiguous()
+    want2 = two.run(kv[0])[1:]
+    graphs = []
+    for x, o in ((b[0], outs[0]), (two, outs2 := (torch.zeros_like(two.q), torch.zeros(two.n, 8, device="cuda")))):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            x.run(kv[0], *o)
+        graphs.append(g)
+    for o in (outs[0], outs2):
+        for t in o:
+            t.zero_()
+    for _ in range(10):
+        for g in graphs:
+            g.replay()
+    torch.cuda.synchronize()
+    for (o, l), (wo, wl) in ((outs[0], want[0]), (outs2, want2)):
+        assert torch.equal(o, wo) and torch.equal(l, wl)
+    assert kv[0].status() == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_offsets_beyond_32_bits(dtype):
+    """Slots and pages at the end of caches of more than 2^32 elements each."""
+    from rabbit2_b200.paged import PagedKv
+    kvh, page, hd, n_pages, n = 2, 256, 128, 65540, 600
+    kc, vc = (torch.empty(n_pages, kvh, page, hd, device="cuda", dtype=DT[dtype]) for _ in range(2))
+    assert kc.numel() > 1 << 32
+    b = Batch([(n - 1, 1)], 4, kvh, hd, page, dtype, seed=31)
+    k, v = b.dense[0]
+    b.k, b.v, b.table = kc, vc, dev([[n_pages - 1, n_pages - 3, n_pages - 2]])
+    p = torch.arange(n, device="cuda")
+    slot = b.table[0].long()[p // page] * page + p % page
+    kv = PagedKv(kc, vc, b.heads)
+    q = torch.zeros(n, b.heads, hd, device="cuda", dtype=DT[dtype])
+    kv.append(q, k, v, slot, None, torch.empty_like(q))
+    assert torch.equal(kc[n_pages - 1, :, 200], k[200]) and torch.equal(vc[n_pages - 2, :, 87], v[599])
+    b.check()
+    b.seqs, b.rows, b.n = [(n - 40, 40)], [40], 40  # and a chunk
+    b.cu, b.q = dev([0, 40]), torch.randn(40, b.heads, hd, device="cuda").to(DT[dtype])
+    b.check()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_the_last_lengths_of_31_bits_are_refused(dtype):
     from rabbit2_b200.paged import PagedKv
     k = torch.zeros(1, 1, 256, 64, device="cuda", dtype=DT[dtype])
