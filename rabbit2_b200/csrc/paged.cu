@@ -433,7 +433,7 @@ int rbt_paged_attention_device(RbtPaged* p, int layer, const RbtPagedAttention* 
         a.rows_hi = INT32_MAX;
         if (bf) CU(launch_paged_tc(c.head_dim, maps, a, ctas, s));
         else CU(launch_paged_rows(c.head_dim, a, ctas, s));
-        if (blocks > 1)  // (a tile of one block is never shared)
+        if (blocks > (bf ? kPagedTcKeep : 1))  // (else no tile is shared)
             CU(launch_paged_join(c.dtype, c.head_dim, bf ? kPagedTcRows : kPagedF32Rows, a, ctas, s));
     }
     return 1;

@@ -324,10 +324,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tmem_relinquish();
     }
     tc_fence_before();
-    find_share<kTcThreads, kTcRows, kTcBlock, 1, 0>(a, plan, &share);
+    find_share<kTcThreads, kTcRows, kTcBlock, 1, kPagedTcKeep>(a, plan, &share);
     tc_fence_after();
     const uint32_t tmem = bars.tmem;
-    Walk<kTcRows, kTcBlock, 0> w(share, plan);
+    Walk<kTcRows, kTcBlock, kPagedTcKeep> w(share, plan);
     Waiter wait;
 
     if (warp == 10) {
