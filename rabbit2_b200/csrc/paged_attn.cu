@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_rows_kernel(const __gri
     const Plan plan(a, sm + C::kFloats);
     __shared__ Share share;
     const int tid = threadIdx.x, tx = tid & 7, ty = tid >> 3;
-    find_share<kRowsThreads, C::kRows, KB, 4, 0>(a, plan, &share);
+    find_share<kRowsThreads, C::kRows, KB, 4, 0, false>(a, plan, &share);
     Walk<C::kRows, KB, 0> w(share, plan);
     if (tid == 0) a.join[blockIdx.x].last = blockIdx.x;
     const float k2 = a.scale * kLog2e;

@@ -19,7 +19,7 @@
 // 541 us, 6.5 TB/s, the rate of a plain copy; 64 f32 tokens at 2048 (2.1 GB): 312 us, 6.9 TB/s.
 // Short sequences are bound by latency instead, about 5 us a tile (128 sequences to 200
 // positions: 37 to 41 us; 16 rows of q, two rounds of blocks, the sums of four warps), a lone token at
-// 4095 with 16 heads by launch, split and join (16.4 us, 2.0 TB/s).
+// 4095 with 16 heads by launch, split and join (14.4 us, 2.3 TB/s).
 // f32: products and sums in f32 on the CUDA cores.  Eight lanes share a position (dims
 // jj, jj + 8, ... in 16-byte groups), four positions at a time; the weights go through
 // shared memory and each lane keeps its own dims of the output.
@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(kDecThreads, DecBf16<HD>::kCtas)
         prefetch_tmap(&tm_k);
         prefetch_tmap(&tm_v);
     }
-    find_share<kDecThreads, C::kRows, KB, kDecMinUnits, kDecKeepBf16>(a, plan, &share);  // (its barriers publish the ring's too)
+    find_share<kDecThreads, C::kRows, KB, kDecMinUnits, kDecKeepBf16, true>(a, plan, &share);  // (its barriers publish the ring's too)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int page = 1 << a.page_shift, box = min(page, KB);
     if (warp >= kDecWarps) {
@@ -521,7 +521,7 @@ __global__ void __launch_bounds__(kDecThreads, DecF32<HD, R>::kCtas) paged_decod
     __shared__ Share share;
     __shared__ int last;
     ring_init(&ring);
-    find_share<kDecThreads, R, KB, kDecMinUnits, kDecKeepF32>(a, plan, &share);
+    find_share<kDecThreads, R, KB, kDecMinUnits, kDecKeepF32, true>(a, plan, &share);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int page = 1 << a.page_shift, box = min(page, KB);
     if (warp >= kDecWarps) {

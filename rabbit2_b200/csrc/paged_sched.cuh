@@ -221,7 +221,7 @@ __device__ __forceinline__ int scan(int v, int* scratch, int* total) {
 // kKeep units is not shared: the CTA that would have its last unit takes all of it (Walk leaves
 // out a tile that goes on in the next share).  The lengths are read here, once; what follows
 // works on shared memory.
-template <int kThreads, int kRows, int kBlock, int kMinUnits, int kKeep>
+template <int kThreads, int kRows, int kBlock, int kMinUnits, int kKeep, bool kEven>
 __device__ __forceinline__ void find_share(const PagedAttnArgs& a, const Plan& plan, Share* share) {
     __shared__ int scratch[2][kThreads / 32];
     const int tid = threadIdx.x, n = a.n_seq;
@@ -268,6 +268,15 @@ __device__ __forceinline__ void find_share(const PagedAttnArgs& a, const Plan& p
     sp.units = (long long)per_head * a.n_kv;
     const long long most = max((sp.units + kMinUnits - 1) / kMinUnits, (long long)n_tiles * a.n_kv);
     sp.ctas = (int)min((long long)gridDim.x, most);
+    // With tiles of one length a multiple of their number of CTAs shares every tile alike, and no CTA has parts
+    // of two; up to an eighth of the CTAs is given up for it.  63 decode batches of one length: 0.93 of the time
+    // (one token at 2000, 16 heads: 18.5 -> 14.4 us), 35 of mixed lengths 0.99; a sixteenth 0.95, a quarter 0.92
+    // and 1.00.
+    const long long tiles = (long long)n_tiles * a.n_kv;
+    if (kEven && tiles > 0 && tiles < sp.ctas) {
+        const int over = (unsigned)sp.ctas % (unsigned)tiles;
+        if (over <= sp.ctas / 8) sp.ctas -= over;
+    }
     if (c < sp.ctas) {
         if (sp.units < (1ll << 31)) sp.per = (unsigned)sp.units / (unsigned)sp.ctas;
         else sp.per = sp.units / sp.ctas;

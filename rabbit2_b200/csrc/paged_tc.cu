@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tmem_relinquish();
     }
     tc_fence_before();
-    find_share<kTcThreads, kTcRows, kTcBlock, 1, kPagedTcKeep>(a, plan, &share);
+    find_share<kTcThreads, kTcRows, kTcBlock, 1, kPagedTcKeep, false>(a, plan, &share);
     tc_fence_after();
     const uint32_t tmem = bars.tmem;
     Walk<kTcRows, kTcBlock, kPagedTcKeep> w(share, plan);
