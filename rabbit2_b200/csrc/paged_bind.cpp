@@ -235,6 +235,7 @@ PyObject* attention(PyObject* const* x) {
         a.d_lse = c.matrix(x[13], &n, heads, "lse");
     }
     a.causal = PyObject_IsTrue(x[14]);
+    if (a.causal < 0) throw Raised();
     a.window = int32(integer(x[15]), "window");
     a.scale = real(x[16]);
     void* s = c.stream(x[17]);
