@@ -1,7 +1,8 @@
 // paged_bind.cpp -- the checks and calls of rabbit2_b200/paged.py for torch tensors, as an
 // extension module (_paged_bind.so): a step's calls come once per layer and take 4 to 8 us on
 // the GPU when it decodes.  The host takes 4 to 5 us a call, of which the launch is half; the
-// same checks through tensor attributes and ctypes took 7 to 11 us.  The module calls the functions of librbt_moe.so that use() is given.
+// same checks through tensor attributes and ctypes took 7 to 11 us.  The module calls the
+// functions of librbt_moe.so that use() is given.
 #include <Python.h>
 
 #include <ATen/ATen.h>
